@@ -1,0 +1,806 @@
+// Attention over a sliding window with visible first tokens, forward, on tcgen05: for a training step or a prompt
+// (contiguous keys), for the drafted tokens of a serving step (a tree of them over a paged or contiguous cache) and for
+// single next tokens.
+//
+//   o_i = sum_j p_ij v_j,   p_i = softmax over the keys that row i sees of  scale * q_i.k_j   (plus, where a head has a sink
+//   logit, one key of that logit and value 0)
+//
+// Row i stands at position P_i and sees key j when j <= P_i, j is a valid key, and P_i - j < window or j < ns; drafted node n
+// stands at prefix + (number of its ancestors) and sees of the other nodes only those in its 64-bit word.
+//
+// Work of a CTA: 128-row tiles (window_attn.h: g heads x 128 / g queries) against 128-key tiles.
+//
+//   S = Q.K^T       tcgen05.mma 128 x n x 16, fp32 in TMEM (n = the tile's keys, rounded up to 16: the few first tokens and the
+//                   last tile cost what they hold)
+//   P = exp2(S c - m)   one row per thread; read from TMEM, written back over S as bf16: P is the next product's A operand
+//                   and never leaves the tensor memory.  P's rounding to bf16 (half a step, 2^-8) is that of the product's
+//                   operand type; the row's sum is of the unrounded values in fp32.
+//   O += P.V        A from TMEM, V read MN-major in place, accumulator resident in TMEM
+//
+// The running maximum m moves only when a tile exceeds it by 2^8 (numerator and denominator share it, so the result does not
+// depend on when); O is rescaled in TMEM only then.  Two streams (softmax warp group + MMA-issuing warp each) share the CTA so
+// that one stream's products run under the other's exponentials:
+//
+//   ROWS   the streams are two row tiles that share every key tile (long sequences: the bound is the exponentials and the
+//          tensor pipe, so key tiles should be fetched once for as many rows as fit)
+//   KEYS   the streams are the even and odd key tiles of one row tile, joined at the end (<= 128 rows: decode, small trees; the
+//          bound is reading the cache, so the shared memory goes to tiles in flight).  With <= 32 (64) rows the tile holds
+//          them four (two) times in its TMEM lane quarters and each copy takes a quarter (half) of a tile's keys, because a
+//          warp can only read its own quarter of the lanes: otherwise one warp would do all the exponentials.
+//
+// Few row tiles are split over the key axis as well (grid), partial results joined by window_combine_kernel.
+//
+// Rows of V that no row may see (past a sequence's end, padding, pages handed on to others) may hold anything, NaN included:
+// a helper warp zeroes them in shared memory before they are multiplied with P's zeros.
+//
+// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 TMA producer, 9 / 10 MMA of stream 0 / 1, 11 the V helper.  Every wait is
+// bounded (sm100.cuh).
+#include <cstring>
+
+#include "window_attn.h"
+
+namespace cmb {
+
+constexpr int WA_THREADS = 384;
+constexpr float WA_RESCALE = 8.f;        // log2 units a tile's maximum may exceed the reference before O is rescaled
+constexpr int WA_CTL = 3072;             // barriers (first 1 KB), (max, sum) of every row and stream (2 KB)
+
+struct WindowParams {
+  int S, T, H, Hk, g;                    // queries, keys per sequence (cache capacity), heads
+  int box_q;                             // queries in a row tile's TMA box
+  int copies, copy_rows;                 // KEYS: how often a tile holds its rows, and 128 / copies
+  int Dv;
+  float scale_log2;                      // softmax scale * log2(e)
+  int window, ns;
+  int cached;                            // 0: row i at T - S + i, lengths = valid keys (or null); 1: lengths = prefix
+  const int* lengths;
+  const unsigned long long* tree;        // cached: [.., S] words, null = a chain
+  int tree_sb;
+  const int* table;                      // null = contiguous
+  int table_w, page, num_pages, box_k;   // box_k: key rows per TMA box; tiles start at its multiples when paged
+  const float* sinks;                    // [H] or null
+  __nv_bfloat16* out;
+  long long o_sb, o_ss, o_sh;
+  float* lse;                            // [B, H, S] natural log, +inf where a row sees nothing; may be null
+  int splits;
+  float* ws_o;                           // [B, S, H, splits, Dv]
+  float2* ws_ml;                         // [B, S, H, splits] (max, sum)
+  int* status;
+};
+
+template <int DB, bool KEYS>
+struct WindowCfg {
+  static constexpr int Q_BYTES = (KEYS ? 1 : 2) * DB * WA_BLK;
+  static constexpr int NK = DB == 2 ? 3 : 4;
+  static constexpr int NV = DB == 2 ? (KEYS ? 3 : 2) : 4;
+  static constexpr int STAGE = DB * WA_BLK;
+  static constexpr int SMEM_BYTES = Q_BYTES + (NK + NV) * STAGE + WA_CTL;
+  static constexpr int PART_PITCH = DB * 64 + 4;         // floats; rows 16 bytes apart in banks
+  static_assert(SMEM_BYTES <= 232448, "shared memory");
+  static_assert(!KEYS || 256 * PART_PITCH * 4 <= (NK + NV) * STAGE, "partial results reuse the rings");
+  static constexpr int O_COL = 0, S_COL = 256;           // stream s: O at s * 128, S (and P over it) at 256 + s * 128
+};
+
+// One row's place in the problem.
+struct WindowRow {
+  int s, h;                    // query, head
+  bool ok;                     // sees anything at all by construction (in range, not padding)
+  int p, plim, lo;             // position; last key seen by position; first key of its window
+  unsigned long long nodes;    // drafted nodes it sees
+};
+
+__device__ __forceinline__ WindowRow window_row(const WindowParams& p, int r, int s0, int hk, int b, int klim, int prefix) {
+  WindowRow w;
+  const int ql = r / p.g;
+  w.s = s0 + ql;
+  w.h = hk * p.g + (r - ql * p.g);
+  w.ok = ql < p.box_q && w.s < p.S;
+  w.nodes = 0ull;
+  w.p = p.cached ? prefix + w.s : p.T - p.S + w.s;
+  w.plim = min(w.p, klim - 1);
+  if (w.ok && p.tree != nullptr) {
+    const unsigned long long* tree = p.tree + static_cast<long long>(b) * p.tree_sb;
+    const unsigned long long word = tree[w.s];
+    const int depth = __popcll(word) - 1;
+    w.ok = word != 0ull;
+    w.p = prefix + depth;
+    w.plim = prefix - 1;
+    w.nodes = p.S < 64 ? word & ((1ull << p.S) - 1ull) : word;
+    if (p.window <= depth) {                 // the window ends inside the drafted nodes
+      unsigned long long left = w.nodes;
+      while (left) {
+        const int m = __ffsll(static_cast<long long>(left)) - 1;
+        left &= left - 1ull;
+        const int dm = __popcll(tree[m]) - 1;
+        if (!(depth - dm < p.window || prefix + dm < p.ns)) w.nodes &= ~(1ull << m);
+      }
+    }
+  }
+  w.lo = w.p - p.window + 1;
+  return w;
+}
+__device__ __forceinline__ unsigned window_word(const WindowParams& p, const WindowRow& w, int j0, int k1, int prefix) {
+  unsigned bits = wa_mask_word(j0, w.plim, w.lo, p.ns, k1);
+  if (p.tree != nullptr) {
+    const int d = j0 - prefix;
+    if (d > -32 && d < 64) bits |= static_cast<unsigned>(d >= 0 ? w.nodes >> d : w.nodes << (-d));
+    bits &= wa_low_bits(k1 - j0);
+  }
+  return w.ok ? bits : 0u;
+}
+
+template <int DB, bool KEYS>
+__global__ void __launch_bounds__(WA_THREADS, 1)
+window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const WindowParams p) {
+  using Cfg = WindowCfg<DB, KEYS>;
+  constexpr int NK = Cfg::NK, NV = Cfg::NV;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {   // swizzled TMA / MMA tiles need 1024-byte aligned buffers
+    if (threadIdx.x == 0 && p.status != nullptr && atomicCAS(p.status, 0, ST_BAD_ARGUMENT) == 0) p.status[1] = -1024;
+    return;
+  }
+  uint8_t* qs = smem;
+  uint8_t* ks = qs + Cfg::Q_BYTES;
+  uint8_t* vs = ks + NK * Cfg::STAGE;
+  uint8_t* ctl = vs + NV * Cfg::STAGE;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ctl);
+  uint64_t* k_full = q_full + 1;           // [NK]
+  uint64_t* k_empty = k_full + NK;         // [NK]
+  uint64_t* v_full = k_empty + NK;         // [NV] landed
+  uint64_t* v_ready = v_full + NV;         // [NV] unseen rows zeroed
+  uint64_t* v_empty = v_ready + NV;        // [NV]
+  uint64_t* s_full = v_empty + NV;         // [2]
+  uint64_t* p_full = s_full + 2;           // [2]
+  uint64_t* pv_done = p_full + 2;          // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float2* xml = reinterpret_cast<float2*>(ctl + 1024);   // [2 streams][128 rows] (max, sum)
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z / p.splits, split = blockIdx.z - b * p.splits;
+  const int hk = blockIdx.y;
+  const int xt = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);   // longest rows first
+  int* status = p.status;
+
+  // rows and keys of this CTA
+  const int rows_q = (KEYS ? 1 : 2) * p.box_q;                     // queries of the CTA
+  const int s_first = xt * rows_q;
+  const int s_last = min(p.S, s_first + rows_q) - 1;
+  const bool two = KEYS || s_first + p.box_q < p.S;                // is there a second row tile?
+  int prefix = 0, klim, pmin, pmax;
+  if (p.cached) {
+    prefix = max(0, min(p.lengths[b], p.T - p.S));                 // out-of-range prefixes are reported below
+    klim = prefix + p.S;
+    pmin = p.tree != nullptr ? prefix : prefix + s_first;
+    pmax = p.tree != nullptr ? prefix + p.S - 1 : prefix + s_last;
+  } else {
+    klim = p.lengths != nullptr ? max(0, min(p.lengths[b], p.T)) : p.T;
+    pmin = p.T - p.S + s_first;
+    pmax = p.T - p.S + s_last;
+  }
+  const WaRange<128> R(pmin, pmax, klim, p.window, p.ns, p.table != nullptr ? p.box_k : 1);
+  const int per = (R.n_t + p.splits - 1) / p.splits;
+  const int t0 = min(R.n_t, split * per), t1 = min(R.n_t, t0 + per);
+  const int NT = t1 - t0;
+
+  if (threadIdx.x == 0) {
+    const uint32_t readers = !KEYS && two ? 2 : 1;     // MMA warps that read each tile
+    mbar_init(q_full, 1);
+    for (int i = 0; i < NK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], readers);
+    }
+    for (int i = 0; i < NV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_ready[i], 1);
+      mbar_init(&v_empty[i], readers);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&pv_done[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    if (p.lengths != nullptr && status != nullptr) {   // a length that the cache cannot hold
+      const int n = p.lengths[b];
+      if ((n < 0 || n > (p.cached ? p.T - p.S : p.T)) && atomicCAS(status, 0, ST_BAD_ARGUMENT) == 0) {
+        status[1] = b;
+        status[2] = n;
+      }
+    }
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- TMA producer (a box per lane)
+    if (lane == 0) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
+    if (NT > 0) {
+      if (lane == 0) {
+        const uint32_t q_box = p.box_q * p.g * 128;
+        const int nq = KEYS ? p.copies : (two ? 2 : 1);
+        mbar_arrive_expect_tx(q_full, q_box * nq * DB);
+        for (int t = 0; t < nq; ++t)
+          for (int kb = 0; kb < DB; ++kb)
+            tma_load_5d(KEYS ? qs + kb * WA_BLK + t * p.copy_rows * 128 : qs + (t * DB + kb) * WA_BLK, &tmQ, q_full, kb * 64, 0,
+                        KEYS ? s_first : s_first + t * p.box_q, hk, b);
+      }
+      __syncwarp();
+      // lane i moves box i / DB of each tile, column block i % DB; 128 / box_k boxes of <= 2 column blocks fit in 32 lanes
+      // (box_k >= 8).  The page is looked up one tile ahead.
+      const int my_box = lane / DB, my_kb = lane % DB;
+      auto page_of = [&](int i) {
+        if (i >= t1) return 0;
+        const WaTile t = R.tile(i);
+        const int j = t.k0 + my_box * p.box_k;
+        if (j >= t.k1 || p.table == nullptr) return b;
+        int id = p.table[static_cast<long long>(b) * p.table_w + j / p.page];
+        if (id < 0 || id >= p.num_pages) {
+          if (status != nullptr && atomicCAS(status, 0, ST_BAD_ARGUMENT) == 0) {
+            status[1] = b;
+            status[2] = j / p.page;
+            status[3] = id;
+          }
+          id = 0;
+        }
+        return id;
+      };
+      int page = page_of(t0);
+      for (int i = t0; i < t1; ++i) {
+        const int n = i - t0, kst = n % NK, vst = n % NV;
+        const WaTile t = R.tile(i);
+        const int boxes = (t.k1 - t.k0 + p.box_k - 1) / p.box_k;
+        const uint32_t bytes = static_cast<uint32_t>(boxes) * p.box_k * 128 * DB;
+        const int next_page = page_of(i + 1);
+        const int j = t.k0 + my_box * p.box_k;
+        const int in_page = p.table != nullptr ? j % p.page : j;
+        const uint32_t off = my_kb * WA_BLK + my_box * p.box_k * 128;
+        bool ok = true;
+        if (lane == 0) {
+          ok = mbar_wait(&k_empty[kst], ((n / NK) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
+          if (ok) mbar_arrive_expect_tx(&k_full[kst], bytes);
+        }
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        if (my_box < boxes) tma_load_4d(ks + kst * Cfg::STAGE + off, &tmK, &k_full[kst], my_kb * 64, in_page, hk, page);
+        if (lane == 0) {
+          ok = mbar_wait(&v_empty[vst], ((n / NV) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
+          if (ok) mbar_arrive_expect_tx(&v_full[vst], bytes);
+        }
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        if (my_box < boxes) tma_load_4d(vs + vst * Cfg::STAGE + off, &tmV, &v_full[vst], my_kb * 64, in_page, hk, page);
+        page = next_page;
+      }
+    }
+  } else if (warp == 11) {
+    // ---------------------------------------------------------------- V helper: rows that nobody sees become zeros
+    unsigned long long nodes_any = ~0ull;
+    if (p.tree != nullptr) {       // which drafted places hold a node
+      nodes_any = 0ull;
+      const unsigned long long* tree = p.tree + static_cast<long long>(b) * p.tree_sb;
+      for (int m = 0; m < p.S; ++m) nodes_any |= tree[m];
+    }
+    for (int i = t0; i < t1; ++i) {
+      const int n = i - t0, st = n % NV;
+      const WaTile t = R.tile(i);
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(&v_full[st], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL);
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      const bool tail = t.k1 - t.k0 < 128, head = i >= R.n_s && t.k0 < R.wtrue;
+      const bool drafted = p.tree != nullptr && t.k1 > prefix;
+      if (tail || head || drafted) {
+        for (int r = lane; r < 128; r += 32) {
+          const int j = t.k0 + r;
+          const bool seen = j < t.k1 && (j >= R.wtrue || j < p.ns) &&
+                            (!drafted || j < prefix || (j - prefix < 64 && ((nodes_any >> (j - prefix)) & 1ull)));
+          if (!seen) {
+#pragma unroll
+            for (int kb = 0; kb < DB; ++kb)
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(vs + st * Cfg::STAGE + kb * WA_BLK + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_ready[st]);
+    }
+  } else if (warp == 9 || warp == 10) {
+    // ---------------------------------------------------------------- MMA issuer of one stream (one thread)
+    const int st = warp - 9;
+    if (lane == 0 && NT > 0 && (st == 0 || two)) {
+      constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
+      const uint32_t q_addr = smem_u32(qs) + (KEYS ? 0 : st * DB * WA_BLK), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
+      const uint32_t s_col = tmem_base + Cfg::S_COL + st * 128, o_col = tmem_base + Cfg::O_COL + st * 128;
+      bool ok = mbar_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
+      int c = 0;                                       // tiles of this stream so far
+      for (int i = t0 + (KEYS ? st : 0); i < t1 && ok; i += KEYS ? 2 : 1, ++c) {
+        const int n = i - t0, kst = n % NK, vst = n % NV;
+        const WaTile t = R.tile(i);
+        const int k16 = (t.k1 - t.k0 + 15) >> 4;
+        const uint32_t idesc_s = make_idesc(128, k16 * 16, 1, 1, 0, 0);
+        if (!mbar_wait(&k_full[kst], (n / NK) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
+        // S takes the place of the previous tile's P: wait until that product has read it
+        if (c > 0 && !mbar_wait(&pv_done[st], (c - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kb = 0; kb < DB; ++kb)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(s_col, make_smem_desc_sw128(q_addr + kb * WA_BLK + k * 32, 16, 1024),
+                     make_smem_desc_sw128(k_addr + kst * Cfg::STAGE + kb * WA_BLK + k * 32, 16, 1024), idesc_s,
+                     (kb > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&k_empty[kst]);
+        umma_commit(&s_full[st]);
+        if (!mbar_wait(&v_ready[vst], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
+        if (!mbar_wait(&p_full[st], c & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
+        tc_fence_after();
+        for (int k = 0; k < k16; ++k)
+          umma_f16_ts(o_col, s_col + k * 8, make_smem_desc_sw128(v_addr + vst * Cfg::STAGE + k * 2048, WA_BLK, 1024), idesc_o,
+                      (c > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&v_empty[vst]);
+        umma_commit(&pv_done[st]);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax and epilogue (a warp group per stream)
+    const int st = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_addr + Cfg::S_COL + st * 128, o_addr = tmem_base + lane_addr + Cfg::O_COL + st * 128;
+    const bool active = st == 0 || two;
+    const int copy = KEYS ? row / p.copy_rows : 0;
+    const int rr = KEYS ? row - copy * p.copy_rows : row;          // row within the tile
+    const WindowRow w = window_row(p, rr, KEYS ? s_first : s_first + st * p.box_q, hk, b, klim, prefix);
+    const int c_first = KEYS ? copy * (4 / p.copies) : 0;          // this thread's 32-key chunks of a tile
+    const int c_count = KEYS ? 4 / p.copies : 4;
+    const bool warp_ok = __any_sync(0xffffffffu, w.ok);
+    float m_ref = -INFINITY, l_sum = 0.f;
+    bool ok = active;
+    int c = 0;
+    if (active) {
+      for (int i = t0 + (KEYS ? st : 0); i < t1; i += KEYS ? 2 : 1, ++c) {
+        const WaTile t = R.tile(i);
+        const int chunks = (t.k1 - t.k0 + 31) >> 5;                // 32-key chunks that the tile has
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[st], c & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (warp_ok) {
+          uint32_t x0[32], x1[32];
+          auto load = [&](int ch) {          // chunks ch and ch + 1
+            if (ch < chunks) tmem_ld_x32(s_addr + ch * 32, x0);
+            if (c_count > 1 && ch + 1 < chunks) tmem_ld_x32(s_addr + ch * 32 + 32, x1);
+            tmem_wait_ld();
+          };
+          auto masked_max = [&](const uint32_t (&x)[32], unsigned word) {
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (__all_sync(0xffffffffu, word == 0xffffffffu)) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(x[e]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], ((word >> e) & 1u) ? __uint_as_float(x[e]) : -INFINITY);
+            }
+            return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          };
+          unsigned words[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            words[e] = e < c_count && c_first + e < chunks ? window_word(p, w, t.k0 + (c_first + e) * 32, t.k1, prefix) : 0u;
+          float mx = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            if (e < c_count && c_first + e < chunks) {
+              load(c_first + e);
+              mx = fmaxf(mx, masked_max(x0, words[e]));
+              if (c_count > 1 && c_first + e + 1 < chunks) mx = fmaxf(mx, masked_max(x1, words[e + 1]));
+            }
+          }
+          mx *= p.scale_log2;
+          float alpha = 1.f;
+          if (mx > m_ref + WA_RESCALE || (m_ref == -INFINITY && mx > -INFINITY)) {
+            alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
+            m_ref = mx;
+            l_sum *= alpha;
+          }
+          // the scores of tile c were issued after the product of tile c - 1 had completed, so O is free to be rescaled
+          if (c > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+            for (int cc = 0; cc < DB * 2; ++cc) {
+              uint32_t o[32];
+              tmem_ld_x32(o_addr + cc * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st_x32(o_addr + cc * 32, o);
+            }
+          }
+          const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;   // a row without a key yet: exp2(-inf - 0) = 0
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          auto put = [&](const uint32_t (&x)[32], unsigned word, int ch) {
+            uint32_t w16[16];
+            const bool full = __all_sync(0xffffffffu, word == 0xffffffffu);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float a0 = fmaf(__uint_as_float(x[2 * e]), p.scale_log2, neg_m);
+              float a1 = fmaf(__uint_as_float(x[2 * e + 1]), p.scale_log2, neg_m);
+              if (!full) {
+                a0 = ((word >> (2 * e)) & 1u) ? a0 : -INFINITY;
+                a1 = ((word >> (2 * e + 1)) & 1u) ? a1 : -INFINITY;
+              }
+              const float p0 = exp2f(a0), p1 = exp2f(a1);
+              acc[(2 * e) & 3] += p0;
+              acc[(2 * e + 1) & 3] += p1;
+              w16[e] = pack_bf16x2(p0, p1);
+            }
+            tmem_st_x16(s_addr + ch * 16, w16);
+          };
+          // P of chunk ch covers columns 16 ch .. 16 ch + 15 of the scores, all read by now (the row's lane is this thread's)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            if (e < c_count && c_first + e < chunks) {
+              if (c_count > 2) load(c_first + e);
+              put(x0, words[e], c_first + e);
+              if (c_count > 1 && c_first + e + 1 < chunks) put(x1, words[e + 1], c_first + e + 1);
+            }
+          }
+          if (KEYS && p.copies > 1) {        // the other copies' chunks count nothing here
+            uint32_t z[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) z[e] = 0u;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch)
+              if (ch < chunks && (ch < c_first || ch >= c_first + c_count)) tmem_st_x16(s_addr + ch * 16, z);
+          }
+          l_sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(&p_full[st]);
+      }
+      if (c > 0 && ok) ok = mbar_wait(&pv_done[st], (c - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    const float LN2 = 0.6931471805599453f;
+    if (!KEYS) {
+      // -------------------------------------------------------------- ROWS: a thread writes its row
+      if (active && ok) {
+        float inv = 0.f;
+        const bool in = rr / p.g < p.box_q && w.s < p.S;       // a padding node's row is written too (zeros)
+        const long long idx = ((static_cast<long long>(b) * p.S + w.s) * p.H + w.h) * p.splits + split;
+        if (p.splits == 1) {
+          float l = l_sum, m = m_ref, f = 1.f;
+          if (p.sinks != nullptr && in) {
+            const float s2 = p.sinks[w.h] * 1.4426950408889634f;
+            const float top = fmaxf(m, s2);
+            f = m == -INFINITY ? 0.f : exp2f(m - top);
+            l = l * f + exp2f(s2 - top);
+            m = top;
+          }
+          inv = l > 0.f ? f / l : (l == l ? 0.f : l);
+          if (p.lse != nullptr && in)
+            p.lse[(static_cast<long long>(b) * p.H + w.h) * p.S + w.s] = l == 0.f ? INFINITY : (m + log2f(l)) * LN2;
+        } else if (in) {
+          p.ws_ml[idx] = make_float2(m_ref, l_sum);
+        }
+        const bool any = __any_sync(0xffffffffu, w.ok) && c > 0;
+#pragma unroll
+        for (int cc = 0; cc < DB * 2; ++cc) {
+          uint32_t o[32];
+          if (any) {
+            tmem_ld_x32(o_addr + cc * 32, o);
+            tmem_wait_ld();
+          }
+          const bool have = any && w.ok;
+          if (in) {
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+              const int col = cc * 32 + ch * 8;
+              if (col < p.Dv) {
+                float f8[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f8[e] = have ? __uint_as_float(o[8 * ch + e]) : 0.f;
+                if (p.splits == 1) {
+                  uint4 v;
+                  v.x = pack_bf16x2(f8[0] * inv, f8[1] * inv);
+                  v.y = pack_bf16x2(f8[2] * inv, f8[3] * inv);
+                  v.z = pack_bf16x2(f8[4] * inv, f8[5] * inv);
+                  v.w = pack_bf16x2(f8[6] * inv, f8[7] * inv);
+                  *reinterpret_cast<uint4*>(p.out + b * p.o_sb + w.s * p.o_ss + w.h * p.o_sh + col) = v;
+                } else {
+                  float4* dst = reinterpret_cast<float4*>(p.ws_o + idx * p.Dv + col);
+                  dst[0] = make_float4(f8[0], f8[1], f8[2], f8[3]);
+                  dst[1] = make_float4(f8[4], f8[5], f8[6], f8[7]);
+                }
+              }
+            }
+          }
+        }
+      }
+    } else {
+      // -------------------------------------------------------------- KEYS: join the streams and copies, then write
+      // The rings are free: both streams' last products have completed, and they read every tile that was fetched.
+      float* part = reinterpret_cast<float*>(ks);
+      if (c == 0) m_ref = -INFINITY;
+      xml[st * 128 + row] = make_float2(w.ok ? m_ref : -INFINITY, l_sum);
+      if (named_bar_and(1, 256, ok)) {
+        float top = -INFINITY;
+        for (int q = 0; q < 2 * p.copies; ++q) top = fmaxf(top, xml[(q & 1) * 128 + (q >> 1) * p.copy_rows + rr].x);
+        const float wt = w.ok && m_ref > -INFINITY ? exp2f(m_ref - top) : (l_sum == l_sum ? 0.f : l_sum);
+        float* mine = part + (st * 128 + row) * Cfg::PART_PITCH;
+#pragma unroll
+        for (int cc = 0; cc < DB * 2; ++cc) {
+          uint32_t o[32];
+          const bool any = __any_sync(0xffffffffu, wt != 0.f);
+          if (any) {
+            tmem_ld_x32(o_addr + cc * 32, o);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (wt != 0.f)
+              v = make_float4(__uint_as_float(o[4 * ch]) * wt, __uint_as_float(o[4 * ch + 1]) * wt,
+                              __uint_as_float(o[4 * ch + 2]) * wt, __uint_as_float(o[4 * ch + 3]) * wt);
+            *reinterpret_cast<float4*>(mine + cc * 32 + ch * 4) = v;
+          }
+        }
+      }
+      if (named_bar_and(1, 256, ok)) {
+        const int vec = p.Dv / 8;                                  // 16-byte output pieces of a row
+        const int rows = min(p.box_q, p.S - s_first) * p.g;
+        for (int it = threadIdx.x; it < rows * vec; it += 256) {
+          const int r = it / vec, col = (it - r * vec) * 8;
+          float top = -INFINITY, l = 0.f, f8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          for (int q = 0; q < 2 * p.copies; ++q) top = fmaxf(top, xml[(q & 1) * 128 + (q >> 1) * p.copy_rows + r].x);
+          for (int q = 0; q < 2 * p.copies; ++q) {
+            const int pr = (q & 1) * 128 + (q >> 1) * p.copy_rows + r;
+            const float2 ml = xml[pr];
+            l += ml.x > -INFINITY ? ml.y * exp2f(ml.x - top) : (ml.y == ml.y ? 0.f : ml.y);
+            const float4 a = *reinterpret_cast<const float4*>(part + pr * Cfg::PART_PITCH + col);
+            const float4 d = *reinterpret_cast<const float4*>(part + pr * Cfg::PART_PITCH + col + 4);
+            f8[0] += a.x; f8[1] += a.y; f8[2] += a.z; f8[3] += a.w;
+            f8[4] += d.x; f8[5] += d.y; f8[6] += d.z; f8[7] += d.w;
+          }
+          const int ql = r / p.g, s = s_first + ql, h = hk * p.g + (r - ql * p.g);
+          if (p.splits == 1) {
+            float m = top, f = 1.f;
+            if (p.sinks != nullptr) {
+              const float s2 = p.sinks[h] * 1.4426950408889634f;
+              const float t2 = fmaxf(m, s2);
+              f = m == -INFINITY ? 0.f : exp2f(m - t2);
+              l = l * f + exp2f(s2 - t2);
+              m = t2;
+            }
+            const float inv = l > 0.f ? f / l : (l == l ? 0.f : l);
+            uint4 v;
+            v.x = pack_bf16x2(f8[0] * inv, f8[1] * inv);
+            v.y = pack_bf16x2(f8[2] * inv, f8[3] * inv);
+            v.z = pack_bf16x2(f8[4] * inv, f8[5] * inv);
+            v.w = pack_bf16x2(f8[6] * inv, f8[7] * inv);
+            *reinterpret_cast<uint4*>(p.out + b * p.o_sb + s * p.o_ss + h * p.o_sh + col) = v;
+            if (p.lse != nullptr && col == 0)
+              p.lse[(static_cast<long long>(b) * p.H + h) * p.S + s] = l == 0.f ? INFINITY : (m + log2f(l)) * LN2;
+          } else {
+            const long long idx = ((static_cast<long long>(b) * p.S + s) * p.H + h) * p.splits + split;
+            float4* dst = reinterpret_cast<float4*>(p.ws_o + idx * p.Dv + col);
+            dst[0] = make_float4(f8[0], f8[1], f8[2], f8[3]);
+            dst[1] = make_float4(f8[4], f8[5], f8[6], f8[7]);
+            if (col == 0) p.ws_ml[idx] = make_float2(top, l);
+          }
+        }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  __syncwarp();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);   // bounded grace period for copies / MMAs still in flight
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Joins the splits of a row: a warp per (sequence, query, head), four output columns per lane.
+struct CombineParams {
+  int S, H, splits, Dv;
+  long long rows;
+  const float* ws_o;
+  const float2* ws_ml;
+  const float* sinks;
+  __nv_bfloat16* out;
+  long long o_sb, o_ss, o_sh;
+  float* lse;
+};
+__global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams p) {
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const int lane = threadIdx.x & 31;
+  const int h = static_cast<int>(row % p.H);
+  const long long bs = row / p.H;
+  const int s = static_cast<int>(bs % p.S);
+  const long long b = bs / p.S;
+  const float2* ml = p.ws_ml + row * p.splits;
+  float top = -INFINITY;
+  for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, ml[i].x);
+  top = warp_max(top);
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < p.splits; ++i) {
+    const float2 v = ml[i];
+    const float wt = v.x > -INFINITY ? exp2f(v.x - top) : (v.y == v.y ? 0.f : v.y);
+    if (wt != 0.f) {
+      l += v.y * wt;
+      if (lane * 4 < p.Dv) {
+        const float4 a = *reinterpret_cast<const float4*>(p.ws_o + (row * p.splits + i) * p.Dv + lane * 4);
+        o.x = fmaf(a.x, wt, o.x);
+        o.y = fmaf(a.y, wt, o.y);
+        o.z = fmaf(a.z, wt, o.z);
+        o.w = fmaf(a.w, wt, o.w);
+      }
+    }
+  }
+  float f = 1.f;
+  if (p.sinks != nullptr) {
+    const float s2 = p.sinks[h] * 1.4426950408889634f;
+    const float t2 = fmaxf(top, s2);
+    f = top == -INFINITY ? 0.f : exp2f(top - t2);
+    l = l * f + exp2f(s2 - t2);
+    top = t2;
+  }
+  const float inv = l > 0.f ? f / l : (l == l ? 0.f : l);
+  if (lane * 4 < p.Dv)
+    *reinterpret_cast<uint2*>(p.out + b * p.o_sb + s * p.o_ss + h * p.o_sh + lane * 4) =
+        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  if (p.lse != nullptr && lane == 0) p.lse[(b * p.H + h) * p.S + s] = l == 0.f ? INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace cmb
+
+namespace cmb_host {
+
+int make_tmap_rows(CUtensorMap* out, const void* base, int D, long long rows, int heads, long long outer, long long s_row,
+                   long long s_head, long long s_outer, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return 101;
+  bind_context_once();
+  if (reinterpret_cast<uintptr_t>(base) & 15) return 102;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(outer)};
+  // the stride of a dimension of size 1 is never used, but has to be a positive multiple of 16 bytes
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(rows > 1 ? s_row : 8) * 2, static_cast<cuuint64_t>(heads > 1 ? s_head : 8) * 2,
+                           static_cast<cuuint64_t>(outer > 1 ? s_outer : 8) * 2};
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] == 0 || (strides[i] & 15) || strides[i] >= (1ull << 40)) return 105;
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 1000 + static_cast<int>(r);
+}
+
+int make_tmap_grouped(CUtensorMap* out, const void* base, int D, int S, int Hk, int g, int Bn, long long s_row, long long s_head,
+                      long long s_batch, int box_q) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return 101;
+  bind_context_once();
+  if (reinterpret_cast<uintptr_t>(base) & 15) return 102;
+  cuuint64_t dims[5] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(g), static_cast<cuuint64_t>(S),
+                        static_cast<cuuint64_t>(Hk), static_cast<cuuint64_t>(Bn)};
+  cuuint64_t strides[4] = {static_cast<cuuint64_t>(g > 1 ? s_head : 8) * 2, static_cast<cuuint64_t>(S > 1 ? s_row : 8) * 2,
+                           static_cast<cuuint64_t>(Hk > 1 ? s_head * g : 8) * 2, static_cast<cuuint64_t>(Bn > 1 ? s_batch : 8) * 2};
+  for (int i = 0; i < 4; ++i)
+    if (strides[i] == 0 || (strides[i] & 15) || strides[i] >= (1ull << 40)) return 105;
+  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(g), static_cast<cuuint32_t>(box_q), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 1000 + static_cast<int>(r);
+}
+
+}  // namespace cmb_host
+
+namespace {
+
+template <int DB, bool KEYS>
+int launch_window_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const cmb::WindowParams& p, int B,
+                      cudaStream_t stream) {
+  using Cfg = cmb::WindowCfg<DB, KEYS>;
+  auto kern = cmb::window_fwd_kernel<DB, KEYS>;
+  static std::atomic<unsigned long long> attr_done{0};
+  if (cmb_host::set_smem_limit_once_per_device(attr_done, reinterpret_cast<const void*>(kern), Cfg::SMEM_BYTES)) return 103;
+  const int per = (KEYS ? 1 : 2) * p.box_q;
+  dim3 grid((p.S + per - 1) / per, p.Hk, B * p.splits);
+  kern<<<grid, cmb::WA_THREADS, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : 104;
+}
+
+}  // namespace
+
+// q [B,S,H,Dq]; k / v rows [outer, rows, Hk, Dq | Dv] with outer = B (contiguous, rows = T) or pages of a pool (table
+// [B, table_w], rows = page size); bf16 with unit inner stride.  Dq, Dv <= 128 and multiples of 8; H / Hk <= 128.
+// ip = {B, S, T, H, Hk, Dq, Dv, window, ns, cached, tree_sb, table_w, page, num_pages, box_k, splits};
+// lp = {q_sb, q_ss, q_sh, k_outer, k_row, k_head, v_outer, v_row, v_head, o_sb, o_ss, o_sh}.
+// ws_o / ws_ml are needed for splits > 1 only.  Returns 0, 1 for arguments that the kernel does not cover.
+extern "C" int cmb_window_fwd(const void* q, const void* k, const void* v, const int* lengths, const void* tree, const int* table,
+                              const float* sinks, void* out, float* lse, float* ws_o, float* ws_ml, const int* ip,
+                              const long long* lp, float scale, int* status, void* stream) {
+  cmb::WindowParams p{};
+  const int B = ip[0], Dq = ip[5];
+  p.S = ip[1]; p.T = ip[2]; p.H = ip[3]; p.Hk = ip[4]; p.Dv = ip[6];
+  p.window = ip[7]; p.ns = ip[8]; p.cached = ip[9];
+  p.tree = static_cast<const unsigned long long*>(tree); p.tree_sb = ip[10];
+  p.table = table; p.table_w = ip[11]; p.page = ip[12]; p.num_pages = ip[13]; p.box_k = ip[14];
+  p.splits = ip[15];
+  if (B <= 0 || p.S <= 0 || p.Hk <= 0 || p.H <= 0 || p.H % p.Hk || p.T < 0 || p.splits < 1) return 1;
+  p.g = p.H / p.Hk;
+  if (p.g > 128 || p.Hk > 65535 || static_cast<long long>(B) * p.splits > 65535) return 1;
+  if (Dq <= 0 || Dq > 128 || Dq % 8 || p.Dv <= 0 || p.Dv > 128 || p.Dv % 8) return 1;
+  if (p.window < 1 || p.window > cmb::WA_NO_WINDOW || p.ns < 0 || !(scale > 0.f)) return 1;
+  if (p.cached && (lengths == nullptr || p.T < p.S)) return 1;
+  if (!p.cached && (p.tree != nullptr || table != nullptr || p.T < p.S)) return 1;
+  if (p.tree != nullptr && p.S > 64) return 1;
+  if (p.box_k != 8 && p.box_k != 16 && p.box_k != 32 && p.box_k != 64 && p.box_k != 128) return 1;
+  if (table != nullptr && (p.page <= 0 || p.page % p.box_k || p.num_pages <= 0 || p.table_w <= 0 ||
+                           static_cast<long long>(p.table_w) * p.page < p.T))
+    return 1;
+  if (p.splits > 1 && (ws_o == nullptr || ws_ml == nullptr)) return 1;
+  if ((lp[9] | lp[10] | lp[11]) & 7 || (reinterpret_cast<uintptr_t>(out) & 15)) return 1;
+  const int rows = p.S * p.g;                              // S <= 2^24 rows is checked by the caller's shapes
+  const bool keys = rows <= 128;
+  p.copies = 1;
+  if (keys) {
+    p.box_q = p.S;
+    p.copies = rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
+  } else {
+    p.box_q = 128 / p.g < p.S ? 128 / p.g : p.S;
+  }
+  p.copy_rows = 128 / p.copies;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.lengths = lengths; p.sinks = sinks;
+  p.out = static_cast<__nv_bfloat16*>(out); p.o_sb = lp[9]; p.o_ss = lp[10]; p.o_sh = lp[11];
+  p.lse = lse; p.ws_o = ws_o; p.ws_ml = reinterpret_cast<float2*>(ws_ml); p.status = status;
+  CUtensorMap tq, tk, tv;
+  int rc = cmb_host::make_tmap_grouped(&tq, q, Dq, p.S, p.Hk, p.g, B, lp[1], lp[2], lp[0], p.box_q);
+  if (rc) return rc;
+  const long long krows = table != nullptr ? p.page : p.T, outer = table != nullptr ? p.num_pages : B;
+  rc = cmb_host::make_tmap_rows(&tk, k, Dq, krows, p.Hk, outer, lp[4], lp[5], lp[3], p.box_k);
+  if (rc) return rc + 10000;
+  rc = cmb_host::make_tmap_rows(&tv, v, p.Dv, krows, p.Hk, outer, lp[7], lp[8], lp[6], p.box_k);
+  if (rc) return rc + 20000;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool wide = Dq > 64 || p.Dv > 64;
+  if (wide) rc = keys ? launch_window_fwd<2, true>(tq, tk, tv, p, B, st) : launch_window_fwd<2, false>(tq, tk, tv, p, B, st);
+  else rc = keys ? launch_window_fwd<1, true>(tq, tk, tv, p, B, st) : launch_window_fwd<1, false>(tq, tk, tv, p, B, st);
+  if (rc || p.splits == 1) return rc;
+  cmb::CombineParams c{};
+  c.S = p.S; c.H = p.H; c.splits = p.splits; c.Dv = p.Dv;
+  c.rows = static_cast<long long>(B) * p.S * p.H;
+  c.ws_o = ws_o; c.ws_ml = p.ws_ml; c.sinks = sinks;
+  c.out = p.out; c.o_sb = p.o_sb; c.o_ss = p.o_ss; c.o_sh = p.o_sh; c.lse = lse;
+  const long long blocks = (c.rows + 3) / 4;
+  if (blocks > 0x7fffffffll) return 1;
+  cmb::window_combine_kernel<<<static_cast<unsigned>(blocks), 128, 0, st>>>(c);
+  return cudaGetLastError() == cudaSuccess ? 0 : 104;
+}

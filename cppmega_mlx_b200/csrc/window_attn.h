@@ -1,0 +1,97 @@
+// Shared by the forward and backward kernels of windowed attention (window_attn.cu, window_attn_bwd.cu): which keys a query
+// sees, and how query rows are packed into tiles.
+//
+// A row tile holds 128 / g consecutive queries of one key/value head, each with the g query heads that share that head
+// (row = query * g + head of the group): grouped heads read a key tile once, and for g > 1 a tile spans few positions, so
+// little of a window's edge is masked work.
+#pragma once
+#include "sm100.cuh"
+
+namespace cmb {
+
+constexpr int WA_BLK = 128 * 128;            // bytes of one [128 rows x 64 bf16] block
+constexpr int WA_NO_WINDOW = 1 << 30;
+
+// Keys [k0, k1) of one tile.
+struct WaTile {
+  int k0, k1;
+};
+
+// The key tiles of a block of rows whose positions lie in [pmin, pmax]: the visible first tokens [0, send), then the window
+// [wlo, kend), BN keys a tile.  Keys of the two ranges are disjoint.
+template <int BN>
+struct WaRange {
+  int wtrue;         // first key inside any row's window
+  int wlo;           // where the window's tiles start (wtrue rounded down to a whole box of rows)
+  int send, kend, n_s, n_t;
+  __host__ __device__ WaRange(int pmin, int pmax, int klim, int window, int ns, int align) {
+    wtrue = pmin - window + 1;
+    if (wtrue < 0) wtrue = 0;
+    wlo = wtrue - wtrue % align;
+    kend = pmax + 1 < klim ? pmax + 1 : klim;
+    if (kend < 0) kend = 0;
+    send = ns < wlo ? ns : wlo;
+    if (send > klim) send = klim;
+    if (send < 0) send = 0;
+    n_s = (send + BN - 1) / BN;
+    n_t = n_s + (kend > wlo ? (kend - wlo + BN - 1) / BN : 0);
+  }
+  __host__ __device__ WaTile tile(int i) const {
+    WaTile t;
+    t.k0 = i < n_s ? BN * i : wlo + BN * (i - n_s);
+    const int end = i < n_s ? send : kend;
+    t.k1 = t.k0 + BN < end ? t.k0 + BN : end;
+    return t;
+  }
+};
+
+// Bits of the 32 keys j0 .. j0 + 31 that a row sees: j <= plim, and j >= lo (its window) or j < ns (a visible first token),
+// and j < k1 (the tile's end; may exceed j0 + 31).
+__device__ __forceinline__ unsigned wa_low_bits(int n) {   // the n lowest bits, any n
+  return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+}
+__device__ __forceinline__ unsigned wa_mask_word(int j0, int plim, int lo, int ns, int k1) {
+  const unsigned upto = wa_low_bits(min(plim + 1, k1) - j0);
+  return upto & (~wa_low_bits(lo - j0) | wa_low_bits(ns - j0));
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]; bf16 inputs (A two to a 32-bit column), fp32 accumulate. One thread issues.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2, int c3,
+                                            int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
+      "r"(c4)
+      : "memory");
+}
+
+}  // namespace cmb
+
+namespace cmb_host {
+
+// Key / value rows: [outer, rows, heads, D] with unit inner stride and any other strides that are multiples of 8 elements
+// (outer = batch of a contiguous cache, or page of a pool); box of `box_rows` rows x 64 columns.  Columns past D read as 0.
+int make_tmap_rows(CUtensorMap* out, const void* base, int D, long long rows, int heads, long long outer, long long s_row,
+                   long long s_head, long long s_outer, int box_rows);
+// Query-side rows [B, S, H = Hk * g, D] as (D, g, S, Hk, B); box of `box_q` queries x g heads x 64 columns.
+int make_tmap_grouped(CUtensorMap* out, const void* base, int D, int S, int Hk, int g, int Bn, long long s_row, long long s_head,
+                      long long s_batch, int box_q);
+
+}  // namespace cmb_host

@@ -1,0 +1,596 @@
+// Backward of windowed attention (window_attn.cu) on tcgen05: three launches (and a join where the first tokens' keys were
+// split), no atomics and no S x T tensor.
+//
+//   delta_i = do_i . o_i                                     window_stats_kernel
+//   P = exp2(S c - lse2),  dS = P o (dO V^T - delta)         recomputed in both of:
+//   DKV  CTA = 128 keys of one (sequence, key head); streams the rows that may see them, 64 at a time (64 / g queries x g heads,
+//        so a group's heads are summed on chip).  Lanes are keys:  S^T = K Q^T,  dP^T = V dO^T  ->  dV += P^T dO,  dK += dS^T Q
+//   DQ   CTA = 128 rows (128 / g queries x g heads); streams the keys that they see, 64 at a time.  Lanes are rows:
+//        S = Q K^T,  dP = dO V^T  ->  dQ += dS K
+//
+// The sinks' gradient, -sum_i p_i,sink (do_i . o_i), would feel the rounding of o to bf16 (the sum has few outputs and both signs), so
+// DQ adds up do_i . o_i = sum_j p_ij dP_ij itself, in fp32, where sinks are trained.
+//
+// dK and dQ carry the softmax scale once, at the end.  P and dS are rounded to bf16 (half a step, 2^-8: the operand type of the
+// gradient products) and written back over S and dP in TMEM, where they are the A operands; dQ, dK, dV accumulate there in fp32.
+// One thread issues every product in order; two warp groups take alternate sub-tiles, so that one's exponentials run under
+// the other's products.  64-wide sub-tiles, because two of {S, dP} and the accumulators have to fit the 512 TMEM columns.
+//
+// The first tokens are seen by every later row: their key tiles would run S / (64 / g) sub-tiles where another runs about
+// (window + 128) / (64 / g).  Their rows are split over CTAs, fp32 partial results are summed in a fixed order by window_join_kernel.
+//
+// A key that no row sees may hold anything: K rows of no row of the tile are zeroed in shared memory before dQ's product.
+#include "window_attn.h"
+
+namespace cmb {
+
+enum : int { WB_DQ = 0, WB_DKV = 1 };
+constexpr int WB_THREADS = 352;            // warps 0-3 / 4-7 elements, 8 TMA, 9 MMA, 10 helper
+constexpr int WB_SUB = 64;
+constexpr int WB_SBLK = WB_SUB * 128;      // bytes of a [64 rows x 64 bf16] block
+constexpr int WB_NS = 4;                   // sub-tiles in flight
+
+struct WindowBwdParams {
+  int S, T, H, Hk, g, Dq, Dv;
+  int box_q;                               // queries of a 128-row tile (DQ)
+  int sub_q;                               // queries of a 64-row sub-tile (DKV)
+  float scale, scale_log2;
+  int window, ns;
+  const int* lengths;
+  const float2* stats;                     // [B, Hk, S * g] (lse * log2 e, delta) of packed rows; lse = +inf: sees nothing
+  __nv_bfloat16 *o1, *o2;                  // DQ: dq, -;  DKV: dk, dv
+  long long o1_sb, o1_ss, o1_sh, o2_sb, o2_ss, o2_sh;
+  int sink_tiles, sink_splits;             // DKV: the first sink_tiles key tiles are split
+  float* part;                             // [B, Hk, sink_tiles, sink_splits, 128, Dq + Dv]
+  const float* sinks;                      // [H], for SINKS
+  float* sink_part;                        // [H, B * row tiles]
+  int* status;
+};
+
+template <int DB>
+struct WindowBwdCfg {
+  static constexpr int R_BYTES = 2 * DB * WA_BLK;               // resident pair of operands
+  static constexpr int STAGE = 2 * DB * WB_SBLK;
+  static constexpr int CTL = 1024 + WB_NS * WB_SUB * 8;        // barriers; row statistics of the stages, then the rows' sums (SINKS)
+  static constexpr int SMEM_BYTES = R_BYTES + WB_NS * STAGE + CTL;
+  static constexpr int X_COL = 0;                               // buffer i: S at 128 i, dP at 128 i + 64
+  static constexpr int O1_COL = 256, O2_COL = 384;
+  static_assert(SMEM_BYTES <= 232448, "shared memory");
+};
+
+template <int MODE, int DB, bool SINKS>
+__global__ void __launch_bounds__(WB_THREADS, 1)
+window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constant__ CUtensorMap tmR2,
+                  const __grid_constant__ CUtensorMap tmT1, const __grid_constant__ CUtensorMap tmT2, const WindowBwdParams p) {
+  using Cfg = WindowBwdCfg<DB>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0 && p.status != nullptr && atomicCAS(p.status, 0, ST_BAD_ARGUMENT) == 0) p.status[1] = -1024;
+    return;
+  }
+  uint8_t* r1s = smem;
+  uint8_t* r2s = r1s + DB * WA_BLK;
+  uint8_t* ts = r2s + DB * WA_BLK;
+  uint8_t* ctl = ts + WB_NS * Cfg::STAGE;
+  uint64_t* r_full = reinterpret_cast<uint64_t*>(ctl);
+  uint64_t* t_full = r_full + 1;             // [WB_NS] landed
+  uint64_t* t_ready = t_full + WB_NS;        // [WB_NS] cleaned, row statistics fetched
+  uint64_t* t_empty = t_ready + WB_NS;       // [WB_NS]
+  uint64_t* x_full = t_empty + WB_NS;        // [2] scores
+  uint64_t* a_full = x_full + 2;             // [2] P, dS written
+  uint64_t* g_done = a_full + 2;             // [2] gradient products
+  uint64_t* all_done = g_done + 2;           // every product (a phase bit of g_done could not tell the last from one two earlier)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float2* aux = reinterpret_cast<float2*>(ctl + 1024);          // [WB_NS][64]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int off = p.T - p.S;                                    // position of query 0
+  const int klim = p.lengths != nullptr ? max(0, min(p.lengths[b], p.T)) : p.T;
+  int* status = p.status;
+
+  // ---- what this CTA holds and what it streams
+  int row0, n_first, NT, split = -1, key_tile = 0;
+  const int xr = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);
+  const int s_first = MODE == WB_DQ ? xr * p.box_q : 0;         // DQ: the last queries first (without a window they see most)
+  const WaRange<64> R(off + s_first, off + min(p.S, s_first + p.box_q) - 1, klim, p.window, p.ns, 1);
+  const int used = p.sub_q * p.g;                               // rows of a sub-tile (DKV)
+  if (MODE == WB_DQ) {
+    row0 = s_first;
+    n_first = 0;
+    NT = R.n_t;
+  } else {
+    int part = 0, parts = 1;
+    const int x = blockIdx.x, n_split = p.sink_tiles * p.sink_splits;
+    if (x < n_split) {
+      key_tile = x / p.sink_splits;
+      part = x - key_tile * p.sink_splits;
+      parts = p.sink_splits;
+      split = p.sink_splits > 1 ? part : -1;
+    } else {
+      key_tile = p.sink_tiles + (x - n_split);
+    }
+    row0 = key_tile * 128;
+    const int k_last = min(row0 + 127, klim - 1);
+    const int q_lo = max(0, row0 - off);
+    const int q_hi = row0 < p.ns ? p.S : min(p.S, k_last - off + p.window);      // exclusive
+    const bool any = k_last >= row0 && q_hi > q_lo;
+    const int sub_lo = q_lo / p.sub_q, sub_n = any ? (q_hi + p.sub_q - 1) / p.sub_q - sub_lo : 0;
+    const int per = (sub_n + parts - 1) / parts;
+    n_first = sub_lo + min(sub_n, part * per);
+    NT = min(sub_n, (part + 1) * per) - min(sub_n, part * per);
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(r_full, 1);
+    for (int i = 0; i < WB_NS; ++i) {
+      mbar_init(&t_full[i], 1);
+      mbar_init(&t_ready[i], 1);
+      mbar_init(&t_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&x_full[i], 1);
+      mbar_init(&a_full[i], 128);
+      mbar_init(&g_done[i], 1);
+    }
+    mbar_init(all_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmR1);
+    tma_prefetch_desc(&tmR2);
+    tma_prefetch_desc(&tmT1);
+    tma_prefetch_desc(&tmT2);
+  }
+  if (MODE == WB_DKV && used < WB_SUB) {     // rows of a sub-tile that no copy fills are multiplied with zeros: no NaN there
+    const int rows = WB_SUB - used;
+    for (int i = threadIdx.x; i < WB_NS * 2 * DB * rows * 8; i += WB_THREADS) {
+      const int c = i & 7, r = (i >> 3) % rows, blk = (i >> 3) / rows;
+      *reinterpret_cast<uint4*>(ts + blk * WB_SBLK + (used + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0 && NT > 0) {
+      const uint32_t r_bytes = (MODE == WB_DQ ? p.box_q * p.g : 128) * 128;
+      mbar_arrive_expect_tx(r_full, 2 * DB * r_bytes);
+      for (int kb = 0; kb < DB; ++kb) {
+        if (MODE == WB_DQ) {
+          tma_load_5d(r1s + kb * WA_BLK, &tmR1, r_full, kb * 64, 0, row0, hk, b);
+          tma_load_5d(r2s + kb * WA_BLK, &tmR2, r_full, kb * 64, 0, row0, hk, b);
+        } else {
+          tma_load_4d(r1s + kb * WA_BLK, &tmR1, r_full, kb * 64, row0, hk, b);
+          tma_load_4d(r2s + kb * WA_BLK, &tmR2, r_full, kb * 64, row0, hk, b);
+        }
+      }
+      const uint32_t t_bytes = (MODE == WB_DQ ? WB_SUB : used) * 128;
+      for (int n = 0; n < NT; ++n) {
+        const int st = n % WB_NS;
+        if (!mbar_wait(&t_empty[st], ((n / WB_NS) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY)) break;
+        mbar_arrive_expect_tx(&t_full[st], 2 * DB * t_bytes);
+        uint8_t* t1 = ts + st * Cfg::STAGE;
+        uint8_t* t2 = t1 + DB * WB_SBLK;
+        for (int kb = 0; kb < DB; ++kb) {
+          if (MODE == WB_DQ) {
+            const int k0 = R.tile(n).k0;
+            tma_load_4d(t1 + kb * WB_SBLK, &tmT1, &t_full[st], kb * 64, k0, hk, b);
+            tma_load_4d(t2 + kb * WB_SBLK, &tmT2, &t_full[st], kb * 64, k0, hk, b);
+          } else {
+            tma_load_5d(t1 + kb * WB_SBLK, &tmT1, &t_full[st], kb * 64, 0, (n_first + n) * p.sub_q, hk, b);
+            tma_load_5d(t2 + kb * WB_SBLK, &tmT2, &t_full[st], kb * 64, 0, (n_first + n) * p.sub_q, hk, b);
+          }
+        }
+      }
+    }
+  } else if (warp == 10) {
+    // ---------------------------------------------------------------- helper: row statistics, keys that nobody sees
+    const long long rows = static_cast<long long>(p.S) * p.g;
+    const float2* stats = p.stats + (static_cast<long long>(b) * p.Hk + hk) * rows;
+    for (int n = 0; n < NT; ++n) {
+      const int st = n % WB_NS;
+      bool ok = true;
+      float2 v[2];
+      if (MODE == WB_DKV) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = lane + 32 * i;
+          const long long r = static_cast<long long>(n_first + n) * used + c;
+          v[i] = c < used && r < rows ? stats[r] : make_float2(INFINITY, 0.f);
+        }
+      }
+      if (lane == 0) ok = mbar_wait(&t_full[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL);
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (MODE == WB_DKV) {
+        aux[st * WB_SUB + lane] = v[0];
+        aux[st * WB_SUB + 32 + lane] = v[1];
+      } else {
+        const WaTile t = R.tile(n);
+        if (t.k1 - t.k0 < WB_SUB) {
+          for (int r = t.k1 - t.k0 + (lane >> 3); r < WB_SUB; r += 4)
+#pragma unroll
+            for (int kb = 0; kb < DB; ++kb)
+              *reinterpret_cast<uint4*>(ts + st * Cfg::STAGE + kb * WB_SBLK + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&t_ready[st]);
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA issuer (one thread)
+    if (lane == 0 && NT > 0) {
+      constexpr uint32_t idesc_x = make_idesc(128, WB_SUB, 1, 1, 0, 0);
+      constexpr uint32_t idesc_g = make_idesc(128, DB * 64, 1, 1, 0, 1);
+      const uint32_t r1a = smem_u32(r1s), r2a = smem_u32(r2s), tsa = smem_u32(ts);
+      bool ok = mbar_wait(r_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
+      auto issue_scores = [&](int n) {
+        const int st = n % WB_NS, buf = n & 1;
+        if (!mbar_wait(&t_ready[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL)) return false;
+        // the buffer holds P and dS of sub-tile n - 2 until its gradient products have read them
+        if (n >= 2 && !mbar_wait(&g_done[buf], ((n >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
+        tc_fence_after();
+        const uint32_t t1 = tsa + st * Cfg::STAGE, t2 = t1 + DB * WB_SBLK, x = tmem_base + Cfg::X_COL + buf * 128;
+#pragma unroll
+        for (int kb = 0; kb < DB; ++kb)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(x, make_smem_desc_sw128(r1a + kb * WA_BLK + k * 32, 16, 1024),
+                     make_smem_desc_sw128(t1 + kb * WB_SBLK + k * 32, 16, 1024), idesc_x, (kb > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+        for (int kb = 0; kb < DB; ++kb)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(x + 64, make_smem_desc_sw128(r2a + kb * WA_BLK + k * 32, 16, 1024),
+                     make_smem_desc_sw128(t2 + kb * WB_SBLK + k * 32, 16, 1024), idesc_x, (kb > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&x_full[buf]);
+        return true;
+      };
+      if (ok) ok = issue_scores(0);
+      for (int n = 0; n < NT && ok; ++n) {
+        if (n + 1 < NT && !issue_scores(n + 1)) break;
+        const int st = n % WB_NS, buf = n & 1;
+        if (!mbar_wait(&a_full[buf], (n >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
+        tc_fence_after();
+        const uint32_t t1 = tsa + st * Cfg::STAGE, t2 = t1 + DB * WB_SBLK, x = tmem_base + Cfg::X_COL + buf * 128;
+#pragma unroll
+        for (int k = 0; k < WB_SUB / 16; ++k) {
+          if (MODE == WB_DKV)
+            umma_f16_ts(tmem_base + Cfg::O2_COL, x + k * 8, make_smem_desc_sw128(t2 + k * 2048, WB_SBLK, 1024), idesc_g,
+                        (n > 0 || k > 0) ? 1u : 0u);
+          umma_f16_ts(tmem_base + Cfg::O1_COL, x + 64 + k * 8, make_smem_desc_sw128(t1 + k * 2048, WB_SBLK, 1024), idesc_g,
+                      (n > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(&t_empty[st]);
+        umma_commit(&g_done[buf]);
+        if (n == NT - 1) umma_commit(all_done);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- P, dS and the epilogue
+    const int st_id = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t x_addr = tmem_base + lane_addr + Cfg::X_COL + st_id * 128;
+    // DQ: this thread's row;  DKV: its key
+    const int ql = row / p.g, qi = row0 + ql;
+    const int head = hk * p.g + (row - ql * p.g);
+    const bool row_ok = MODE == WB_DQ ? (ql < p.box_q && qi < p.S) : (row0 + row < klim);
+    float lse2 = INFINITY, delta = 0.f;
+    if (MODE == WB_DQ && row_ok) {
+      const float2 v = p.stats[(static_cast<long long>(b) * p.Hk + hk) * p.S * p.g + static_cast<long long>(qi) * p.g + (row - ql * p.g)];
+      lse2 = v.x;
+      delta = v.y;
+    }
+    bool ok = true;
+    float row_dot = 0.f;                   // SINKS: sum_j p_ij dP_ij over this warp group's keys
+    for (int n = st_id; n < NT; n += 2) {
+      const int st = n % WB_NS;
+      unsigned words[2] = {0u, 0u};
+      if (row_ok) {
+        if (MODE == WB_DQ) {
+          const WaTile t = R.tile(n);
+          const int pos = off + qi;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            words[i] = wa_mask_word(t.k0 + 32 * i, min(pos, klim - 1), pos - p.window + 1, p.ns, t.k1);
+        } else {     // the columns [lo, hi) of this key: rows at or behind it, inside its window
+          const int j = row0 + row, q0 = (n_first + n) * p.sub_q;
+          const int first = min(max(j - off - q0, 0), p.sub_q);
+          const int last = j < p.ns ? p.sub_q : min(max(j - off - q0 + p.window, 0), p.sub_q);
+          const int lo = first * p.g, hi = min(last, p.S - q0) * p.g;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) words[i] = wa_low_bits(hi - 32 * i) & ~wa_low_bits(lo - 32 * i);
+        }
+      }
+      bool got = mbar_wait(&x_full[st_id], (n >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+      if (MODE == WB_DKV) got = got && mbar_wait(&t_ready[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL);
+      if (!__all_sync(0xffffffffu, got)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t x1[32], x2[32], pw[16], dw[16];
+        tmem_ld_x32(x_addr + 32 * i, x1);
+        tmem_ld_x32(x_addr + 64 + 32 * i, x2);
+        tmem_wait_ld();
+        const bool full = __all_sync(0xffffffffu, words[i] == 0xffffffffu);
+        const float4* a4 = reinterpret_cast<const float4*>(aux + st * WB_SUB + 32 * i);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float4 a;
+          if (MODE == WB_DKV) a = a4[e];
+          else a = make_float4(lse2, delta, lse2, delta);
+          float p0 = exp2f(fmaf(__uint_as_float(x1[2 * e]), p.scale_log2, -a.x));
+          float p1 = exp2f(fmaf(__uint_as_float(x1[2 * e + 1]), p.scale_log2, -a.z));
+          float d0 = p0 * (__uint_as_float(x2[2 * e]) - a.y);
+          float d1 = p1 * (__uint_as_float(x2[2 * e + 1]) - a.w);
+          if (!full) {      // selected, not multiplied: what is masked may be NaN
+            const bool v0 = (words[i] >> (2 * e)) & 1u, v1 = (words[i] >> (2 * e + 1)) & 1u;
+            p0 = v0 ? p0 : 0.f;
+            d0 = v0 ? d0 : 0.f;
+            p1 = v1 ? p1 : 0.f;
+            d1 = v1 ? d1 : 0.f;
+          }
+          if (SINKS) row_dot += fmaf(p0, delta, d0) + fmaf(p1, delta, d1);
+          pw[e] = pack_bf16x2(p0, p1);
+          dw[e] = pack_bf16x2(d0, d1);
+        }
+        if (MODE == WB_DKV) tmem_st_x16(x_addr + 16 * i, pw);
+        tmem_st_x16(x_addr + 64 + 16 * i, dw);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&a_full[st_id]);
+    }
+    if (NT > 0 && ok) ok = mbar_wait(all_done, 0, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    if (SINKS) {
+      // -exp(sink - lse) do.o, summed over the tile's queries for each head
+      float* red = reinterpret_cast<float*>(aux);      // [2][128]
+      red[st_id * 128 + row] = row_ok ? -exp2f(p.sinks[head] * 1.4426950408889634f - lse2) * row_dot : 0.f;
+      if (named_bar_and(1, 256, ok) && threadIdx.x < p.g) {
+        float t = 0.f;
+        for (int i = threadIdx.x; i < p.box_q * p.g; i += p.g) t += red[i] + red[128 + i];
+        p.sink_part[(static_cast<long long>(hk * p.g + threadIdx.x) * gridDim.z + b) * gridDim.x + blockIdx.x] = t;
+      }
+    }
+    if (ok) {
+      // DQ: each warp group half of dq's columns;  DKV: dk by the first, dv by the second
+      const bool second = MODE == WB_DKV && st_id == 1;
+      const int col0 = MODE == WB_DQ ? st_id * DB * 32 : 0;
+      constexpr int CHUNKS = MODE == WB_DQ ? DB : 2 * DB;
+      const int D = second ? p.Dv : p.Dq;
+      const float mul = second ? 1.f : p.scale;
+      const bool in = MODE == WB_DQ ? row_ok : row0 + row < p.T;
+      __nv_bfloat16* dst = second ? p.o2 + b * p.o2_sb + (row0 + row) * p.o2_ss + hk * p.o2_sh
+                                  : (MODE == WB_DQ ? p.o1 + b * p.o1_sb + qi * p.o1_ss + head * p.o1_sh
+                                                   : p.o1 + b * p.o1_sb + (row0 + row) * p.o1_ss + hk * p.o1_sh);
+      float* fdst = nullptr;
+      if (MODE == WB_DKV && split >= 0)
+        fdst = p.part + ((((static_cast<long long>(b) * p.Hk + hk) * p.sink_tiles + key_tile) * p.sink_splits + split) * 128 + row) *
+                            (p.Dq + p.Dv) + (second ? p.Dq : 0);
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        uint32_t o[32];
+        if (NT > 0) {
+          tmem_ld_x32(tmem_base + lane_addr + (second ? Cfg::O2_COL : Cfg::O1_COL) + col0 + c * 32, o);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          const int col = col0 + c * 32 + ch * 8;
+          if (in && col < D) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = NT > 0 ? __uint_as_float(o[8 * ch + e]) * mul : 0.f;
+            if (fdst != nullptr) {
+              *reinterpret_cast<float4*>(fdst + col) = make_float4(f[0], f[1], f[2], f[3]);
+              *reinterpret_cast<float4*>(fdst + col + 4) = make_float4(f[4], f[5], f[6], f[7]);
+            } else {
+              *reinterpret_cast<uint4*>(dst + col) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
+                                                               pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+            }
+          }
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Row statistics for the kernel above: stats[b, hk, s, hg] = (lse log2 e, do.o).  16 lanes to a row (8 columns each).
+struct StatsParams {
+  int B, S, H, g, Dv;
+  const __nv_bfloat16* o;
+  const __nv_bfloat16* d;
+  long long o_sb, o_ss, o_sh, d_sb, d_ss, d_sh;
+  const float* lse;                        // [B, H, S]
+  float2* stats;
+};
+constexpr int WS_ROWS = 64;                // queries of a block (one head)
+__global__ void __launch_bounds__(256) window_stats_kernel(const StatsParams p) {
+  const int h = blockIdx.y, b = blockIdx.z, hk = h / p.g, hg = h - hk * p.g, Hk = p.H / p.g;
+  const int sub = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+  const int s0 = blockIdx.x * WS_ROWS;
+  uint4 a[4], c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = s0 + i * 16 + sub;
+    a[i] = c[i] = make_uint4(0, 0, 0, 0);
+    if (s < p.S && l16 * 8 < p.Dv) {
+      a[i] = *reinterpret_cast<const uint4*>(p.o + b * p.o_sb + s * p.o_ss + h * p.o_sh + l16 * 8);
+      c[i] = *reinterpret_cast<const uint4*>(p.d + b * p.d_sb + s * p.d_ss + h * p.d_sh + l16 * 8);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = s0 + i * 16 + sub;
+    float fa[8], fc[8], sum = 0.f;
+    unpack8_bf16(a[i], fa);
+    unpack8_bf16(c[i], fc);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(fa[e], fc[e], sum);
+#pragma unroll
+    for (int m = 8; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    if (s < p.S && l16 == 0) {
+      const float lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.S + s];
+      p.stats[((static_cast<long long>(b) * Hk + hk) * p.S + s) * p.g + hg] = make_float2(lse * 1.4426950408889634f, sum);
+    }
+  }
+}
+
+// Sums the split key tiles' partial gradients in order: a thread per (sequence, key head, key, 4 columns).
+struct JoinParams {
+  int T, Hk, Dq, Dv, tiles, splits;
+  const float* part;
+  __nv_bfloat16 *dk, *dv;
+  long long k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
+  long long n;
+};
+__global__ void __launch_bounds__(256) window_join_kernel(const JoinParams p) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.n) return;
+  const int vec = (p.Dq + p.Dv) / 4;
+  const int col = static_cast<int>(i % vec) * 4;
+  long long r = i / vec;
+  const int key = static_cast<int>(r % (p.tiles * 128));
+  r /= p.tiles * 128;
+  const int hk = static_cast<int>(r % p.Hk);
+  const long long b = r / p.Hk;
+  if (key >= p.T) return;
+  const float* src = p.part + ((((b * p.Hk + hk) * p.tiles + key / 128) * p.splits) * 128 + key % 128) * (p.Dq + p.Dv) + col;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int q = 0; q < p.splits; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(src + static_cast<long long>(q) * 128 * (p.Dq + p.Dv));
+    s.x += v.x;
+    s.y += v.y;
+    s.z += v.z;
+    s.w += v.w;
+  }
+  __nv_bfloat16* dst = col < p.Dq ? p.dk + b * p.k_sb + key * p.k_ss + hk * p.k_sh + col
+                                  : p.dv + b * p.v_sb + key * p.v_ss + hk * p.v_sh + (col - p.Dq);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+}
+
+}  // namespace cmb
+
+namespace {
+
+template <int MODE, int DB, bool SINKS = false>
+int launch_window_bwd(const CUtensorMap (&m)[4], const cmb::WindowBwdParams& p, int gx, int B, cudaStream_t stream) {
+  using Cfg = cmb::WindowBwdCfg<DB>;
+  auto kern = cmb::window_bwd_kernel<MODE, DB, SINKS>;
+  static std::atomic<unsigned long long> attr_done{0};
+  if (cmb_host::set_smem_limit_once_per_device(attr_done, reinterpret_cast<const void*>(kern), Cfg::SMEM_BYTES)) return 103;
+  kern<<<dim3(gx, p.Hk, B), cmb::WB_THREADS, Cfg::SMEM_BYTES, stream>>>(m[0], m[1], m[2], m[3], p);
+  return cudaGetLastError() == cudaSuccess ? 0 : 104;
+}
+
+}  // namespace
+
+// Backward of cmb_window_fwd's contiguous form.  o (the forward's output), dO [B,S,H,Dv]; lse [B,H,S]; dq [B,S,H,Dq],
+// dk [B,T,Hk,Dq], dv [B,T,Hk,Dv] bf16 (every element written; dq or dk and dv may be null together).  stats: scratch of
+// 2 B S H floats; sink_part (with sinks and dq): [H, B * ceil(S / min(S, 128 / (H / Hk)))] floats
+// or null; part: B Hk sink_tiles sink_splits 128 (Dq + Dv) floats where
+// sink_splits > 1.  ip = {B, S, T, H, Hk, Dq, Dv, window, ns, sink_tiles, sink_splits};
+// lp = 3 strides (batch, row, head) of each of q, k, v, o, dO, dq, dk, dv.  H / Hk <= 64.
+extern "C" int cmb_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dO, const int* lengths,
+                              const float* sinks, const float* lse, void* dq, void* dk, void* dv, float* stats, float* sink_part,
+                              float* part, const int* ip, const long long* lp, float scale, int* status, void* stream) {
+  const int B = ip[0], S = ip[1], T = ip[2], H = ip[3], Hk = ip[4], Dq = ip[5], Dv = ip[6];
+  if (B <= 0 || B > 65535 || S <= 0 || T < S || Hk <= 0 || Hk > 65535 || H <= 0 || H > 65535 || H % Hk || H / Hk > 64) return 1;
+  if (Dq <= 0 || Dq > 128 || Dq % 8 || Dv <= 0 || Dv > 128 || Dv % 8) return 1;
+  if (ip[7] < 1 || ip[7] > cmb::WA_NO_WINDOW || ip[8] < 0 || !(scale > 0.f)) return 1;
+  for (int i = 9; i < 24; ++i)
+    if (lp[i] & 7) return 1;
+  if (sink_part != nullptr && (sinks == nullptr || dq == nullptr)) return 1;
+  const int key_tiles = (T + 127) / 128;
+  cmb::WindowBwdParams p{};
+  p.S = S; p.T = T; p.H = H; p.Hk = Hk; p.g = H / Hk; p.Dq = Dq; p.Dv = Dv;
+  p.box_q = 128 / p.g < S ? 128 / p.g : S;
+  p.sub_q = cmb::WB_SUB / p.g;
+  p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
+  p.window = ip[7]; p.ns = ip[8]; p.lengths = lengths;
+  p.stats = reinterpret_cast<const float2*>(stats);
+  p.sink_tiles = ip[9]; p.sink_splits = ip[10]; p.part = part; p.status = status;
+  if (p.sink_tiles < 0 || p.sink_tiles > key_tiles || p.sink_splits < 1 || (p.sink_splits > 1 && part == nullptr)) return 1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+
+  cmb::StatsParams sp{};
+  sp.B = B; sp.S = S; sp.H = H; sp.g = p.g; sp.Dv = Dv;
+  sp.o = static_cast<const __nv_bfloat16*>(o); sp.o_sb = lp[9]; sp.o_ss = lp[10]; sp.o_sh = lp[11];
+  sp.d = static_cast<const __nv_bfloat16*>(dO); sp.d_sb = lp[12]; sp.d_ss = lp[13]; sp.d_sh = lp[14];
+  sp.lse = lse; sp.stats = reinterpret_cast<float2*>(stats);
+  cmb::window_stats_kernel<<<dim3((S + cmb::WS_ROWS - 1) / cmb::WS_ROWS, H, B), 256, 0, st>>>(sp);
+  if (cudaGetLastError() != cudaSuccess) return 104;
+
+  const bool wide = Dq > 64 || Dv > 64;
+  auto maps = [&](CUtensorMap& mq, CUtensorMap& mo, CUtensorMap& mk, CUtensorMap& mv, int box_q, int box_k) {
+    int rc = cmb_host::make_tmap_grouped(&mq, q, Dq, S, Hk, p.g, B, lp[1], lp[2], lp[0], box_q);
+    if (!rc) rc = cmb_host::make_tmap_grouped(&mo, dO, Dv, S, Hk, p.g, B, lp[13], lp[14], lp[12], box_q);
+    if (!rc) rc = cmb_host::make_tmap_rows(&mk, k, Dq, T, Hk, B, lp[4], lp[5], lp[3], box_k);
+    if (!rc) rc = cmb_host::make_tmap_rows(&mv, v, Dv, T, Hk, B, lp[7], lp[8], lp[6], box_k);
+    return rc;
+  };
+  if (dk != nullptr) {
+    CUtensorMap mq, mo, mk, mv;
+    int rc = maps(mq, mo, mk, mv, p.sub_q, 128);
+    if (rc) return rc;
+    cmb::WindowBwdParams pk = p;
+    pk.o1 = static_cast<__nv_bfloat16*>(dk); pk.o1_sb = lp[18]; pk.o1_ss = lp[19]; pk.o1_sh = lp[20];
+    pk.o2 = static_cast<__nv_bfloat16*>(dv); pk.o2_sb = lp[21]; pk.o2_ss = lp[22]; pk.o2_sh = lp[23];
+    const CUtensorMap m[4] = {mk, mv, mq, mo};
+    const int gx = key_tiles + p.sink_tiles * (p.sink_splits - 1);
+    rc = wide ? launch_window_bwd<cmb::WB_DKV, 2>(m, pk, gx, B, st) : launch_window_bwd<cmb::WB_DKV, 1>(m, pk, gx, B, st);
+    if (rc) return rc + 10000;
+    if (p.sink_splits > 1 && p.sink_tiles > 0) {
+      cmb::JoinParams j{};
+      j.T = T; j.Hk = Hk; j.Dq = Dq; j.Dv = Dv; j.tiles = p.sink_tiles; j.splits = p.sink_splits; j.part = part;
+      j.dk = pk.o1; j.k_sb = pk.o1_sb; j.k_ss = pk.o1_ss; j.k_sh = pk.o1_sh;
+      j.dv = pk.o2; j.v_sb = pk.o2_sb; j.v_ss = pk.o2_ss; j.v_sh = pk.o2_sh;
+      j.n = static_cast<long long>(B) * Hk * p.sink_tiles * 128 * ((Dq + Dv) / 4);
+      cmb::window_join_kernel<<<static_cast<unsigned>((j.n + 255) / 256), 256, 0, st>>>(j);
+      if (cudaGetLastError() != cudaSuccess) return 104;
+    }
+  }
+  if (dq != nullptr) {
+    CUtensorMap mq, mo, mk, mv;
+    int rc = maps(mq, mo, mk, mv, p.box_q, cmb::WB_SUB);
+    if (rc) return rc;
+    cmb::WindowBwdParams pq = p;
+    pq.o1 = static_cast<__nv_bfloat16*>(dq); pq.o1_sb = lp[15]; pq.o1_ss = lp[16]; pq.o1_sh = lp[17];
+    const CUtensorMap m[4] = {mq, mo, mk, mv};
+    const int gx = (S + p.box_q - 1) / p.box_q;
+    if (sink_part != nullptr) {
+      pq.sinks = sinks; pq.sink_part = sink_part;
+      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2, true>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1, true>(m, pq, gx, B, st);
+    } else {
+      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1>(m, pq, gx, B, st);
+    }
+    if (rc) return rc + 20000;
+  }
+  return 0;
+}

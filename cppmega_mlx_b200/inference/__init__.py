@@ -7,5 +7,5 @@ from .serving_engine import ServingEngine, ServingRequest
 from .infilling import build_infilling_prompt, splice_infill
 from .sampling import apply_top_k, apply_top_p, sample_next_token
 from .serving import (ContinuousBatchScheduler, PagedKVBlockManager, build_paged_block_table, paged_decode_attention,
-                      paged_latent_decode_attention)
-from .speculative_decode import leviathan_accept, speculative_generate, typical_accept
+                      paged_latent_decode_attention, paged_tree_attention)
+from .speculative_decode import greedy_tree_accept, leviathan_accept, speculative_generate, typical_accept

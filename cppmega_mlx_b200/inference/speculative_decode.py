@@ -64,6 +64,22 @@ def typical_accept(draft_tokens: torch.Tensor, target_probs: torch.Tensor, *, th
     return AcceptanceResult(torch.cat([draft_tokens, bonus]), k, True)
 
 
+def greedy_tree_accept(parents, draft_tokens, target_tokens) -> tuple[list[int], int]:
+    """The longest path of a drafted tree that the target's greedy choice follows.  ``parents`` [N] as in ``ops.tree_words``; ``draft_tokens``
+    [N]; ``target_tokens`` [N + 1]: the target's choice after the prefix, then after each drafted token.  Returns (the accepted tokens'
+    indexes, root first, for ``PagedKVBlockManager.accept``; the target's token after them)."""
+    par, tok, want = (torch.as_tensor(x).tolist() for x in (parents, draft_tokens, target_tokens))
+    if len(tok) != len(par) or len(want) != len(par) + 1:
+        raise ValueError("parents and draft_tokens must have N entries and target_tokens N + 1")
+    path, at = [], -1
+    while True:
+        nxt = next((n for n, m in enumerate(par) if m == at and n > at and tok[n] == want[at + 1]), None)
+        if nxt is None:
+            return path, want[at + 1]
+        path.append(nxt)
+        at = nxt
+
+
 def batched_leviathan_accept(draft_tokens, draft_probs, target_probs, *, generator=None, pad: int = -1):
     """Row-wise acceptance for [B,K] drafts; returns ([B,K+1] tokens padded with ``pad``, [B] accepted counts)."""
     b, k = draft_tokens.shape

@@ -2,8 +2,9 @@
 
 Modes: ``mla`` / ``full`` (dense causal SDPA), ``gqa`` (grouped KV heads), ``dsa`` (sparse top-k keys
 through :func:`ops.sparse_mla_attention` over a shared ``sparse_kv`` projection).  Supports split-half
-RoPE (standard / llama3 / YaRN), sliding windows, document masks, attention sinks and a contiguous KV
-cache for decode.  Behavioural parity: ``cppmega_mlx/nn/attention.py:47-188`` (config),
+RoPE (standard / llama3 / YaRN), sliding windows with visible first tokens, document masks, attention sinks and a contiguous or
+static KV cache for decode.  A window or sink logits without a mask tensor run ``ops.window_attention`` / ``ops.cached_attention`` on
+CUDA bf16.  Behavioural parity: ``cppmega_mlx/nn/attention.py:47-188`` (config),
 ``:214-248`` (mask), ``:251-284`` (recency-window indices), ``:287-360`` (mask → indices),
 ``:541-986`` (module).  The low-rank MLA + learned-indexer attention lives in ``nn/mla.py``.
 """
@@ -17,6 +18,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..ops.rope import RopeScaling
+from ..ops.window_attention import kernel_covers
 from .basic import Linear
 
 ATTENTION_MODES = ("mla", "dsa", "full", "gqa")
@@ -43,6 +45,7 @@ class AttentionConfig:
     bias: bool = False
     sliding_window: int | None = None
     sparse_topk: int = 16
+    sink_tokens: int = 0              # with sliding_window: first tokens that stay visible to every query
 
     def __post_init__(self) -> None:
         if self.mode not in ATTENTION_MODES:
@@ -77,6 +80,10 @@ class AttentionConfig:
             raise NotImplementedError("attention logit soft-capping is not implemented")
         if self.sliding_window is not None and self.sliding_window <= 0:
             raise ValueError("sliding_window must be positive")
+        if self.sink_tokens < 0:
+            raise ValueError("sink_tokens must be non-negative")
+        if self.sink_tokens and self.sliding_window is None:
+            raise ValueError("sink_tokens need a sliding_window")
         if self.sparse_topk <= 0:
             raise ValueError("sparse_topk must be positive")
 
@@ -107,8 +114,9 @@ class AttentionConfig:
 
 
 def causal_sdpa_mask(seq_length: int, *, sliding_window: int | None = None, expand_heads: bool = False,
-                     query_offset: int = 0, key_length: int | None = None, device=None) -> torch.Tensor:
-    """Boolean [S, K] mask (True = attend). ``sliding_window`` counts the current token."""
+                     query_offset: int = 0, key_length: int | None = None, device=None, sink_tokens: int = 0) -> torch.Tensor:
+    """Boolean [S, K] mask (True = attend). ``sliding_window`` counts the current token; the first ``sink_tokens`` keys stay visible
+    behind it."""
     if seq_length <= 0:
         raise ValueError(f"seq_length must be positive, got {seq_length}")
     if query_offset < 0:
@@ -122,7 +130,7 @@ def causal_sdpa_mask(seq_length: int, *, sliding_window: int | None = None, expa
     kp = torch.arange(key_length, device=device)[None, :]
     mask = qp >= kp
     if sliding_window is not None:
-        mask = mask & (qp < kp + sliding_window)
+        mask = mask & ((qp < kp + sliding_window) | (kp < sink_tokens))
     return mask[None, None] if expand_heads else mask
 
 
@@ -249,7 +257,7 @@ class CausalSelfAttention(nn.Module):
         return ops.apply_rope(x, cos, sin)
 
     @torch.no_grad()
-    def _static_step(self, x, cache, layer_idx: int) -> torch.Tensor:
+    def _static_step(self, x, cache, layer_idx: int, sinks: torch.Tensor | None = None) -> torch.Tensor:
         """One-token step against a ``StaticDecodeCache`` (device-side position; CUDA-graph replayable)."""
         from ..ops import decode_attention as DA
         c = self.config
@@ -269,12 +277,14 @@ class CausalSelfAttention(nn.Module):
             idx = torch.where(idx >= 0, idx, torch.full_like(idx, -1)).contiguous()
             out = DA.decode_attention(q, rows, None, cache.table(), lengths, scale=scale, topk=idx, d_v=c.q_head_dim, max_keys=k)
         else:
-            if c.sliding_window is not None:
-                raise ValueError("sliding-window attention has no static decode path")
             kk = cache.write_a(layer_idx, rope(self.k_proj(xt).view(1, b, c.kv_heads, c.q_head_dim)).transpose(0, 1))
             vv = cache.write_b(layer_idx, self.v_proj(xt).view(b, 1, c.kv_heads, c.q_head_dim))
-            out = DA.decode_attention(q, cache.attention_rows(kk, c.kv_heads, c.q_head_dim), cache.attention_rows(vv, c.kv_heads, c.q_head_dim),
-                                      cache.table(), lengths, scale=scale, max_keys=cache.capacity)
+            kk, vv = (cache.attention_rows(t, c.kv_heads, c.q_head_dim) for t in (kk, vv))
+            if c.sliding_window is not None or sinks is not None:
+                out = ops.cached_attention(q[:, None], kk, vv, cache.table(), lengths - 1, window=c.sliding_window, sink_tokens=c.sink_tokens,
+                                           sinks=sinks, scale=scale, max_keys=cache.capacity)
+            else:
+                out = DA.decode_attention(q, kk, vv, cache.table(), lengths, scale=scale, max_keys=cache.capacity)
         return self._out(out.reshape(b, 1, c.q_proj_dim))
 
     def forward(self, hidden_states: torch.Tensor, mask: torch.Tensor | str | None = "causal", *, kv_cache=None,
@@ -282,9 +292,9 @@ class CausalSelfAttention(nn.Module):
         c = self.config
         b, s, _ = hidden_states.shape
         if getattr(kv_cache, "static", False):
-            if s != 1 or isinstance(mask, torch.Tensor) or sinks is not None:
-                raise ValueError("a static decode cache serves one-token steps without an explicit mask or sinks")
-            return self._static_step(hidden_states, kv_cache, layer_idx)
+            if s != 1 or isinstance(mask, torch.Tensor) or (sinks is not None and c.mode == "dsa"):
+                raise ValueError("a static decode cache serves one-token steps without an explicit mask (nor, in mode 'dsa', sinks)")
+            return self._static_step(hidden_states, kv_cache, layer_idx, sinks)
         if self.tp_group is not None:
             if self.sequence_parallel and kv_cache is not None:
                 raise NotImplementedError("sequence-parallel attention has no cache path")
@@ -318,12 +328,16 @@ class CausalSelfAttention(nn.Module):
                 lengths = torch.full((b,), klen, dtype=torch.int32, device=q.device)
                 out = DA.decode_attention(q[:, 0], k, v, None, lengths, scale=c.q_head_dim ** -0.5, max_keys=klen)
                 return self._out(out.reshape(b, s, c.q_proj_dim))
+        if plain_causal and (c.sliding_window is not None or sinks is not None) and kernel_covers(q, k, v):
+            # the window's kernel (training, prompts and single tokens alike): work and memory go by the visible pairs
+            out = ops.window_attention(q, k, v, window=c.sliding_window, sink_tokens=c.sink_tokens, sinks=sinks)
+            return self._out(out.reshape(b, s, c.q_proj_dim))
         qh, kh, vh = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
         if plain_causal and c.sliding_window is None and klen == s and sinks is None:
             out = dense_attention(qh, kh, vh, is_causal=True)
         else:
             m = causal_sdpa_mask(s, sliding_window=c.sliding_window, query_offset=klen - s, key_length=klen,
-                                 device=hidden_states.device)[None, None]
+                                 device=hidden_states.device, sink_tokens=c.sink_tokens)[None, None]
             if isinstance(mask, torch.Tensor):
                 extra = mask if mask.dtype == torch.bool else torch.isfinite(mask.float())
                 while extra.dim() < 4:

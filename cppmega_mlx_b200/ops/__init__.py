@@ -14,4 +14,7 @@ from .sparse_mla import indices_to_mask, sparse_mla_attention, sparse_mla_masked
 from .fp8_scale import fp8_amax, fp8_pack, fp8_quantize, linear_with_amax
 from .sparse_mla_blockscaled import mxfp8_roundtrip_ste, sparse_mla_blockscaled
 from . import decode_attention  # module: decode_attention.decode_attention(...) / .decode_attention_reference(...)
+from .window_attention import window_attention, window_attention_reference
+from .cached_attention import cached_attention, cached_attention_reference, tree_words
+from .pages import compact_rows, copy_pages
 from .topk import topk_select, topk_select_reference

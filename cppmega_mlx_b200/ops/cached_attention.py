@@ -1,0 +1,132 @@
+"""Attention of the newest tokens of every sequence over its cache: a tree of drafted tokens, a chain of them (a chunk of a prompt),
+or a single next token; with an optional sliding window and first tokens that stay visible.
+
+``q`` [B, N, H, Dq] are N new tokens per sequence whose keys and values have been written to the cache already, at positions
+``prefix_lengths[b] .. prefix_lengths[b] + N - 1``.  The cache is read in place:
+
+* paged: ``k_rows`` / ``v_rows`` are views ``[num_pages, page_size, kv_heads, D]`` of one layer of a block pool and ``table`` [B, W]
+  int32 maps a sequence's logical pages to pool pages;
+* contiguous: ``table is None`` and the views are ``[B, T, kv_heads, D]``.
+
+``tree`` [N] (one for the batch) or [B, N] int64, N <= 64: bit m of word n is set where token n sees token m — itself and its
+ancestors (``tree_words``).  Token n then stands at position ``prefix + (bits of word n) - 1``, a token whose word is 0 is padding
+and yields zeros.  ``tree is None``: a chain, token n sees all tokens up to itself (any N).  Every token sees the sequence's
+prefix.  ``window`` and ``sink_tokens`` restrict both by position: a key at position j is seen from position P when ``P - j < window``
+or ``j < sink_tokens``.  ``sinks`` [H]: one more key per head with that logit and value 0.
+
+What no token sees — rows past a sequence's end, table entries past them, pages behind the window — may hold anything.  A table
+entry or a length that the pool or the table cannot hold is reported by ``ops.check_status`` (the kernel stays inside the pool).
+
+CUDA bf16 tensors run ``csrc/window_attn.cu`` (tcgen05, split over the keys when there are few rows); page sizes that are not a
+multiple of 8, other types and CPU tensors use ``cached_attention_reference``, the test oracle.  No gradients: inputs that require
+one are refused.  The reference verifies drafts as a plain chain (``cppmega_mlx/inference/speculative_decode.py:92``) and never attends
+over its pages (``cppmega_mlx/inference/serving.py:522``).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _backend as B
+from .window_attention import (NO_WINDOW, _check, _check_lengths, kernel_covers, launch_forward, masked_softmax_attention, on_device,
+                               usable)
+
+MAX_TREE = 64
+
+
+def tree_words(parents) -> torch.Tensor:
+    """[N] or [B, N] parents (the index of each drafted token's parent among the drafted tokens; -1: it follows the prefix; -2:
+    padding) in an order where a parent stands before its children → int64 words for ``cached_attention(tree=...)``, on the CPU."""
+    par = torch.as_tensor(parents, dtype=torch.int64).cpu()
+    if par.dim() not in (1, 2) or par.shape[-1] > MAX_TREE:
+        raise ValueError(f"tree_words: parents must be [N] or [B, N] with N <= {MAX_TREE}, got {tuple(par.shape)}")
+    rows = []
+    for row in par.reshape(-1, par.shape[-1]).tolist():
+        words: list[int] = []
+        for n, m in enumerate(row):
+            if m >= n or m < -2 or (m >= 0 and words[m] == 0):
+                raise ValueError(f"tree_words: token {n} has parent {m}: parents stand before their children and are no padding")
+            words.append(0 if m == -2 else (words[m] if m >= 0 else 0) | (1 << n))
+        rows.append([w - (1 << 64) if w >> 63 else w for w in words])
+    return torch.tensor(rows, dtype=torch.int64).reshape(par.shape)
+
+
+def _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale):
+    scale = _check(q, k_rows, v_rows, window, sink_tokens, sinks, scale, "cached_attention")
+    b, n = q.shape[:2]
+    _check_lengths(prefix_lengths, b, q.device, "cached_attention: prefix_lengths")
+    if table is not None:
+        if table.dim() != 2 or table.shape[0] != b or table.dtype not in (torch.int32, torch.int64) or table.device != q.device:
+            raise ValueError(f"cached_attention: table must be [{b}, pages] int32 / int64 on {q.device}, got {tuple(table.shape)} "
+                             f"{table.dtype} on {table.device}")
+    elif k_rows.shape[0] != b:
+        raise ValueError(f"cached_attention: a contiguous cache has {b} rows, got {k_rows.shape[0]}")
+    if tree is not None:
+        if tree.shape not in ((n,), (b, n)) or tree.dtype != torch.int64 or tree.device != q.device:
+            raise ValueError(f"cached_attention: tree must be int64 words [{n}] or [{b}, {n}] on {q.device}, got {tuple(tree.shape)} "
+                             f"{tree.dtype} on {tree.device}")
+        if n > MAX_TREE:
+            raise ValueError(f"cached_attention: a tree has at most {MAX_TREE} tokens, got {n}")
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k_rows, v_rows, sinks)):
+        raise ValueError("cached_attention has no gradient: call it under torch.no_grad(), or use window_attention")
+    return scale
+
+
+def cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, *, tree=None, window: int | None = None, sink_tokens: int = 0,
+                               sinks=None, scale: float | None = None):
+    scale = _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale)
+    b, n = q.shape[:2]
+    dev = q.device
+    prefix = prefix_lengths.long()
+    if table is not None:       # entries that no token reaches may be anything
+        ps = k_rows.shape[1]
+        need = torch.arange(table.shape[1], device=dev)[None] * ps < (prefix + n)[:, None]
+        pages = torch.where(need, table.long(), torch.zeros_like(table.long())).clamp_min(0)
+        k, v = k_rows[pages].flatten(1, 2), v_rows[pages].flatten(1, 2)
+    else:
+        k, v = k_rows, v_rows
+    t = k.shape[1]
+    idx = torch.arange(n, device=dev)
+    bits = (idx[None] <= idx[:, None])[None] if tree is None else ((tree.reshape(-1, n, 1) >> idx) & 1).bool()
+    bits = bits.expand(b, n, n)
+    depth = bits.sum(-1) - 1
+    pos = (prefix[:, None] + depth)[..., None]                            # [B, N, 1]
+    j = torch.arange(t, device=dev)[None, None]
+    w = NO_WINDOW if window is None else window
+    old = (j < prefix[:, None, None]) & ((pos - j < w) | (j < sink_tokens)) & (depth >= 0)[..., None]
+    m = (j[:, 0] - prefix[:, None]).clamp(0, max(n - 1, 0))               # [B, T]: which drafted token a row holds
+    held = (j >= prefix[:, None, None]) & (j < prefix[:, None, None] + n)
+    mpos = (prefix[:, None] + depth.gather(1, m))[:, None]                # [B, 1, T]
+    new = bits.gather(2, m[:, None].expand(b, n, t)) & held & ((pos - mpos < w) | (mpos < sink_tokens))
+    return masked_softmax_attention(q, k, v, old | new, sinks, scale)
+
+
+def kernel_supported(q, k_rows, v_rows, table) -> bool:
+    if not (kernel_covers(q, k_rows, v_rows) and usable(k_rows) and usable(v_rows)):
+        return False
+    if table is not None and (k_rows.shape[1] % 8 or not table.shape[1] or not k_rows.shape[0]):
+        return False
+    t = k_rows.shape[1] * (1 if table is None else table.shape[1])
+    return q.shape[1] <= t <= NO_WINDOW // 2 and q.shape[0] <= 65535
+
+
+def cached_attention(q, k_rows, v_rows, table, prefix_lengths, *, tree: torch.Tensor | None = None, window: int | None = None,
+                     sink_tokens: int = 0, sinks: torch.Tensor | None = None, scale: float | None = None,
+                     max_keys: int | None = None) -> torch.Tensor:
+    """See the module docstring; returns [B, N, H, Dv] in ``q.dtype``.  ``max_keys`` (a bound on ``prefix_lengths + N``) only tunes how
+    the work is split and never costs correctness."""
+    scale = _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale)
+    if q.shape[0] == 0 or q.shape[1] == 0:
+        return q.new_zeros(*q.shape[:3], v_rows.shape[3])
+    if not kernel_supported(q, k_rows, v_rows, table):
+        return cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, tree=tree, window=window, sink_tokens=sink_tokens,
+                                          sinks=sinks, scale=scale)
+    with on_device(q.device):
+        q = q if usable(q) else q.contiguous()
+        i32 = lambda x: None if x is None else x.to(torch.int32).contiguous()  # noqa: E731
+        tbl = i32(table)
+        page = k_rows.shape[1] if tbl is not None else 0
+        t = page * tbl.shape[1] if tbl is not None else k_rows.shape[1]
+        return launch_forward(q, k_rows, v_rows, t=t, lengths=i32(prefix_lengths), cached=True,
+                              tree=None if tree is None else tree.contiguous(), table=tbl, page=page, window=window,
+                              sink_tokens=int(sink_tokens), sinks=None if sinks is None else sinks.float().contiguous(), scale=scale,
+                              want_lse=False, max_keys=max_keys)[0]

@@ -1,0 +1,162 @@
+"""Movements of a paged cache: pages duplicated, rows closed up within sequences.
+
+``copy_pages(pools, src, dst)`` copies page ``src[i]`` of every pool to page ``dst[i]`` (a sequence forks, a page that others share is
+about to be written, the pool is put in order).  A pool is ``[num_pages, ...]`` with dense pages.  A page is written at most once in a
+call and not read in the same call; a pair (-1, -1) is an unused place of the list.
+
+``compact_rows(pools, table, start, path, counts)`` moves, in every sequence b, the cached rows of tokens ``start[b] + path[b, i]`` to
+``start[b] + i`` for ``i < counts[b]``, as if all were read before any is written: the accepted path of a drafted tree closes up
+behind the prefix.  Pools are ``[num_pages, layers, page_size, ...]`` with dense rows.
+
+Both work in place on CPU and CUDA tensors of any type, one launch for all pools of a cache (``csrc/pages.cu``).  Indexes given as
+Python lists or CPU tensors are checked before anything moves; in CUDA tensors, which are never read back, what lies outside the
+pool or the table is skipped and reported by ``ops.check_status``.  ``inference.PagedKVBlockManager`` builds fork, copy on write,
+acceptance and compaction of the pool on them.  The reference's manager only hands blocks out and takes them back
+(``cppmega_mlx/inference/serving.py:47-215``).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _backend as B
+from .window_attention import on_device
+
+MAX_POOLS = 32          # of one launch
+MAX_PAIRS = 65535
+MAX_MOVES = 2048        # rows of one sequence in one call
+
+
+def _pools(pools, rank: int, what: str) -> list[torch.Tensor]:
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    if not pools:
+        raise ValueError(f"{what}: no pools")
+    for p in pools:
+        if p.dim() < rank or p.shape[0] != pools[0].shape[0] or p.device != pools[0].device:
+            raise ValueError(f"{what}: pools have at least {rank} dimensions, one number of pages and one device")
+        if p.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: pools are written in place and cannot require a gradient")
+    return pools
+
+
+def _dense(t: torch.Tensor, first: int) -> bool:
+    """Whether the dimensions from ``first`` on are one dense piece of memory."""
+    want = 1
+    for n, s in zip(reversed(t.shape[first:]), reversed(t.stride()[first:])):
+        if n != 1 and s != want:
+            return False
+        want *= n
+    return True
+
+
+def _indexes(x, what: str) -> torch.Tensor:
+    t = x if isinstance(x, torch.Tensor) else torch.as_tensor(list(x), dtype=torch.int64)
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what} must be int32 / int64, got {t.dtype}")
+    return t
+
+
+def copy_pages(pools, src, dst) -> None:
+    """See the module docstring."""
+    pools = _pools(pools, 2, "copy_pages")
+    src, dst = _indexes(src, "copy_pages: src"), _indexes(dst, "copy_pages: dst")
+    if src.dim() != 1 or src.shape != dst.shape or src.device != dst.device:
+        raise ValueError(f"copy_pages: src and dst are one list each, got {tuple(src.shape)} and {tuple(dst.shape)}")
+    dev, n = pools[0].device, pools[0].shape[0]
+    if src.device.type == "cpu":
+        used = [(s, d) for s, d in zip(src.tolist(), dst.tolist()) if (s, d) != (-1, -1)]
+        for s, d in used:
+            if not (0 <= s < n and 0 <= d < n):
+                raise ValueError(f"copy_pages: page {s} to page {d} of {n}")
+        to = [d for _, d in used]
+        if len(set(to)) != len(to) or set(to) & {s for s, d in used if s != d}:
+            raise ValueError("copy_pages: a page is written twice, or read and written")
+        if not used:
+            return
+        if len(used) < src.shape[0]:
+            src, dst = torch.tensor([s for s, _ in used]), torch.tensor(to)
+    elif src.device != dev:
+        raise ValueError(f"copy_pages: indexes on {src.device}, pools on {dev}")
+    if src.shape[0] == 0 or n == 0:
+        return
+    if not B.on_gpu(*pools) or not all(_dense(p, 1) for p in pools) or src.shape[0] > MAX_PAIRS:
+        s, d = src.to(dev, torch.int64), dst.to(dev, torch.int64)
+        if src.device.type != "cpu":       # unused places copy page 0 to itself
+            pad = (s == -1) & (d == -1)
+            s, d = (s[~pad], d[~pad]) if bool(pad.any()) else (s, d)
+        for p in pools:
+            p[d] = p[s]
+        return
+    lib = B.load_library()
+    with on_device(dev):
+        s, d = (x.to(dev, torch.int32, non_blocking=True).contiguous() for x in (src, dst))
+        for at in range(0, len(pools), MAX_POOLS):
+            part = [p for p in pools[at:at + MAX_POOLS] if p.numel()]
+            if not part:
+                continue
+            bases = (ctypes.c_void_p * len(part))(*(p.data_ptr() for p in part))
+            lp = (ctypes.c_longlong * (4 * len(part)))(*(x for p in part for x in (
+                p.stride(0) * p.element_size(), 0, 0, p[0].numel() * p.element_size())))
+            B.check(lib.cmb_copy_pages(bases, lp, len(part), B.ptr(s), B.ptr(d), s.shape[0], n, B.ptr(B.status_buffer(dev)),
+                                       B.stream_ptr()), "copy_pages")
+
+
+def compact_rows_reference(pools, table, start, path, counts) -> None:
+    page = pools[0].shape[2]
+    i = torch.arange(path.shape[1], device=path.device)
+    to = start.long()[:, None] + i
+    fro = torch.where(i < counts[:, None], start.long()[:, None] + path, to)
+    use = (i < counts[:, None]) & (fro != to)
+    b = torch.arange(table.shape[0], device=path.device)[:, None].expand_as(to)[use]
+    to, fro = to[use], fro[use]
+    for p in pools:
+        p[table[b, to // page].long(), :, to % page] = p[table[b, fro // page].long(), :, fro % page]
+
+
+def compact_rows(pools, table, start, path, counts) -> None:
+    """See the module docstring.  table [B, W], start [B], path [B, P], counts [B], int32 / int64 on the pools' device."""
+    pools = _pools(pools, 4, "compact_rows")
+    dev = pools[0].device
+    if any(p.shape[:3] != pools[0].shape[:3] for p in pools):
+        raise ValueError("compact_rows: pools differ in pages, layers or page size")
+    table, start, path, counts = (_indexes(x, f"compact_rows: {n}") for x, n in
+                                  ((table, "table"), (start, "start"), (path, "path"), (counts, "counts")))
+    b = table.shape[0]
+    if table.dim() != 2 or path.dim() != 2 or path.shape[0] != b or start.shape != (b,) or counts.shape != (b,):
+        raise ValueError(f"compact_rows: table {tuple(table.shape)}, start {tuple(start.shape)}, path {tuple(path.shape)} and counts "
+                         f"{tuple(counts.shape)} do not fit")
+    if any(x.device != dev for x in (table, start, path, counts)):
+        raise ValueError(f"compact_rows: indexes and pools are on one device ({dev})")
+    if path.shape[1] > MAX_MOVES:
+        raise ValueError(f"compact_rows: at most {MAX_MOVES} rows of a sequence, got {path.shape[1]}")
+    if b == 0 or path.shape[1] == 0 or pools[0].numel() == 0:
+        return
+    n, layers, page = pools[0].shape[:3]
+    if dev.type == "cpu":
+        i = torch.arange(path.shape[1])
+        use = i < counts[:, None]
+        far = torch.where(use, torch.maximum(path, i.to(path.dtype)), torch.full_like(path, -1)).amax(1) + start
+        if bool((counts < 0).any()) or bool((counts > path.shape[1]).any()) or bool((path[use] < 0).any()) or bool((start < 0).any()) or \
+                bool((far >= table.shape[1] * page).any()):
+            raise ValueError("compact_rows: a row outside the table")
+        need = torch.arange(table.shape[1]) * page <= far[:, None]
+        need &= (torch.arange(table.shape[1]) + 1) * page > start[:, None]
+        need &= (counts > 0)[:, None]
+        if bool(((table < 0) | (table >= n))[need].any()):
+            raise ValueError(f"compact_rows: a page outside the pool of {n}")
+    if not B.on_gpu(*pools) or not all(_dense(p, 3) for p in pools) or b > 65535 or len(pools[:MAX_POOLS]) * layers > 65535:
+        compact_rows_reference(pools, table, start, path, counts)
+        return
+    lib = B.load_library()
+    with on_device(dev):
+        table, start, path, counts = (x.to(torch.int32).contiguous() for x in (table, start, path, counts))
+        ip = (ctypes.c_int * 6)(b, table.shape[1], path.shape[1], page, n, layers)
+        for at in range(0, len(pools), MAX_POOLS):
+            part = pools[at:at + MAX_POOLS]
+            bases = (ctypes.c_void_p * len(part))(*(p.data_ptr() for p in part))
+            lp = (ctypes.c_longlong * (4 * len(part)))(*(x for p in part for x in (
+                p.stride(0) * p.element_size(), p.stride(1) * p.element_size(), p.stride(2) * p.element_size(),
+                p[0, 0, 0].numel() * p.element_size())))
+            B.check(lib.cmb_compact_rows(bases, lp, len(part), B.ptr(table), B.ptr(start), B.ptr(path), B.ptr(counts), ip,
+                                         B.ptr(B.status_buffer(dev)), B.stream_ptr()), "compact_rows")
