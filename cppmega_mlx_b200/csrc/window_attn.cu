@@ -8,21 +8,23 @@
 // Row i stands at position P_i and sees key j when j <= P_i, j is a valid key, and P_i - j < window or j < ns; drafted node n
 // stands at prefix + (number of its ancestors) and sees of the other nodes only those in its 64-bit word.
 //
-// Work of a CTA: 128-row tiles (window_attn.h: g heads x 128 / g queries) against 128-key tiles.
+// Work of a CTA: 128-row tiles (window_attn.h: g heads x 128 / g queries) against tiles of 64 or 128 keys.
 //
 //   S = Q.K^T       tcgen05.mma 128 x n x 16, fp32 in TMEM (n = the tile's keys, rounded up to 16: the few first tokens and the
 //                   last tile cost what they hold)
-//   P = exp2(S c - m)   one row per thread; read from TMEM, written back over S as bf16: P is the next product's A operand
-//                   and never leaves the tensor memory.  P's rounding to bf16 (half a step, 2^-8) is that of the product's
-//                   operand type; the row's sum is of the unrounded values in fp32.
-//   O += P.V        A from TMEM, V read MN-major in place, accumulator resident in TMEM
+//   P = exp2(S c - m)   one row per thread, its scores in registers (setmaxnreg), P written back to TMEM as bf16.  P's rounding (half
+//                   a step, 2^-8) is that of the product's operand type; the row's sum is of the unrounded values in fp32.
+//   O += P.V        A from TMEM (from shared memory, P and its reads would cost half as much shared-memory bandwidth again as
+//                   the K, V and Q reads that already take most of it), V read MN-major in place, accumulator resident in TMEM
 //
 // The running maximum m moves only when a tile exceeds it by 2^8 (numerator and denominator share it, so the result does not
 // depend on when); O is rescaled in TMEM only then.  Two streams (softmax warp group + MMA-issuing warp each) share the CTA so
 // that one stream's products run under the other's exponentials:
 //
 //   ROWS   the streams are two row tiles that share every key tile (long sequences: the bound is the exponentials and the
-//          tensor pipe, so key tiles should be fetched once for as many rows as fit)
+//          tensor pipe, so key tiles should be fetched once for as many rows as fit).  Tiles of 64 keys, so that a stream has two
+//          score buffers and the next scores run under this tile's exponentials: with one buffer of 128 (P lies over S, and O and
+//          S of two streams fill the TMEM) every tile waited for its product and the next scores, 2000 of 5200 clocks.
 //   KEYS   the streams are the even and odd key tiles of one row tile, joined at the end (<= 128 rows: decode, small trees; the
 //          bound is reading the cache, so the shared memory goes to tiles in flight).  With <= 32 (64) rows the tile holds
 //          them four (two) times in its TMEM lane quarters and each copy takes a quarter (half) of a tile's keys, because a
@@ -33,7 +35,7 @@
 // Rows of V that no row may see (past a sequence's end, padding, pages handed on to others) may hold anything, NaN included:
 // a helper warp zeroes them in shared memory before they are multiplied with P's zeros.
 //
-// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 TMA producer, 9 / 10 MMA of stream 0 / 1, 11 the V helper.  Every wait is
+// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 TMA producer, 9 / 10 scores and 12 / 13 products of stream 0 / 1, 11 the V helper.  Every wait is
 // bounded (sm100.cuh).
 #include <cstring>
 
@@ -41,7 +43,7 @@
 
 namespace cmb {
 
-constexpr int WA_THREADS = 384;
+constexpr int WA_THREADS = 512;          // 14 warps with a role, in whole warp groups
 constexpr float WA_RESCALE = 8.f;        // log2 units a tile's maximum may exceed the reference before O is rescaled
 constexpr int WA_CTL = 3072;             // barriers (first 1 KB), (max, sum) of every row and stream (2 KB)
 
@@ -70,15 +72,19 @@ struct WindowParams {
 
 template <int DB, bool KEYS>
 struct WindowCfg {
+  static constexpr int BN = KEYS ? 128 : 64;             // keys of a tile
+  static constexpr int BUFS = KEYS ? 1 : 2;              // score buffers of a stream
+  static constexpr int KBLK = BN * 128;                  // bytes of a [BN keys x 64 columns] block
   static constexpr int Q_BYTES = (KEYS ? 1 : 2) * DB * WA_BLK;
-  static constexpr int NK = DB == 2 ? 3 : 4;
-  static constexpr int NV = DB == 2 ? (KEYS ? 3 : 2) : 4;
-  static constexpr int STAGE = DB * WA_BLK;
+  static constexpr int NK = KEYS ? (DB == 2 ? 3 : 4) : (DB == 2 ? 5 : 8);
+  static constexpr int NV = NK;
+  static constexpr int STAGE = DB * KBLK;
   static constexpr int SMEM_BYTES = Q_BYTES + (NK + NV) * STAGE + WA_CTL;
   static constexpr int PART_PITCH = DB * 64 + 4;         // floats; rows 16 bytes apart in banks
   static_assert(SMEM_BYTES <= 232448, "shared memory");
   static_assert(!KEYS || 256 * PART_PITCH * 4 <= (NK + NV) * STAGE, "partial results reuse the rings");
-  static constexpr int O_COL = 0, S_COL = 256;           // stream s: O at s * 128, S (and P over it) at 256 + s * 128
+  // TMEM: stream s has O at 128 s and its scores at 256 + 128 s (+ 64 for ROWS' second buffer); P is written over the scores
+  static constexpr int O_STEP = 128, S_COL = 256, S_STEP = 128;
 };
 
 // One row's place in the problem.
@@ -134,7 +140,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const WindowParams p) {
   using Cfg = WindowCfg<DB, KEYS>;
-  constexpr int NK = Cfg::NK, NV = Cfg::NV;
+  constexpr int NK = Cfg::NK, NV = Cfg::NV, BN = Cfg::BN, BUFS = Cfg::BUFS;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {   // swizzled TMA / MMA tiles need 1024-byte aligned buffers
     if (threadIdx.x == 0 && p.status != nullptr && atomicCAS(p.status, 0, ST_BAD_ARGUMENT) == 0) p.status[1] = -1024;
@@ -150,10 +156,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* v_full = k_empty + NK;         // [NV] landed
   uint64_t* v_ready = v_full + NV;         // [NV] unseen rows zeroed
   uint64_t* v_empty = v_ready + NV;        // [NV]
-  uint64_t* s_full = v_empty + NV;         // [2]
-  uint64_t* p_full = s_full + 2;           // [2]
-  uint64_t* pv_done = p_full + 2;          // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  uint64_t* s_full = v_empty + NV;         // [stream][buffer]
+  uint64_t* p_full = s_full + 4;           // [stream][buffer] P written
+  uint64_t* pv_done = p_full + 4;          // [stream][buffer] P read, O added to
+  uint64_t* go = pv_done + 4;              // ROWS: stream 0 is through its first tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(go + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* xml = reinterpret_cast<float2*>(ctl + 1024);   // [2 streams][128 rows] (max, sum)
 
@@ -179,7 +186,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     pmin = p.T - p.S + s_first;
     pmax = p.T - p.S + s_last;
   }
-  const WaRange<128> R(pmin, pmax, klim, p.window, p.ns, p.table != nullptr ? p.box_k : 1);
+  const WaRange<BN> R(pmin, pmax, klim, p.window, p.ns, p.table != nullptr ? p.box_k : 1);
   const int per = (R.n_t + p.splits - 1) / p.splits;
   const int t0 = min(R.n_t, split * per), t1 = min(R.n_t, t0 + per);
   const int NT = t1 - t0;
@@ -196,11 +203,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       mbar_init(&v_ready[i], 1);
       mbar_init(&v_empty[i], readers);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
       mbar_init(&pv_done[i], 1);
     }
+    mbar_init(go, 1);
     *abort_flag = 0;
     fence_mbar_init();
     if (p.lengths != nullptr && status != nullptr) {   // a length that the cache cannot hold
@@ -219,7 +227,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-
+  // KEYS keeps 128 scores of a row in registers: 256 x 176 + 256 x 80 = the 512 x 128 that the block was launched with
+  if (warp >= 8) {
+  if constexpr (KEYS) wa_fewer_registers<80>();
   if (warp == 8) {
     // ---------------------------------------------------------------- TMA producer (a box per lane)
     if (lane == 0) {
@@ -237,8 +247,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         KEYS ? s_first : s_first + t * p.box_q, hk, b);
       }
       __syncwarp();
-      // lane i moves box i / DB of each tile, column block i % DB; 128 / box_k boxes of <= 2 column blocks fit in 32 lanes
-      // (box_k >= 8).  The page is looked up one tile ahead.
+      // lane i moves box i / DB of each tile, column block i % DB; BN / box_k boxes of <= 2 column blocks fit in 32 lanes
+      // (box_k >= 8).
       const int my_box = lane / DB, my_kb = lane % DB;
       auto page_of = [&](int i) {
         if (i >= t1) return 0;
@@ -256,30 +266,32 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         return id;
       };
-      int page = page_of(t0);
-      for (int i = t0; i < t1; ++i) {
-        const int n = i - t0, kst = n % NK, vst = n % NV;
+      auto load = [&](int i, uint8_t* ring, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int depth, int page) {
+        const int n = i - t0, st = n % depth;
         const WaTile t = R.tile(i);
         const int boxes = (t.k1 - t.k0 + p.box_k - 1) / p.box_k;
-        const uint32_t bytes = static_cast<uint32_t>(boxes) * p.box_k * 128 * DB;
-        const int next_page = page_of(i + 1);
-        const int j = t.k0 + my_box * p.box_k;
-        const int in_page = p.table != nullptr ? j % p.page : j;
-        const uint32_t off = my_kb * WA_BLK + my_box * p.box_k * 128;
         bool ok = true;
         if (lane == 0) {
-          ok = mbar_wait(&k_empty[kst], ((n / NK) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
-          if (ok) mbar_arrive_expect_tx(&k_full[kst], bytes);
+          ok = mbar_wait(&empty[st], ((n / depth) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
+          if (ok) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(boxes) * p.box_k * 128 * DB);
         }
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        if (my_box < boxes) tma_load_4d(ks + kst * Cfg::STAGE + off, &tmK, &k_full[kst], my_kb * 64, in_page, hk, page);
-        if (lane == 0) {
-          ok = mbar_wait(&v_empty[vst], ((n / NV) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
-          if (ok) mbar_arrive_expect_tx(&v_full[vst], bytes);
-        }
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        if (my_box < boxes) tma_load_4d(vs + vst * Cfg::STAGE + off, &tmV, &v_full[vst], my_kb * 64, in_page, hk, page);
-        page = next_page;
+        if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
+        const int j = t.k0 + my_box * p.box_k;
+        if (my_box < boxes)
+          tma_load_4d(ring + st * Cfg::STAGE + my_kb * Cfg::KBLK + my_box * p.box_k * 128, map, &full[st], my_kb * 64,
+                      p.table != nullptr ? j % p.page : j, hk, page);
+        return true;
+      };
+      // The keys run a tile ahead of the values: the next scores are wanted before this tile's product, and a stage of values
+      // is free later than one of keys.  Pages are looked up a tile before they are needed.
+      int page0 = page_of(t0), page1 = page_of(t0 + 1);
+      bool ok = load(t0, ks, &tmK, k_full, k_empty, NK, page0);
+      for (int i = t0; i < t1 && ok; ++i) {
+        const int page2 = page_of(i + 2);
+        if (i + 1 < t1) ok = load(i + 1, ks, &tmK, k_full, k_empty, NK, page1);
+        ok = ok && load(i, vs, &tmV, v_full, v_empty, NV, page0);
+        page0 = page1;
+        page1 = page2;
       }
     }
   } else if (warp == 11) {
@@ -296,10 +308,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       bool ok = true;
       if (lane == 0) ok = mbar_wait(&v_full[st], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL);
       if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      const bool tail = t.k1 - t.k0 < 128, head = i >= R.n_s && t.k0 < R.wtrue;
+      const bool tail = t.k1 - t.k0 < BN, head = i >= R.n_s && t.k0 < R.wtrue;
       const bool drafted = p.tree != nullptr && t.k1 > prefix;
       if (tail || head || drafted) {
-        for (int r = lane; r < 128; r += 32) {
+        for (int r = lane; r < BN; r += 32) {
           const int j = t.k0 + r;
           const bool seen = j < t.k1 && (j >= R.wtrue || j < p.ns) &&
                             (!drafted || j < prefix || (j - prefix < 64 && ((nodes_any >> (j - prefix)) & 1ull)));
@@ -308,7 +320,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             for (int kb = 0; kb < DB; ++kb)
 #pragma unroll
               for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(vs + st * Cfg::STAGE + kb * WA_BLK + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(vs + st * Cfg::STAGE + kb * Cfg::KBLK + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
@@ -316,109 +328,159 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_ready[st]);
     }
-  } else if (warp == 9 || warp == 10) {
-    // ---------------------------------------------------------------- MMA issuer of one stream (one thread)
-    const int st = warp - 9;
-    if (lane == 0 && NT > 0 && (st == 0 || two)) {
-      constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
-      const uint32_t q_addr = smem_u32(qs) + (KEYS ? 0 : st * DB * WA_BLK), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
-      const uint32_t s_col = tmem_base + Cfg::S_COL + st * 128, o_col = tmem_base + Cfg::O_COL + st * 128;
-      bool ok = mbar_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
+  } else if (warp < 14) {
+    // ---------------------------------------------------------------- MMA issuers: a thread each for the scores (warps 9, 10)
+    // and the products (12, 13) of each stream.  One thread for both would hold a finished P back behind the scores of two tiles
+    // later: an issuing thread advances no faster than the tensor pipe takes its instructions.
+    const bool scores = warp < 11;
+    const int st = scores ? warp - 9 : warp - 12;
+    if (lane == 0 && (st == 0 || two)) {
+      // one descriptor each, advanced by adding to its address field (16-byte units)
+      const uint32_t s_col = tmem_base + Cfg::S_COL + st * Cfg::S_STEP, o_col = tmem_base + Cfg::O_STEP * st;
+      const int first = t0 + (KEYS ? st : 0), step = KEYS ? 2 : 1;
       int c = 0;                                       // tiles of this stream so far
-      for (int i = t0 + (KEYS ? st : 0); i < t1 && ok; i += KEYS ? 2 : 1, ++c) {
-        const int n = i - t0, kst = n % NK, vst = n % NV;
-        const WaTile t = R.tile(i);
-        const int k16 = (t.k1 - t.k0 + 15) >> 4;
-        const uint32_t idesc_s = make_idesc(128, k16 * 16, 1, 1, 0, 0);
-        if (!mbar_wait(&k_full[kst], (n / NK) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
-        // S takes the place of the previous tile's P: wait until that product has read it
-        if (c > 0 && !mbar_wait(&pv_done[st], (c - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
-        tc_fence_after();
+      if (scores) {
+        const uint64_t q_desc = make_smem_desc_sw128(smem_u32(qs) + (KEYS ? 0 : st * DB * WA_BLK), 16, 1024);
+        const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ks), 16, 1024);
+        bool ok = first >= t1 || mbar_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
+        if (!KEYS && st == 1 && first < t1) ok = ok && mbar_wait(go, 0, abort_flag, status, ST_TIMEOUT_FULL);
+        for (int i = first; i < t1 && ok; i += step, ++c) {
+          const int n = i - t0, kst = n % NK, buf = c % BUFS;
+          const WaTile t = R.tile(i);
+          const uint32_t idesc_s = make_idesc(128, ((t.k1 - t.k0 + 15) >> 4) * 16, 1, 1, 0, 0);
+          const uint64_t kd = k_desc + static_cast<uint32_t>(kst * (Cfg::STAGE >> 4));
+          const uint32_t d = s_col + buf * 64;
+          // the scores take the place of an earlier tile's P, once the product has read it
+          if (c >= BUFS && !mbar_wait(&pv_done[st * 2 + buf], (c / BUFS - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
+          if (!mbar_wait(&k_full[kst], (n / NK) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
+          tc_fence_after();
 #pragma unroll
-        for (int kb = 0; kb < DB; ++kb)
+          for (int kb = 0; kb < DB; ++kb)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16(s_col, make_smem_desc_sw128(q_addr + kb * WA_BLK + k * 32, 16, 1024),
-                     make_smem_desc_sw128(k_addr + kst * Cfg::STAGE + kb * WA_BLK + k * 32, 16, 1024), idesc_s,
-                     (kb > 0 || k > 0) ? 1u : 0u);
-        umma_commit(&k_empty[kst]);
-        umma_commit(&s_full[st]);
-        if (!mbar_wait(&v_ready[vst], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
-        if (!mbar_wait(&p_full[st], c & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
-        tc_fence_after();
-        for (int k = 0; k < k16; ++k)
-          umma_f16_ts(o_col, s_col + k * 8, make_smem_desc_sw128(v_addr + vst * Cfg::STAGE + k * 2048, WA_BLK, 1024), idesc_o,
-                      (c > 0 || k > 0) ? 1u : 0u);
-        umma_commit(&v_empty[vst]);
-        umma_commit(&pv_done[st]);
+            for (int k = 0; k < 4; ++k)
+              umma_f16(d, q_desc + ((kb * WA_BLK + k * 32) >> 4), kd + ((kb * Cfg::KBLK + k * 32) >> 4), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&k_empty[kst]);
+          umma_commit(&s_full[st * 2 + buf]);
+        }
+      } else {
+        constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
+        const uint64_t v_desc = make_smem_desc_sw128(smem_u32(vs), Cfg::KBLK, 1024);
+        for (int i = first; i < t1; i += step, ++c) {
+          const int n = i - t0, vst = n % NV, buf = c % BUFS;
+          const WaTile t = R.tile(i);
+          const int k16 = (t.k1 - t.k0 + 15) >> 4;
+          const uint64_t vd = v_desc + static_cast<uint32_t>(vst * (Cfg::STAGE >> 4));
+          const uint32_t a = s_col + buf * 64;
+          if (!mbar_wait(&v_ready[vst], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
+          if (!mbar_wait(&p_full[st * 2 + buf], (c / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
+          tc_fence_after();
+          umma_f16_ts(o_col, a, vd, idesc_o, c > 0 ? 1u : 0u);
+          if (k16 == BN / 16) {
+#pragma unroll
+            for (int k = 1; k < BN / 16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
+          } else {
+            for (int k = 1; k < k16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
+          }
+          umma_commit(&v_empty[vst]);
+          umma_commit(&pv_done[st * 2 + buf]);
+        }
       }
     }
+  }
   } else {
     // ---------------------------------------------------------------- softmax and epilogue (a warp group per stream)
+    if constexpr (KEYS) wa_more_registers<176>();
     const int st = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem_base + lane_addr + Cfg::S_COL + st * 128, o_addr = tmem_base + lane_addr + Cfg::O_COL + st * 128;
+    const uint32_t s_base = tmem_base + lane_addr + Cfg::S_COL + st * Cfg::S_STEP, o_addr = tmem_base + lane_addr + Cfg::O_STEP * st;
     const bool active = st == 0 || two;
     const int copy = KEYS ? row / p.copy_rows : 0;
     const int rr = KEYS ? row - copy * p.copy_rows : row;          // row within the tile
     const WindowRow w = window_row(p, rr, KEYS ? s_first : s_first + st * p.box_q, hk, b, klim, prefix);
-    const int c_first = KEYS ? copy * (4 / p.copies) : 0;          // this thread's 32-key chunks of a tile
-    const int c_count = KEYS ? 4 / p.copies : 4;
+    const int c_first = KEYS ? copy * (BN / 32 / p.copies) : 0;          // this thread's 32-key chunks of a tile
+    constexpr int CH = BN / 32;
+    const int c_count = KEYS ? CH / p.copies : CH;
     const bool warp_ok = __any_sync(0xffffffffu, w.ok);
+    // what every row of the warp sees (rows that are not ok are never read): most tiles need no mask
+    const int all_upto = __reduce_min_sync(0xffffffffu, w.ok ? w.plim : 0x7fffffff);
+    const int all_from = __reduce_max_sync(0xffffffffu, w.ok ? w.lo : -0x7fffffff);
     float m_ref = -INFINITY, l_sum = 0.f;
     bool ok = active;
     int c = 0;
     if (active) {
-      for (int i = t0 + (KEYS ? st : 0); i < t1; i += KEYS ? 2 : 1, ++c) {
-        const WaTile t = R.tile(i);
-        const int chunks = (t.k1 - t.k0 + 31) >> 5;                // 32-key chunks that the tile has
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[st], c & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL))) {
+      const int first = t0 + (KEYS ? st : 0), step = KEYS ? 2 : 1;
+      auto scores_in = [&](int at) {         // tile `at` of this stream: are its scores there?
+        return static_cast<bool>(__all_sync(
+            0xffffffffu, mbar_wait(&s_full[st * 2 + at % BUFS], (at / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)));
+      };
+      uint32_t x[CH][32];                    // the scores of this thread's chunks
+      auto load = [&](int e, int chunks, int at) {
+        if (e < c_count && c_first + e < chunks) tmem_ld_x32(s_base + (at % BUFS) * 64 + (c_first + e) * 32, x[e]);
+      };
+      for (int i = first; i < t1 && !warp_ok; i += step, ++c) {    // no rows: this warp only keeps step
+        if (!scores_in(c)) {
           ok = false;
           break;
         }
+        mbar_arrive(&p_full[st * 2 + c % BUFS]);
+        if (!KEYS && c == 0 && threadIdx.x == 0) mbar_arrive(go);
+      }
+      WaTile t = R.tile(first);
+      int chunks = (t.k1 - t.k0 + 31) >> 5;  // 32-key chunks that the tile has
+      if (warp_ok && first < t1) {
+        ok = scores_in(0);
         tc_fence_after();
-        if (warp_ok) {
-          uint32_t x0[32], x1[32];
-          auto load = [&](int ch) {          // chunks ch and ch + 1
-            if (ch < chunks) tmem_ld_x32(s_addr + ch * 32, x0);
-            if (c_count > 1 && ch + 1 < chunks) tmem_ld_x32(s_addr + ch * 32 + 32, x1);
-            tmem_wait_ld();
-          };
-          auto masked_max = [&](const uint32_t (&x)[32], unsigned word) {
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (__all_sync(0xffffffffu, word == 0xffffffffu)) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(x[e]));
-            } else {
+        for (int e = 0; e < CH; ++e)
+          if (ok) load(e, chunks, 0);
+        tmem_wait_ld();
+      }
+      for (int i = first; i < t1 && warp_ok && ok; i += step, ++c) {
+        const int buf = c % BUFS;
+        const uint32_t s_addr = s_base + buf * 64;
+        const bool whole = t.k1 - t.k0 == BN && t.k1 - 1 <= all_upto && (t.k0 >= all_from || t.k1 <= p.ns);
+        if (!whole) {                        // what is masked may be NaN: selected, not added to
 #pragma unroll
-              for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], ((word >> e) & 1u) ? __uint_as_float(x[e]) : -INFINITY);
-            }
-            return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          };
-          unsigned words[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            words[e] = e < c_count && c_first + e < chunks ? window_word(p, w, t.k0 + (c_first + e) * 32, t.k1, prefix) : 0u;
-          float mx = -INFINITY;
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
+          for (int e = 0; e < CH; ++e) {
             if (e < c_count && c_first + e < chunks) {
-              load(c_first + e);
-              mx = fmaxf(mx, masked_max(x0, words[e]));
-              if (c_count > 1 && c_first + e + 1 < chunks) mx = fmaxf(mx, masked_max(x1, words[e + 1]));
+              const unsigned word = window_word(p, w, t.k0 + (c_first + e) * 32, t.k1, prefix);
+#pragma unroll
+              for (int i2 = 0; i2 < 32; ++i2) x[e][i2] = (word >> i2) & 1u ? x[e][i2] : 0xff800000u;
             }
           }
-          mx *= p.scale_log2;
+        }
+        float m8[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+          if (e < c_count && c_first + e < chunks) {
+#pragma unroll
+            for (int i2 = 0; i2 < 32; i2 += 16)
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                m8[u] = fmaxf(fmaxf(m8[u], __uint_as_float(x[e][i2 + 2 * u])), __uint_as_float(x[e][i2 + 2 * u + 1]));
+          }
+        }
+        const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * p.scale_log2;
+        const bool moved = mx > m_ref + WA_RESCALE || (m_ref == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, moved)) {
           float alpha = 1.f;
-          if (mx > m_ref + WA_RESCALE || (m_ref == -INFINITY && mx > -INFINITY)) {
+          if (moved) {
             alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
             m_ref = mx;
             l_sum *= alpha;
           }
-          // the scores of tile c were issued after the product of tile c - 1 had completed, so O is free to be rescaled
-          if (c > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
+          if (c > 0) {
+            // O is rescaled when the previous tile's product has completed (KEYS: these scores were issued after it)
+            if (BUFS > 1 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status,
+                                                               ST_TIMEOUT_TMEM_EMPTY))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
             for (int cc = 0; cc < DB * 2; ++cc) {
               uint32_t o[32];
               tmem_ld_x32(o_addr + cc * 32, o);
@@ -428,50 +490,60 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               tmem_st_x32(o_addr + cc * 32, o);
             }
           }
-          const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;   // a row without a key yet: exp2(-inf - 0) = 0
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          auto put = [&](const uint32_t (&x)[32], unsigned word, int ch) {
-            uint32_t w16[16];
-            const bool full = __all_sync(0xffffffffu, word == 0xffffffffu);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float a0 = fmaf(__uint_as_float(x[2 * e]), p.scale_log2, neg_m);
-              float a1 = fmaf(__uint_as_float(x[2 * e + 1]), p.scale_log2, neg_m);
-              if (!full) {
-                a0 = ((word >> (2 * e)) & 1u) ? a0 : -INFINITY;
-                a1 = ((word >> (2 * e + 1)) & 1u) ? a1 : -INFINITY;
-              }
-              const float p0 = exp2f(a0), p1 = exp2f(a1);
-              acc[(2 * e) & 3] += p0;
-              acc[(2 * e + 1) & 3] += p1;
-              w16[e] = pack_bf16x2(p0, p1);
-            }
-            tmem_st_x16(s_addr + ch * 16, w16);
-          };
-          // P of chunk ch covers columns 16 ch .. 16 ch + 15 of the scores, all read by now (the row's lane is this thread's)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            if (e < c_count && c_first + e < chunks) {
-              if (c_count > 2) load(c_first + e);
-              put(x0, words[e], c_first + e);
-              if (c_count > 1 && c_first + e + 1 < chunks) put(x1, words[e + 1], c_first + e + 1);
-            }
-          }
-          if (KEYS && p.copies > 1) {        // the other copies' chunks count nothing here
-            uint32_t z[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) z[e] = 0u;
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch)
-              if (ch < chunks && (ch < c_first || ch >= c_first + c_count)) tmem_st_x16(s_addr + ch * 16, z);
-          }
-          l_sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-          tmem_wait_st();
         }
+        // a row without a key yet: exp2(-inf - 0) = 0
+        const float2 neg_m = m_ref == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m_ref, -m_ref);
+        const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto probs = [&](int e) {
+          // P of chunk ch is columns 16 ch .. 16 ch + 15 of the scores, all read by now (the row's lane is this thread's)
+          if (e < c_count && c_first + e < chunks) {
+            uint32_t w16[16];
+#pragma unroll
+            for (int i2 = 0; i2 < 16; ++i2) {
+              float2 v = fma2(make_float2(__uint_as_float(x[e][2 * i2]), __uint_as_float(x[e][2 * i2 + 1])), c2, neg_m);
+              v.x = exp2f(v.x);
+              v.y = exp2f(v.y);
+              acc[i2 & 1] = add2(acc[i2 & 1], v);
+              w16[i2] = pack_bf16x2(v.x, v.y);
+            }
+            tmem_st_x16(s_addr + (c_first + e) * 16, w16);
+          }
+        };
+        const bool more = i + step < t1;
+        const WaTile tn = R.tile(i + step);
+        const int chunks_n = (tn.k1 - tn.k0 + 31) >> 5;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) probs(e);
+        if (KEYS && p.copies > 1) {          // the other copies' chunks count nothing here
+          uint32_t z[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[e] = 0u;
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch)
+            if (ch < chunks && (ch < c_first || ch >= c_first + c_count)) tmem_st_x16(s_addr + ch * 16, z);
+        }
+        tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[st]);
+        mbar_arrive(&p_full[st * 2 + buf]);
+        if (!KEYS && c == 0 && threadIdx.x == 0) mbar_arrive(go);
+        if (more) {
+          if (!scores_in(c + 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int e = 0; e < CH; ++e) load(e, chunks_n, c + 1);
+        }
+        l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+        tmem_wait_ld();
+        t = tn;
+        chunks = chunks_n;
       }
-      if (c > 0 && ok) ok = mbar_wait(&pv_done[st], (c - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+      // (the product before the last completes before it: one thread issued both)
+      if (c > 0 && ok)
+        ok = mbar_wait(&pv_done[st * 2 + (c - 1) % BUFS], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
@@ -765,6 +837,7 @@ extern "C" int cmb_window_fwd(const void* q, const void* k, const void* v, const
   if (table != nullptr && (p.page <= 0 || p.page % p.box_k || p.num_pages <= 0 || p.table_w <= 0 ||
                            static_cast<long long>(p.table_w) * p.page < p.T))
     return 1;
+  if (p.S * static_cast<long long>(p.g) > 128 && p.box_k > 64) return 1;   // a tile of 64 keys
   if (p.splits > 1 && (ws_o == nullptr || ws_ml == nullptr)) return 1;
   if ((lp[9] | lp[10] | lp[11]) & 7 || (reinterpret_cast<uintptr_t>(out) & 15)) return 1;
   const int rows = p.S * p.g;                              // S <= 2^24 rows is checked by the caller's shapes

@@ -11,6 +11,9 @@
 // The sinks' gradient, -sum_i p_i,sink (do_i . o_i), would feel the rounding of o to bf16 (the sum has few outputs and both signs), so
 // DQ adds up do_i . o_i = sum_j p_ij dP_ij itself, in fp32, where sinks are trained.
 //
+// Rows that see few keys have an o as large as single values, and dP - delta cancels: there o's rounding would be most of dS's error.
+// Where a row tile sees at most one sub-tile of keys, DQ (launched first) takes delta from sum_j p_ij dP_ij too, and leaves it for DKV.
+//
 // dK and dQ carry the softmax scale once, at the end.  P and dS are rounded to bf16 (half a step, 2^-8: the operand type of the
 // gradient products) and written back over S and dP in TMEM, where they are the A operands; dQ, dK, dV accumulate there in fp32.
 // One thread issues every product in order; two warp groups take alternate sub-tiles, so that one's exponentials run under
@@ -37,7 +40,7 @@ struct WindowBwdParams {
   float scale, scale_log2;
   int window, ns;
   const int* lengths;
-  const float2* stats;                     // [B, Hk, S * g] (lse * log2 e, delta) of packed rows; lse = +inf: sees nothing
+  float2* stats;                           // [B, Hk, S * g] (lse * log2 e, delta) of packed rows; lse = +inf: sees nothing
   __nv_bfloat16 *o1, *o2;                  // DQ: dq, -;  DKV: dk, dv
   long long o1_sb, o1_ss, o1_sh, o2_sb, o2_ss, o2_sh;
   int sink_tiles, sink_splits;             // DKV: the first sink_tiles key tiles are split
@@ -231,7 +234,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     if (lane == 0 && NT > 0) {
       constexpr uint32_t idesc_x = make_idesc(128, WB_SUB, 1, 1, 0, 0);
       constexpr uint32_t idesc_g = make_idesc(128, DB * 64, 1, 1, 0, 1);
-      const uint32_t r1a = smem_u32(r1s), r2a = smem_u32(r2s), tsa = smem_u32(ts);
+      // descriptors are advanced by adding to their address field (16-byte units)
+      const uint64_t r1d = make_smem_desc_sw128(smem_u32(r1s), 16, 1024), r2d = make_smem_desc_sw128(smem_u32(r2s), 16, 1024);
+      const uint64_t td = make_smem_desc_sw128(smem_u32(ts), 16, 1024), gd = make_smem_desc_sw128(smem_u32(ts), WB_SBLK, 1024);
       bool ok = mbar_wait(r_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
       auto issue_scores = [&](int n) {
         const int st = n % WB_NS, buf = n & 1;
@@ -239,19 +244,18 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         // the buffer holds P and dS of sub-tile n - 2 until its gradient products have read them
         if (n >= 2 && !mbar_wait(&g_done[buf], ((n >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
         tc_fence_after();
-        const uint32_t t1 = tsa + st * Cfg::STAGE, t2 = t1 + DB * WB_SBLK, x = tmem_base + Cfg::X_COL + buf * 128;
+        const uint32_t x = tmem_base + Cfg::X_COL + buf * 128;
+        const uint64_t t1 = td + static_cast<uint32_t>(st * (Cfg::STAGE >> 4)), t2 = t1 + ((DB * WB_SBLK) >> 4);
 #pragma unroll
         for (int kb = 0; kb < DB; ++kb)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16(x, make_smem_desc_sw128(r1a + kb * WA_BLK + k * 32, 16, 1024),
-                     make_smem_desc_sw128(t1 + kb * WB_SBLK + k * 32, 16, 1024), idesc_x, (kb > 0 || k > 0) ? 1u : 0u);
+            umma_f16(x, r1d + ((kb * WA_BLK + k * 32) >> 4), t1 + ((kb * WB_SBLK + k * 32) >> 4), idesc_x, (kb > 0 || k > 0) ? 1u : 0u);
 #pragma unroll
         for (int kb = 0; kb < DB; ++kb)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16(x + 64, make_smem_desc_sw128(r2a + kb * WA_BLK + k * 32, 16, 1024),
-                     make_smem_desc_sw128(t2 + kb * WB_SBLK + k * 32, 16, 1024), idesc_x, (kb > 0 || k > 0) ? 1u : 0u);
+            umma_f16(x + 64, r2d + ((kb * WA_BLK + k * 32) >> 4), t2 + ((kb * WB_SBLK + k * 32) >> 4), idesc_x, (kb > 0 || k > 0) ? 1u : 0u);
         umma_commit(&x_full[buf]);
         return true;
       };
@@ -261,14 +265,12 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         const int st = n % WB_NS, buf = n & 1;
         if (!mbar_wait(&a_full[buf], (n >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
         tc_fence_after();
-        const uint32_t t1 = tsa + st * Cfg::STAGE, t2 = t1 + DB * WB_SBLK, x = tmem_base + Cfg::X_COL + buf * 128;
+        const uint32_t x = tmem_base + Cfg::X_COL + buf * 128;
+        const uint64_t t1 = gd + static_cast<uint32_t>(st * (Cfg::STAGE >> 4)), t2 = t1 + ((DB * WB_SBLK) >> 4);
 #pragma unroll
         for (int k = 0; k < WB_SUB / 16; ++k) {
-          if (MODE == WB_DKV)
-            umma_f16_ts(tmem_base + Cfg::O2_COL, x + k * 8, make_smem_desc_sw128(t2 + k * 2048, WB_SBLK, 1024), idesc_g,
-                        (n > 0 || k > 0) ? 1u : 0u);
-          umma_f16_ts(tmem_base + Cfg::O1_COL, x + 64 + k * 8, make_smem_desc_sw128(t1 + k * 2048, WB_SBLK, 1024), idesc_g,
-                      (n > 0 || k > 0) ? 1u : 0u);
+          if (MODE == WB_DKV) umma_f16_ts(tmem_base + Cfg::O2_COL, x + k * 8, t2 + ((k * 2048) >> 4), idesc_g, (n > 0 || k > 0) ? 1u : 0u);
+          umma_f16_ts(tmem_base + Cfg::O1_COL, x + 64 + k * 8, t1 + ((k * 2048) >> 4), idesc_g, (n > 0 || k > 0) ? 1u : 0u);
         }
         umma_commit(&t_empty[st]);
         umma_commit(&g_done[buf]);
@@ -319,6 +321,23 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         break;
       }
       tc_fence_after();
+      if (MODE == WB_DQ && NT == 1) {
+        float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          uint32_t x1[32], x2[32];
+          tmem_ld_x32(x_addr + 32 * i, x1);
+          tmem_ld_x32(x_addr + 64 + 32 * i, x2);
+          tmem_wait_ld();
+          const unsigned word = i ? words[1] : words[0];
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if ((word >> e) & 1u) sum[e & 1] = fmaf(exp2f(fmaf(__uint_as_float(x1[e]), p.scale_log2, -lse2)), __uint_as_float(x2[e]), sum[e & 1]);
+        }
+        delta = sum[0] + sum[1];
+        if (row_ok)
+          p.stats[(static_cast<long long>(b) * p.Hk + hk) * p.S * p.g + static_cast<long long>(qi) * p.g + (row - ql * p.g)].y = delta;
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t x1[32], x2[32], pw[16], dw[16];
@@ -534,7 +553,7 @@ extern "C" int cmb_window_bwd(const void* q, const void* k, const void* v, const
   p.sub_q = cmb::WB_SUB / p.g;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
   p.window = ip[7]; p.ns = ip[8]; p.lengths = lengths;
-  p.stats = reinterpret_cast<const float2*>(stats);
+  p.stats = reinterpret_cast<float2*>(stats);
   p.sink_tiles = ip[9]; p.sink_splits = ip[10]; p.part = part; p.status = status;
   if (p.sink_tiles < 0 || p.sink_tiles > key_tiles || p.sink_splits < 1 || (p.sink_splits > 1 && part == nullptr)) return 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -555,6 +574,22 @@ extern "C" int cmb_window_bwd(const void* q, const void* k, const void* v, const
     if (!rc) rc = cmb_host::make_tmap_rows(&mv, v, Dv, T, Hk, B, lp[7], lp[8], lp[6], box_k);
     return rc;
   };
+  if (dq != nullptr) {
+    CUtensorMap mq, mo, mk, mv;
+    int rc = maps(mq, mo, mk, mv, p.box_q, cmb::WB_SUB);
+    if (rc) return rc;
+    cmb::WindowBwdParams pq = p;
+    pq.o1 = static_cast<__nv_bfloat16*>(dq); pq.o1_sb = lp[15]; pq.o1_ss = lp[16]; pq.o1_sh = lp[17];
+    const CUtensorMap m[4] = {mq, mo, mk, mv};
+    const int gx = (S + p.box_q - 1) / p.box_q;
+    if (sink_part != nullptr) {
+      pq.sinks = sinks; pq.sink_part = sink_part;
+      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2, true>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1, true>(m, pq, gx, B, st);
+    } else {
+      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1>(m, pq, gx, B, st);
+    }
+    if (rc) return rc + 20000;
+  }
   if (dk != nullptr) {
     CUtensorMap mq, mo, mk, mv;
     int rc = maps(mq, mo, mk, mv, p.sub_q, 128);
@@ -575,22 +610,6 @@ extern "C" int cmb_window_bwd(const void* q, const void* k, const void* v, const
       cmb::window_join_kernel<<<static_cast<unsigned>((j.n + 255) / 256), 256, 0, st>>>(j);
       if (cudaGetLastError() != cudaSuccess) return 104;
     }
-  }
-  if (dq != nullptr) {
-    CUtensorMap mq, mo, mk, mv;
-    int rc = maps(mq, mo, mk, mv, p.box_q, cmb::WB_SUB);
-    if (rc) return rc;
-    cmb::WindowBwdParams pq = p;
-    pq.o1 = static_cast<__nv_bfloat16*>(dq); pq.o1_sb = lp[15]; pq.o1_ss = lp[16]; pq.o1_sh = lp[17];
-    const CUtensorMap m[4] = {mq, mo, mk, mv};
-    const int gx = (S + p.box_q - 1) / p.box_q;
-    if (sink_part != nullptr) {
-      pq.sinks = sinks; pq.sink_part = sink_part;
-      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2, true>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1, true>(m, pq, gx, B, st);
-    } else {
-      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1>(m, pq, gx, B, st);
-    }
-    if (rc) return rc + 20000;
   }
   return 0;
 }

@@ -168,9 +168,10 @@ def launch_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page:
     splits = choose_splits(b * hk * blocks, -(-reach // 128) + -(-min(sink_tokens, t) // 128))
     if b * splits > 65535:
         splits = 1
-    box_k = 64 if blocks > 1 else 32
+    one_tile = s * g <= 128                                # the kernel's form for few rows: 128 keys a tile, else 64
+    box_k = 32 if one_tile else 64
     if table is not None:
-        box_k = min(128, page & -page)
+        box_k = min(128 if one_tile else 64, page & -page)
     out = torch.empty(b, s, h, dv, dtype=torch.bfloat16, device=dev)
     lse = torch.empty(b, h, s, dtype=torch.float32, device=dev) if want_lse else None
     ws = torch.empty(b * s * h * splits * (dv + 2), dtype=torch.float32, device=dev) if splits > 1 else None
