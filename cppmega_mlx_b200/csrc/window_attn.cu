@@ -159,8 +159,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* s_full = v_empty + NV;         // [stream][buffer]
   uint64_t* p_full = s_full + 4;           // [stream][buffer] P written
   uint64_t* pv_done = p_full + 4;          // [stream][buffer] P read, O added to
-  uint64_t* go = pv_done + 4;              // ROWS: stream 0 is through its first tile
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(go + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* xml = reinterpret_cast<float2*>(ctl + 1024);   // [2 streams][128 rows] (max, sum)
 
@@ -205,10 +204,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
     }
-    mbar_init(go, 1);
     *abort_flag = 0;
     fence_mbar_init();
     if (p.lengths != nullptr && status != nullptr) {   // a length that the cache cannot hold
@@ -237,7 +235,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tma_prefetch_desc(&tmV);
     }
     if (NT > 0) {
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t q_box = p.box_q * p.g * 128;
         const int nq = KEYS ? p.copies : (two ? 2 : 1);
         mbar_arrive_expect_tx(q_full, q_box * nq * DB);
@@ -271,11 +269,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const WaTile t = R.tile(i);
         const int boxes = (t.k1 - t.k0 + p.box_k - 1) / p.box_k;
         bool ok = true;
-        if (lane == 0) {
-          ok = mbar_wait(&empty[st], ((n / depth) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
+        if (elect_one()) {
+          ok = wa_wait(&empty[st], ((n / depth) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
           if (ok) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(boxes) * p.box_k * 128 * DB);
         }
-        if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
+        if (!__all_sync(0xffffffffu, ok)) return false;
         const int j = t.k0 + my_box * p.box_k;
         if (my_box < boxes)
           tma_load_4d(ring + st * Cfg::STAGE + my_kb * Cfg::KBLK + my_box * p.box_k * 128, map, &full[st], my_kb * 64,
@@ -305,9 +303,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int i = t0; i < t1; ++i) {
       const int n = i - t0, st = n % NV;
       const WaTile t = R.tile(i);
-      bool ok = true;
-      if (lane == 0) ok = mbar_wait(&v_full[st], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL);
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (!wa_warp_wait(&v_full[st], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
       const bool tail = t.k1 - t.k0 < BN, head = i >= R.n_s && t.k0 < R.wtrue;
       const bool drafted = p.tree != nullptr && t.k1 > prefix;
       if (tail || head || drafted) {
@@ -325,8 +321,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         fence_proxy_async_smem();
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_ready[st]);
+      wa_warp_arrive(&v_ready[st]);
     }
   } else if (warp < 14) {
     // ---------------------------------------------------------------- MMA issuers: a thread each for the scores (warps 9, 10)
@@ -334,7 +329,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     // later: an issuing thread advances no faster than the tensor pipe takes its instructions.
     const bool scores = warp < 11;
     const int st = scores ? warp - 9 : warp - 12;
-    if (lane == 0 && (st == 0 || two)) {
+    if ((st == 0 || two) && elect_one()) {
       // one descriptor each, advanced by adding to its address field (16-byte units)
       const uint32_t s_col = tmem_base + Cfg::S_COL + st * Cfg::S_STEP, o_col = tmem_base + Cfg::O_STEP * st;
       const int first = t0 + (KEYS ? st : 0), step = KEYS ? 2 : 1;
@@ -342,8 +337,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (scores) {
         const uint64_t q_desc = make_smem_desc_sw128(smem_u32(qs) + (KEYS ? 0 : st * DB * WA_BLK), 16, 1024);
         const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ks), 16, 1024);
-        bool ok = first >= t1 || mbar_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
-        if (!KEYS && st == 1 && first < t1) ok = ok && mbar_wait(go, 0, abort_flag, status, ST_TIMEOUT_FULL);
+        bool ok = first >= t1 || wa_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
         for (int i = first; i < t1 && ok; i += step, ++c) {
           const int n = i - t0, kst = n % NK, buf = c % BUFS;
           const WaTile t = R.tile(i);
@@ -351,8 +345,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const uint64_t kd = k_desc + static_cast<uint32_t>(kst * (Cfg::STAGE >> 4));
           const uint32_t d = s_col + buf * 64;
           // the scores take the place of an earlier tile's P, once the product has read it
-          if (c >= BUFS && !mbar_wait(&pv_done[st * 2 + buf], (c / BUFS - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
-          if (!mbar_wait(&k_full[kst], (n / NK) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
+          if (c >= BUFS && !wa_wait(&pv_done[st * 2 + buf], (c / BUFS - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
+          if (!wa_wait(&k_full[kst], (n / NK) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
           tc_fence_after();
 #pragma unroll
           for (int kb = 0; kb < DB; ++kb)
@@ -371,8 +365,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const int k16 = (t.k1 - t.k0 + 15) >> 4;
           const uint64_t vd = v_desc + static_cast<uint32_t>(vst * (Cfg::STAGE >> 4));
           const uint32_t a = s_col + buf * 64;
-          if (!mbar_wait(&v_ready[vst], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
-          if (!mbar_wait(&p_full[st * 2 + buf], (c / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
+          if (!wa_wait(&v_ready[vst], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
+          if (!wa_wait(&p_full[st * 2 + buf], (c / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
           tc_fence_after();
           umma_f16_ts(o_col, a, vd, idesc_o, c > 0 ? 1u : 0u);
           if (k16 == BN / 16) {
@@ -411,8 +405,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (active) {
       const int first = t0 + (KEYS ? st : 0), step = KEYS ? 2 : 1;
       auto scores_in = [&](int at) {         // tile `at` of this stream: are its scores there?
-        return static_cast<bool>(__all_sync(
-            0xffffffffu, mbar_wait(&s_full[st * 2 + at % BUFS], (at / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)));
+        return wa_warp_wait(&s_full[st * 2 + at % BUFS], (at / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       };
       uint32_t x[CH][32];                    // the scores of this thread's chunks
       auto load = [&](int e, int chunks, int at) {
@@ -423,8 +416,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           ok = false;
           break;
         }
-        mbar_arrive(&p_full[st * 2 + c % BUFS]);
-        if (!KEYS && c == 0 && threadIdx.x == 0) mbar_arrive(go);
+        wa_warp_arrive(&p_full[st * 2 + c % BUFS]);
       }
       WaTile t = R.tile(first);
       int chunks = (t.k1 - t.k0 + 31) >> 5;  // 32-key chunks that the tile has
@@ -474,8 +466,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           if (c > 0) {
             // O is rescaled when the previous tile's product has completed (KEYS: these scores were issued after it)
-            if (BUFS > 1 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status,
-                                                               ST_TIMEOUT_TMEM_EMPTY))) {
+            if (BUFS > 1 &&
+                !wa_warp_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) {
               ok = false;
               break;
             }
@@ -525,8 +517,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[st * 2 + buf]);
-        if (!KEYS && c == 0 && threadIdx.x == 0) mbar_arrive(go);
+        wa_warp_arrive(&p_full[st * 2 + buf]);
         if (more) {
           if (!scores_in(c + 1)) {
             ok = false;
@@ -543,8 +534,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       // (the product before the last completes before it: one thread issued both)
       if (c > 0 && ok)
-        ok = mbar_wait(&pv_done[st * 2 + (c - 1) % BUFS], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
-      ok = __all_sync(0xffffffffu, ok);
+        ok = wa_warp_wait(&pv_done[st * 2 + (c - 1) % BUFS], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       tc_fence_after();
     }
     const float LN2 = 0.6931471805599453f;

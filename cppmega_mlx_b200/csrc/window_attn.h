@@ -73,6 +73,36 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// Barrier over `threads` threads that ORs a predicate.
+__device__ __forceinline__ bool named_bar_or(int id, int threads, bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(out)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(pred))
+      : "memory");
+  return out != 0;
+}
+// Waits.  A role's thread is chosen with elect_one(): the compiler then knows that one thread runs, and a product issues in the 33
+// to 65 clocks that it takes (44 at the least behind `lane == 0`) and a wait on a completed barrier in 70 clocks (205).  A whole
+// warp waits through one of its threads, because 32 polls of a barrier take their turns (140 clocks on a completed one).
+__device__ __forceinline__ bool wa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort_flag, status, code);
+}
+__device__ __forceinline__ bool wa_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  bool ok = true;
+  if (elect_one()) ok = wa_wait(bar, parity, abort_flag, status, code);
+  ok = __all_sync(0xffffffffu, ok);
+  __syncwarp();
+  return ok;
+}
+__device__ __forceinline__ void wa_warp_arrive(uint64_t* bar) {      // one arrival for the warp's work so far
+  __syncwarp();
+  if (elect_one()) mbar_arrive(bar);
+}
 // Registers of a warp group, moved between the groups of a block: the sum never exceeds what the block was launched with.
 template <int N>
 __device__ __forceinline__ void wa_more_registers() {

@@ -134,7 +134,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&x_full[i], 1);
-      mbar_init(&a_full[i], 128);
+      mbar_init(&a_full[i], 4);
       mbar_init(&g_done[i], 1);
     }
     mbar_init(all_done, 1);
@@ -164,7 +164,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
 
   if (warp == 8) {
     // ---------------------------------------------------------------- TMA producer
-    if (lane == 0 && NT > 0) {
+    if (NT > 0 && elect_one()) {
       const uint32_t r_bytes = (MODE == WB_DQ ? p.box_q * p.g : 128) * 128;
       mbar_arrive_expect_tx(r_full, 2 * DB * r_bytes);
       for (int kb = 0; kb < DB; ++kb) {
@@ -179,7 +179,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       const uint32_t t_bytes = (MODE == WB_DQ ? WB_SUB : used) * 128;
       for (int n = 0; n < NT; ++n) {
         const int st = n % WB_NS;
-        if (!mbar_wait(&t_empty[st], ((n / WB_NS) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY)) break;
+        if (!wa_wait(&t_empty[st], ((n / WB_NS) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY)) break;
         mbar_arrive_expect_tx(&t_full[st], 2 * DB * t_bytes);
         uint8_t* t1 = ts + st * Cfg::STAGE;
         uint8_t* t2 = t1 + DB * WB_SBLK;
@@ -201,7 +201,6 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     const float2* stats = p.stats + (static_cast<long long>(b) * p.Hk + hk) * rows;
     for (int n = 0; n < NT; ++n) {
       const int st = n % WB_NS;
-      bool ok = true;
       float2 v[2];
       if (MODE == WB_DKV) {
 #pragma unroll
@@ -211,8 +210,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
           v[i] = c < used && r < rows ? stats[r] : make_float2(INFINITY, 0.f);
         }
       }
-      if (lane == 0) ok = mbar_wait(&t_full[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL);
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (!wa_warp_wait(&t_full[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
       if (MODE == WB_DKV) {
         aux[st * WB_SUB + lane] = v[0];
         aux[st * WB_SUB + 32 + lane] = v[1];
@@ -226,23 +224,22 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
           fence_proxy_async_smem();
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&t_ready[st]);
+      wa_warp_arrive(&t_ready[st]);
     }
   } else if (warp == 9) {
     // ---------------------------------------------------------------- MMA issuer (one thread)
-    if (lane == 0 && NT > 0) {
+    if (NT > 0 && elect_one()) {
       constexpr uint32_t idesc_x = make_idesc(128, WB_SUB, 1, 1, 0, 0);
       constexpr uint32_t idesc_g = make_idesc(128, DB * 64, 1, 1, 0, 1);
       // descriptors are advanced by adding to their address field (16-byte units)
       const uint64_t r1d = make_smem_desc_sw128(smem_u32(r1s), 16, 1024), r2d = make_smem_desc_sw128(smem_u32(r2s), 16, 1024);
       const uint64_t td = make_smem_desc_sw128(smem_u32(ts), 16, 1024), gd = make_smem_desc_sw128(smem_u32(ts), WB_SBLK, 1024);
-      bool ok = mbar_wait(r_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
+      bool ok = wa_wait(r_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
       auto issue_scores = [&](int n) {
         const int st = n % WB_NS, buf = n & 1;
-        if (!mbar_wait(&t_ready[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL)) return false;
+        if (!wa_wait(&t_ready[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL)) return false;
         // the buffer holds P and dS of sub-tile n - 2 until its gradient products have read them
-        if (n >= 2 && !mbar_wait(&g_done[buf], ((n >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
+        if (n >= 2 && !wa_wait(&g_done[buf], ((n >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
         tc_fence_after();
         const uint32_t x = tmem_base + Cfg::X_COL + buf * 128;
         const uint64_t t1 = td + static_cast<uint32_t>(st * (Cfg::STAGE >> 4)), t2 = t1 + ((DB * WB_SBLK) >> 4);
@@ -263,7 +260,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       for (int n = 0; n < NT && ok; ++n) {
         if (n + 1 < NT && !issue_scores(n + 1)) break;
         const int st = n % WB_NS, buf = n & 1;
-        if (!mbar_wait(&a_full[buf], (n >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
+        if (!wa_wait(&a_full[buf], (n >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
         tc_fence_after();
         const uint32_t x = tmem_base + Cfg::X_COL + buf * 128;
         const uint64_t t1 = gd + static_cast<uint32_t>(st * (Cfg::STAGE >> 4)), t2 = t1 + ((DB * WB_SBLK) >> 4);
@@ -314,9 +311,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
           for (int i = 0; i < 2; ++i) words[i] = wa_low_bits(hi - 32 * i) & ~wa_low_bits(lo - 32 * i);
         }
       }
-      bool got = mbar_wait(&x_full[st_id], (n >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
-      if (MODE == WB_DKV) got = got && mbar_wait(&t_ready[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL);
-      if (!__all_sync(0xffffffffu, got)) {
+      // (the row statistics came before the scores: their barrier is waited for so that this warp sees them)
+      if (!wa_warp_wait(&x_full[st_id], (n >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL) ||
+          (MODE == WB_DKV && !wa_warp_wait(&t_ready[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL))) {
         ok = false;
         break;
       }
@@ -371,10 +368,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&a_full[st_id]);
+      wa_warp_arrive(&a_full[st_id]);
     }
-    if (NT > 0 && ok) ok = mbar_wait(all_done, 0, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
-    ok = __all_sync(0xffffffffu, ok);
+    if (NT > 0 && ok) ok = wa_warp_wait(all_done, 0, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
     tc_fence_after();
     if (SINKS) {
       // -exp(sink - lse) do.o, summed over the tile's queries for each head
