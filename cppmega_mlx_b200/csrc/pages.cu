@@ -132,15 +132,6 @@ int pool_width(const cmb::PagePools& pools, int n, bool rows) {
   }
   return static_cast<int>(all & (~all + 1));
 }
-void fill_pools(cmb::PagePools& pools, void* const* bases, const long long* lp, int n, int layers) {
-  for (int i = 0; i < n; ++i) {
-    cmb::PagePool& p = pools.pool[i];
-    p.base = static_cast<uint8_t*>(bases[i]);
-    p.page_stride = lp[4 * i]; p.layer_stride = lp[4 * i + 1]; p.row_stride = lp[4 * i + 2]; p.bytes = lp[4 * i + 3];
-    p.layers = layers;
-  }
-}
-
 template <typename V>
 int launch_copy(const cmb::PagePools& pools, int n, const int* src, const int* dst, int pairs, int num_pages, int* status, cudaStream_t st) {
   long long most = 0;
@@ -167,15 +158,21 @@ int launch_compact(const cmb::PagePools& pools, int n, const int* table, int tab
 
 }  // namespace
 
-// bases[n]; lp = n x {page stride, 0, 0, bytes of a page} in bytes.  src, dst [pairs] page ids on the device (-1, -1: unused).
-// pairs <= 65535, n <= 32.
-extern "C" int cmb_copy_pages(void* const* bases, const long long* lp, int n, const int* src, const int* dst, int pairs, int num_pages,
-                              int* status, void* stream) {
+// A pool as callers describe it: sizes and strides in bytes (host memory); bytes: of a page (copy) or of a row (compact).
+struct cmb_page_pool {
+  unsigned long long base;
+  long long page_stride, layer_stride, row_stride, bytes;
+};
+
+// src, dst [pairs] page ids on the device (-1, -1: unused).  pairs <= 65535, n <= 32.
+extern "C" int cmb_copy_pages(const cmb_page_pool* pool, int n, const int* src, const int* dst, int pairs, int num_pages, int* status,
+                              void* stream) {
   if (n < 1 || n > cmb::PG_MAX_POOLS || pairs < 1 || pairs > 65535 || num_pages < 1) return 1;
   cmb::PagePools pools{};
-  fill_pools(pools, bases, lp, n, 1);
-  for (int i = 0; i < n; ++i)
-    if (pools.pool[i].bytes <= 0) return 1;
+  for (int i = 0; i < n; ++i) {
+    if (pool[i].bytes <= 0) return 1;
+    pools.pool[i] = {reinterpret_cast<uint8_t*>(pool[i].base), pool[i].page_stride, 0, 0, pool[i].bytes, 1};
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (pool_width(pools, n, false)) {
     case 16: return launch_copy<uint4>(pools, n, src, dst, pairs, num_pages, status, st);
@@ -186,18 +183,20 @@ extern "C" int cmb_copy_pages(void* const* bases, const long long* lp, int n, co
   }
 }
 
-// bases[n]; lp = n x {page, layer, row stride, bytes of a row}; ip = {B, table_w, most, page, num_pages, layers};
-// table [B, table_w], start [B], path [B, most], counts [B] int32 on the device; most <= 2048.
-extern "C" int cmb_compact_rows(void* const* bases, const long long* lp, int n, const int* table, const int* start, const int* path,
-                                const int* counts, const int* ip, int* status, void* stream) {
+// ip = {B, table_w, most, page, num_pages, layers}; table [B, table_w], start [B], path [B, most], counts [B] int32 on the device;
+// most <= 2048.
+extern "C" int cmb_compact_rows(const cmb_page_pool* pool, int n, const int* table, const int* start, const int* path, const int* counts,
+                                const int* ip, int* status, void* stream) {
   const int B = ip[0], table_w = ip[1], most = ip[2], page = ip[3], num_pages = ip[4], layers = ip[5];
   if (n < 1 || n > cmb::PG_MAX_POOLS || B < 1 || B > 65535 || most < 1 || most > cmb::PG_THREADS * cmb::PG_UNROLL || page < 1 ||
       num_pages < 1 || layers < 1 || table_w < 1 || static_cast<long long>(n) * layers > 65535)
     return 1;
   cmb::PagePools pools{};
-  fill_pools(pools, bases, lp, n, layers);
-  for (int i = 0; i < n; ++i)
-    if (pools.pool[i].bytes <= 0 || pools.pool[i].bytes > (1ll << 30)) return 1;
+  for (int i = 0; i < n; ++i) {
+    if (pool[i].bytes <= 0 || pool[i].bytes > (1ll << 30)) return 1;
+    pools.pool[i] = {reinterpret_cast<uint8_t*>(pool[i].base), pool[i].page_stride, pool[i].layer_stride, pool[i].row_stride, pool[i].bytes,
+                     layers};
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (pool_width(pools, n, true)) {
     case 16: return launch_compact<uint4>(pools, n, table, table_w, start, path, counts, B, most, page, num_pages, layers, status, st);

@@ -60,7 +60,7 @@ struct WindowParams {
   int tree_sb;
   const int* table;                      // null = contiguous
   int table_w, page, num_pages, box_k;   // box_k: key rows per TMA box; tiles start at its multiples when paged
-  const float* sinks;                    // [H] or null
+  WaSinks sinks;
   __nv_bfloat16* out;
   long long o_sb, o_ss, o_sh;
   float* lse;                            // [B, H, S] natural log, +inf where a row sees nothing; may be null
@@ -546,8 +546,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const long long idx = ((static_cast<long long>(b) * p.S + w.s) * p.H + w.h) * p.splits + split;
         if (p.splits == 1) {
           float l = l_sum, m = m_ref, f = 1.f;
-          if (p.sinks != nullptr && in) {
-            const float s2 = p.sinks[w.h] * 1.4426950408889634f;
+          if (p.sinks.p != nullptr && in) {
+            const float s2 = p.sinks.log2_at(w.h);
             const float top = fmaxf(m, s2);
             f = m == -INFINITY ? 0.f : exp2f(m - top);
             l = l * f + exp2f(s2 - top);
@@ -641,8 +641,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const int ql = r / p.g, s = s_first + ql, h = hk * p.g + (r - ql * p.g);
           if (p.splits == 1) {
             float m = top, f = 1.f;
-            if (p.sinks != nullptr) {
-              const float s2 = p.sinks[h] * 1.4426950408889634f;
+            if (p.sinks.p != nullptr) {
+              const float s2 = p.sinks.log2_at(h);
               const float t2 = fmaxf(m, s2);
               f = m == -INFINITY ? 0.f : exp2f(m - t2);
               l = l * f + exp2f(s2 - t2);
@@ -688,7 +688,7 @@ struct CombineParams {
   long long rows;
   const float* ws_o;
   const float2* ws_ml;
-  const float* sinks;
+  WaSinks sinks;
   __nv_bfloat16* out;
   long long o_sb, o_ss, o_sh;
   float* lse;
@@ -722,8 +722,8 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams
     }
   }
   float f = 1.f;
-  if (p.sinks != nullptr) {
-    const float s2 = p.sinks[h] * 1.4426950408889634f;
+  if (p.sinks.p != nullptr) {
+    const float s2 = p.sinks.log2_at(h);
     const float t2 = fmaxf(top, s2);
     f = top == -INFINITY ? 0.f : exp2f(top - t2);
     l = l * f + exp2f(s2 - t2);
@@ -800,38 +800,47 @@ int launch_window_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 
 }  // namespace
 
+// One call: what its tensors look like, then where they are (host memory, both).
+struct cmb_window_call {
+  int B, S, T, H, Hk, Dq, Dv, window, ns, cached, tree_sb, table_w, page, num_pages, box_k, splits, sinks_bf16, pad;
+  long long q_sb, q_ss, q_sh, k_outer, k_row, k_head, v_outer, v_row, v_head, o_sb, o_ss, o_sh;
+  double scale;
+};
+struct cmb_window_ptrs {
+  const void *q, *k, *v, *lengths, *tree, *table, *sinks;
+  void *out, *lse, *ws_o, *ws_ml, *status;
+};
 // q [B,S,H,Dq]; k / v rows [outer, rows, Hk, Dq | Dv] with outer = B (contiguous, rows = T) or pages of a pool (table
-// [B, table_w], rows = page size); bf16 with unit inner stride.  Dq, Dv <= 128 and multiples of 8; H / Hk <= 128.
-// ip = {B, S, T, H, Hk, Dq, Dv, window, ns, cached, tree_sb, table_w, page, num_pages, box_k, splits};
-// lp = {q_sb, q_ss, q_sh, k_outer, k_row, k_head, v_outer, v_row, v_head, o_sb, o_ss, o_sh}.
-// ws_o / ws_ml are needed for splits > 1 only.  Returns 0, 1 for arguments that the kernel does not cover.
-extern "C" int cmb_window_fwd(const void* q, const void* k, const void* v, const int* lengths, const void* tree, const int* table,
-                              const float* sinks, void* out, float* lse, float* ws_o, float* ws_ml, const int* ip,
-                              const long long* lp, float scale, int* status, void* stream) {
+// [B, table_w], rows = page size); bf16 with unit inner stride.  Dq, Dv <= 128 and multiples of 8; H / Hk <= 128.  ws_o / ws_ml
+// are needed for splits > 1 only.  Returns 0, 1 for arguments that the kernel does not cover.
+extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs* at, void* stream) {
+  const cmb_window_call& a = *call;
   cmb::WindowParams p{};
-  const int B = ip[0], Dq = ip[5];
-  p.S = ip[1]; p.T = ip[2]; p.H = ip[3]; p.Hk = ip[4]; p.Dv = ip[6];
-  p.window = ip[7]; p.ns = ip[8]; p.cached = ip[9];
-  p.tree = static_cast<const unsigned long long*>(tree); p.tree_sb = ip[10];
-  p.table = table; p.table_w = ip[11]; p.page = ip[12]; p.num_pages = ip[13]; p.box_k = ip[14];
-  p.splits = ip[15];
+  const int B = a.B, Dq = a.Dq;
+  p.S = a.S; p.T = a.T; p.H = a.H; p.Hk = a.Hk; p.Dv = a.Dv;
+  p.window = a.window; p.ns = a.ns; p.cached = a.cached;
+  p.tree = static_cast<const unsigned long long*>(at->tree); p.tree_sb = a.tree_sb;
+  p.table = static_cast<const int*>(at->table); p.table_w = a.table_w; p.page = a.page; p.num_pages = a.num_pages; p.box_k = a.box_k;
+  p.splits = a.splits;
+  p.lengths = static_cast<const int*>(at->lengths);
+  p.sinks.p = at->sinks; p.sinks.bf16 = a.sinks_bf16;
   if (B <= 0 || p.S <= 0 || p.Hk <= 0 || p.H <= 0 || p.H % p.Hk || p.T < 0 || p.splits < 1) return 1;
   p.g = p.H / p.Hk;
   if (p.g > 128 || p.Hk > 65535 || static_cast<long long>(B) * p.splits > 65535) return 1;
   if (Dq <= 0 || Dq > 128 || Dq % 8 || p.Dv <= 0 || p.Dv > 128 || p.Dv % 8) return 1;
-  if (p.window < 1 || p.window > cmb::WA_NO_WINDOW || p.ns < 0 || !(scale > 0.f)) return 1;
-  if (p.cached && (lengths == nullptr || p.T < p.S)) return 1;
-  if (!p.cached && (p.tree != nullptr || table != nullptr || p.T < p.S)) return 1;
+  if (p.window < 1 || p.window > cmb::WA_NO_WINDOW || p.ns < 0 || !(a.scale > 0.)) return 1;
+  if (p.cached && (p.lengths == nullptr || p.T < p.S)) return 1;
+  if (!p.cached && (p.tree != nullptr || p.table != nullptr || p.T < p.S)) return 1;
   if (p.tree != nullptr && p.S > 64) return 1;
   if (p.box_k != 8 && p.box_k != 16 && p.box_k != 32 && p.box_k != 64 && p.box_k != 128) return 1;
-  if (table != nullptr && (p.page <= 0 || p.page % p.box_k || p.num_pages <= 0 || p.table_w <= 0 ||
-                           static_cast<long long>(p.table_w) * p.page < p.T))
+  if (p.table != nullptr && (p.page <= 0 || p.page % p.box_k || p.num_pages <= 0 || p.table_w <= 0 ||
+                             static_cast<long long>(p.table_w) * p.page < p.T))
     return 1;
-  if (p.S * static_cast<long long>(p.g) > 128 && p.box_k > 64) return 1;   // a tile of 64 keys
-  if (p.splits > 1 && (ws_o == nullptr || ws_ml == nullptr)) return 1;
-  if ((lp[9] | lp[10] | lp[11]) & 7 || (reinterpret_cast<uintptr_t>(out) & 15)) return 1;
-  const int rows = p.S * p.g;                              // S <= 2^24 rows is checked by the caller's shapes
+  const long long rows = static_cast<long long>(p.S) * p.g;
   const bool keys = rows <= 128;
+  if (!keys && p.box_k > 64) return 1;                     // a tile of 64 keys
+  if (p.splits > 1 && (at->ws_o == nullptr || at->ws_ml == nullptr)) return 1;
+  if ((a.o_sb | a.o_ss | a.o_sh) & 7 || (reinterpret_cast<uintptr_t>(at->out) & 15)) return 1;
   p.copies = 1;
   if (keys) {
     p.box_q = p.S;
@@ -840,17 +849,18 @@ extern "C" int cmb_window_fwd(const void* q, const void* k, const void* v, const
     p.box_q = 128 / p.g < p.S ? 128 / p.g : p.S;
   }
   p.copy_rows = 128 / p.copies;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.lengths = lengths; p.sinks = sinks;
-  p.out = static_cast<__nv_bfloat16*>(out); p.o_sb = lp[9]; p.o_ss = lp[10]; p.o_sh = lp[11];
-  p.lse = lse; p.ws_o = ws_o; p.ws_ml = reinterpret_cast<float2*>(ws_ml); p.status = status;
+  p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
+  p.out = static_cast<__nv_bfloat16*>(at->out); p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
+  p.lse = static_cast<float*>(at->lse);
+  p.ws_o = static_cast<float*>(at->ws_o); p.ws_ml = static_cast<float2*>(at->ws_ml);
+  p.status = static_cast<int*>(at->status);
   CUtensorMap tq, tk, tv;
-  int rc = cmb_host::make_tmap_grouped(&tq, q, Dq, p.S, p.Hk, p.g, B, lp[1], lp[2], lp[0], p.box_q);
+  int rc = cmb_host::make_tmap_grouped(&tq, at->q, Dq, p.S, p.Hk, p.g, B, a.q_ss, a.q_sh, a.q_sb, p.box_q);
   if (rc) return rc;
-  const long long krows = table != nullptr ? p.page : p.T, outer = table != nullptr ? p.num_pages : B;
-  rc = cmb_host::make_tmap_rows(&tk, k, Dq, krows, p.Hk, outer, lp[4], lp[5], lp[3], p.box_k);
+  const long long krows = p.table != nullptr ? p.page : p.T, outer = p.table != nullptr ? p.num_pages : B;
+  rc = cmb_host::make_tmap_rows(&tk, at->k, Dq, krows, p.Hk, outer, a.k_row, a.k_head, a.k_outer, p.box_k);
   if (rc) return rc + 10000;
-  rc = cmb_host::make_tmap_rows(&tv, v, p.Dv, krows, p.Hk, outer, lp[7], lp[8], lp[6], p.box_k);
+  rc = cmb_host::make_tmap_rows(&tv, at->v, p.Dv, krows, p.Hk, outer, a.v_row, a.v_head, a.v_outer, p.box_k);
   if (rc) return rc + 20000;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = Dq > 64 || p.Dv > 64;
@@ -860,8 +870,8 @@ extern "C" int cmb_window_fwd(const void* q, const void* k, const void* v, const
   cmb::CombineParams c{};
   c.S = p.S; c.H = p.H; c.splits = p.splits; c.Dv = p.Dv;
   c.rows = static_cast<long long>(B) * p.S * p.H;
-  c.ws_o = ws_o; c.ws_ml = p.ws_ml; c.sinks = sinks;
-  c.out = p.out; c.o_sb = p.o_sb; c.o_ss = p.o_ss; c.o_sh = p.o_sh; c.lse = lse;
+  c.ws_o = p.ws_o; c.ws_ml = p.ws_ml; c.sinks = p.sinks;
+  c.out = p.out; c.o_sb = p.o_sb; c.o_ss = p.o_ss; c.o_sh = p.o_sh; c.lse = p.lse;
   const long long blocks = (c.rows + 3) / 4;
   if (blocks > 0x7fffffffll) return 1;
   cmb::window_combine_kernel<<<static_cast<unsigned>(blocks), 128, 0, st>>>(c);

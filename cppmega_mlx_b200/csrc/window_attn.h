@@ -12,6 +12,16 @@ namespace cmb {
 constexpr int WA_BLK = 128 * 128;            // bytes of one [128 rows x 64 bf16] block
 constexpr int WA_NO_WINDOW = 1 << 30;
 
+// Sink logits, fp32 or bf16, in log2 units.
+struct WaSinks {
+  const void* p;                             // [H] or null
+  int bf16;
+  __device__ __forceinline__ float log2_at(int h) const {
+    const float v = bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[h]) : static_cast<const float*>(p)[h];
+    return v * 1.4426950408889634f;
+  }
+};
+
 // Keys [k0, k1) of one tile.
 struct WaTile {
   int k0, k1;

@@ -45,7 +45,7 @@ struct WindowBwdParams {
   long long o1_sb, o1_ss, o1_sh, o2_sb, o2_ss, o2_sh;
   int sink_tiles, sink_splits;             // DKV: the first sink_tiles key tiles are split
   float* part;                             // [B, Hk, sink_tiles, sink_splits, 128, Dq + Dv]
-  const float* sinks;                      // [H], for SINKS
+  WaSinks sinks;                           // for SINKS
   float* sink_part;                        // [H, B * row tiles]
   int* status;
 };
@@ -375,7 +375,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     if (SINKS) {
       // -exp(sink - lse) do.o, summed over the tile's queries for each head
       float* red = reinterpret_cast<float*>(aux);      // [2][128]
-      red[st_id * 128 + row] = row_ok ? -exp2f(p.sinks[head] * 1.4426950408889634f - lse2) * row_dot : 0.f;
+      red[st_id * 128 + row] = row_ok ? -exp2f(p.sinks.log2_at(head) - lse2) * row_dot : 0.f;
       if (named_bar_and(1, 256, ok) && threadIdx.x < p.g) {
         float t = 0.f;
         for (int i = threadIdx.x; i < p.box_q * p.g; i += p.g) t += red[i] + red[128 + i];
@@ -510,6 +510,18 @@ __global__ void __launch_bounds__(256) window_join_kernel(const JoinParams p) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
 }
 
+// The sinks' gradient: a warp per head sums its row tiles in a fixed order.
+__global__ void __launch_bounds__(32) window_sinks_kernel(const float* part, int n, void* out, int bf16) {
+  const float* src = part + static_cast<long long>(blockIdx.x) * n;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n; i += 32) s += src[i];
+  s = warp_sum(s);
+  if (threadIdx.x == 0) {
+    if (bf16) static_cast<__nv_bfloat16*>(out)[blockIdx.x] = __float2bfloat16(s);
+    else static_cast<float*>(out)[blockIdx.x] = s;
+  }
+}
+
 }  // namespace cmb
 
 namespace {
@@ -526,83 +538,98 @@ int launch_window_bwd(const CUtensorMap (&m)[4], const cmb::WindowBwdParams& p, 
 
 }  // namespace
 
+// One call: what its tensors look like, then where they are (host memory, both).
+struct cmb_window_bwd_call {
+  int B, S, T, H, Hk, Dq, Dv, window, ns, sink_tiles, sink_splits, sinks_bf16;
+  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh, do_sb, do_ss, do_sh;
+  long long dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
+  double scale;
+};
+struct cmb_window_bwd_ptrs {
+  const void *q, *k, *v, *o, *dO, *lengths, *sinks, *lse;
+  void *dq, *dk, *dv, *dsinks, *stats, *sink_part, *part, *status;
+};
 // Backward of cmb_window_fwd's contiguous form.  o (the forward's output), dO [B,S,H,Dv]; lse [B,H,S]; dq [B,S,H,Dq],
-// dk [B,T,Hk,Dq], dv [B,T,Hk,Dv] bf16 (every element written; dq or dk and dv may be null together).  stats: scratch of
-// 2 B S H floats; sink_part (with sinks and dq): [H, B * ceil(S / min(S, 128 / (H / Hk)))] floats
-// or null; part: B Hk sink_tiles sink_splits 128 (Dq + Dv) floats where
-// sink_splits > 1.  ip = {B, S, T, H, Hk, Dq, Dv, window, ns, sink_tiles, sink_splits};
-// lp = 3 strides (batch, row, head) of each of q, k, v, o, dO, dq, dk, dv.  H / Hk <= 64.
-extern "C" int cmb_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dO, const int* lengths,
-                              const float* sinks, const float* lse, void* dq, void* dk, void* dv, float* stats, float* sink_part,
-                              float* part, const int* ip, const long long* lp, float scale, int* status, void* stream) {
-  const int B = ip[0], S = ip[1], T = ip[2], H = ip[3], Hk = ip[4], Dq = ip[5], Dv = ip[6];
+// dk [B,T,Hk,Dq], dv [B,T,Hk,Dv] bf16 (every element written; dq, or dk and dv together, may be null), dsinks [H] of the sinks' type
+// or null.  stats: scratch of 2 B S H floats; sink_part (with dsinks and dq): [H, B * ceil(S / min(S, 128 / (H / Hk)))] floats;
+// part: B Hk sink_tiles sink_splits 128 (Dq + Dv) floats where sink_splits > 1.  H / Hk <= 64.
+extern "C" int cmb_window_bwd(const cmb_window_bwd_call* call, const cmb_window_bwd_ptrs* at, void* stream) {
+  const cmb_window_bwd_call& a = *call;
+  const int B = a.B, S = a.S, T = a.T, H = a.H, Hk = a.Hk, Dq = a.Dq, Dv = a.Dv;
   if (B <= 0 || B > 65535 || S <= 0 || T < S || Hk <= 0 || Hk > 65535 || H <= 0 || H > 65535 || H % Hk || H / Hk > 64) return 1;
   if (Dq <= 0 || Dq > 128 || Dq % 8 || Dv <= 0 || Dv > 128 || Dv % 8) return 1;
-  if (ip[7] < 1 || ip[7] > cmb::WA_NO_WINDOW || ip[8] < 0 || !(scale > 0.f)) return 1;
-  for (int i = 9; i < 24; ++i)
-    if (lp[i] & 7) return 1;
-  if (sink_part != nullptr && (sinks == nullptr || dq == nullptr)) return 1;
+  if (a.window < 1 || a.window > cmb::WA_NO_WINDOW || a.ns < 0 || !(a.scale > 0.)) return 1;
+  if ((a.o_sb | a.o_ss | a.o_sh | a.do_sb | a.do_ss | a.do_sh | a.dq_sb | a.dq_ss | a.dq_sh | a.dk_sb | a.dk_ss | a.dk_sh | a.dv_sb |
+       a.dv_ss | a.dv_sh) & 7)
+    return 1;
+  if (at->dsinks != nullptr && (at->sinks == nullptr || at->dq == nullptr || at->sink_part == nullptr)) return 1;
   const int key_tiles = (T + 127) / 128;
   cmb::WindowBwdParams p{};
   p.S = S; p.T = T; p.H = H; p.Hk = Hk; p.g = H / Hk; p.Dq = Dq; p.Dv = Dv;
   p.box_q = 128 / p.g < S ? 128 / p.g : S;
   p.sub_q = cmb::WB_SUB / p.g;
-  p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
-  p.window = ip[7]; p.ns = ip[8]; p.lengths = lengths;
-  p.stats = reinterpret_cast<float2*>(stats);
-  p.sink_tiles = ip[9]; p.sink_splits = ip[10]; p.part = part; p.status = status;
-  if (p.sink_tiles < 0 || p.sink_tiles > key_tiles || p.sink_splits < 1 || (p.sink_splits > 1 && part == nullptr)) return 1;
+  p.scale = static_cast<float>(a.scale); p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
+  p.window = a.window; p.ns = a.ns; p.lengths = static_cast<const int*>(at->lengths);
+  p.stats = static_cast<float2*>(at->stats);
+  p.sink_tiles = a.sink_tiles; p.sink_splits = a.sink_splits; p.part = static_cast<float*>(at->part);
+  p.status = static_cast<int*>(at->status);
+  if (p.sink_tiles < 0 || p.sink_tiles > key_tiles || p.sink_splits < 1 || (p.sink_splits > 1 && at->dk != nullptr && p.part == nullptr))
+    return 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
   cmb::StatsParams sp{};
   sp.B = B; sp.S = S; sp.H = H; sp.g = p.g; sp.Dv = Dv;
-  sp.o = static_cast<const __nv_bfloat16*>(o); sp.o_sb = lp[9]; sp.o_ss = lp[10]; sp.o_sh = lp[11];
-  sp.d = static_cast<const __nv_bfloat16*>(dO); sp.d_sb = lp[12]; sp.d_ss = lp[13]; sp.d_sh = lp[14];
-  sp.lse = lse; sp.stats = reinterpret_cast<float2*>(stats);
+  sp.o = static_cast<const __nv_bfloat16*>(at->o); sp.o_sb = a.o_sb; sp.o_ss = a.o_ss; sp.o_sh = a.o_sh;
+  sp.d = static_cast<const __nv_bfloat16*>(at->dO); sp.d_sb = a.do_sb; sp.d_ss = a.do_ss; sp.d_sh = a.do_sh;
+  sp.lse = static_cast<const float*>(at->lse); sp.stats = p.stats;
   cmb::window_stats_kernel<<<dim3((S + cmb::WS_ROWS - 1) / cmb::WS_ROWS, H, B), 256, 0, st>>>(sp);
   if (cudaGetLastError() != cudaSuccess) return 104;
 
   const bool wide = Dq > 64 || Dv > 64;
   auto maps = [&](CUtensorMap& mq, CUtensorMap& mo, CUtensorMap& mk, CUtensorMap& mv, int box_q, int box_k) {
-    int rc = cmb_host::make_tmap_grouped(&mq, q, Dq, S, Hk, p.g, B, lp[1], lp[2], lp[0], box_q);
-    if (!rc) rc = cmb_host::make_tmap_grouped(&mo, dO, Dv, S, Hk, p.g, B, lp[13], lp[14], lp[12], box_q);
-    if (!rc) rc = cmb_host::make_tmap_rows(&mk, k, Dq, T, Hk, B, lp[4], lp[5], lp[3], box_k);
-    if (!rc) rc = cmb_host::make_tmap_rows(&mv, v, Dv, T, Hk, B, lp[7], lp[8], lp[6], box_k);
+    int rc = cmb_host::make_tmap_grouped(&mq, at->q, Dq, S, Hk, p.g, B, a.q_ss, a.q_sh, a.q_sb, box_q);
+    if (!rc) rc = cmb_host::make_tmap_grouped(&mo, at->dO, Dv, S, Hk, p.g, B, a.do_ss, a.do_sh, a.do_sb, box_q);
+    if (!rc) rc = cmb_host::make_tmap_rows(&mk, at->k, Dq, T, Hk, B, a.k_ss, a.k_sh, a.k_sb, box_k);
+    if (!rc) rc = cmb_host::make_tmap_rows(&mv, at->v, Dv, T, Hk, B, a.v_ss, a.v_sh, a.v_sb, box_k);
     return rc;
   };
-  if (dq != nullptr) {
+  if (at->dq != nullptr) {
     CUtensorMap mq, mo, mk, mv;
     int rc = maps(mq, mo, mk, mv, p.box_q, cmb::WB_SUB);
     if (rc) return rc;
     cmb::WindowBwdParams pq = p;
-    pq.o1 = static_cast<__nv_bfloat16*>(dq); pq.o1_sb = lp[15]; pq.o1_ss = lp[16]; pq.o1_sh = lp[17];
+    pq.o1 = static_cast<__nv_bfloat16*>(at->dq); pq.o1_sb = a.dq_sb; pq.o1_ss = a.dq_ss; pq.o1_sh = a.dq_sh;
     const CUtensorMap m[4] = {mq, mo, mk, mv};
     const int gx = (S + p.box_q - 1) / p.box_q;
-    if (sink_part != nullptr) {
-      pq.sinks = sinks; pq.sink_part = sink_part;
+    if (at->dsinks != nullptr) {
+      pq.sinks.p = at->sinks; pq.sinks.bf16 = a.sinks_bf16; pq.sink_part = static_cast<float*>(at->sink_part);
       rc = wide ? launch_window_bwd<cmb::WB_DQ, 2, true>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1, true>(m, pq, gx, B, st);
+      if (rc) return rc + 20000;
+      cmb::window_sinks_kernel<<<H, 32, 0, st>>>(pq.sink_part, B * gx, at->dsinks, a.sinks_bf16);
+      if (cudaGetLastError() != cudaSuccess) return 104;
     } else {
       rc = wide ? launch_window_bwd<cmb::WB_DQ, 2>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1>(m, pq, gx, B, st);
+      if (rc) return rc + 20000;
     }
-    if (rc) return rc + 20000;
   }
-  if (dk != nullptr) {
+  if (at->dk != nullptr) {
     CUtensorMap mq, mo, mk, mv;
     int rc = maps(mq, mo, mk, mv, p.sub_q, 128);
     if (rc) return rc;
     cmb::WindowBwdParams pk = p;
-    pk.o1 = static_cast<__nv_bfloat16*>(dk); pk.o1_sb = lp[18]; pk.o1_ss = lp[19]; pk.o1_sh = lp[20];
-    pk.o2 = static_cast<__nv_bfloat16*>(dv); pk.o2_sb = lp[21]; pk.o2_ss = lp[22]; pk.o2_sh = lp[23];
+    pk.o1 = static_cast<__nv_bfloat16*>(at->dk); pk.o1_sb = a.dk_sb; pk.o1_ss = a.dk_ss; pk.o1_sh = a.dk_sh;
+    pk.o2 = static_cast<__nv_bfloat16*>(at->dv); pk.o2_sb = a.dv_sb; pk.o2_ss = a.dv_ss; pk.o2_sh = a.dv_sh;
     const CUtensorMap m[4] = {mk, mv, mq, mo};
     const int gx = key_tiles + p.sink_tiles * (p.sink_splits - 1);
     rc = wide ? launch_window_bwd<cmb::WB_DKV, 2>(m, pk, gx, B, st) : launch_window_bwd<cmb::WB_DKV, 1>(m, pk, gx, B, st);
     if (rc) return rc + 10000;
     if (p.sink_splits > 1 && p.sink_tiles > 0) {
       cmb::JoinParams j{};
-      j.T = T; j.Hk = Hk; j.Dq = Dq; j.Dv = Dv; j.tiles = p.sink_tiles; j.splits = p.sink_splits; j.part = part;
+      j.T = T; j.Hk = Hk; j.Dq = Dq; j.Dv = Dv; j.tiles = p.sink_tiles; j.splits = p.sink_splits; j.part = p.part;
       j.dk = pk.o1; j.k_sb = pk.o1_sb; j.k_ss = pk.o1_ss; j.k_sh = pk.o1_sh;
       j.dv = pk.o2; j.v_sb = pk.o2_sb; j.v_ss = pk.o2_ss; j.v_sh = pk.o2_sh;
       j.n = static_cast<long long>(B) * Hk * p.sink_tiles * 128 * ((Dq + Dv) / 4);
+      if ((j.n + 255) / 256 > 0x7fffffffll) return 1;
       cmb::window_join_kernel<<<static_cast<unsigned>((j.n + 255) / 256), 256, 0, st>>>(j);
       if (cudaGetLastError() != cudaSuccess) return 104;
     }

@@ -27,8 +27,8 @@ from __future__ import annotations
 import torch
 
 from . import _backend as B
-from .window_attention import (NO_WINDOW, _check, _check_lengths, kernel_covers, launch_forward, masked_softmax_attention, on_device,
-                               usable)
+from .window_attention import (NO_WINDOW, ForwardPlan, Plans, _check, _check_lengths, _sizes_covered, converted, in_place, launch_forward,
+                               masked_softmax_attention, meta, on_device, plan_forward, usable)
 
 MAX_TREE = 64
 
@@ -66,14 +66,18 @@ def _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens
                              f"{tree.dtype} on {tree.device}")
         if n > MAX_TREE:
             raise ValueError(f"cached_attention: a tree has at most {MAX_TREE} tokens, got {n}")
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k_rows, v_rows, sinks)):
-        raise ValueError("cached_attention has no gradient: call it under torch.no_grad(), or use window_attention")
     return scale
+
+
+def _no_gradient(q, k_rows, v_rows, sinks) -> None:
+    if torch.is_grad_enabled() and (q.requires_grad or k_rows.requires_grad or v_rows.requires_grad or (sinks is not None and sinks.requires_grad)):
+        raise ValueError("cached_attention has no gradient: call it under torch.no_grad(), or use window_attention")
 
 
 def cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, *, tree=None, window: int | None = None, sink_tokens: int = 0,
                                sinks=None, scale: float | None = None):
     scale = _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale)
+    _no_gradient(q, k_rows, v_rows, sinks)
     b, n = q.shape[:2]
     dev = q.device
     prefix = prefix_lengths.long()
@@ -100,13 +104,20 @@ def cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, *, tree
     return masked_softmax_attention(q, k, v, old | new, sinks, scale)
 
 
-def kernel_supported(q, k_rows, v_rows, table) -> bool:
-    if not (kernel_covers(q, k_rows, v_rows) and usable(k_rows) and usable(v_rows)):
-        return False
-    if table is not None and (k_rows.shape[1] % 8 or not table.shape[1] or not k_rows.shape[0]):
-        return False
-    t = k_rows.shape[1] * (1 if table is None else table.shape[1])
-    return q.shape[1] <= t <= NO_WINDOW // 2 and q.shape[0] <= 65535
+_plans = Plans()
+
+
+def _plan(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale, max_keys) -> ForwardPlan:
+    scale = _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale)
+    rows = k_rows.shape[1]
+    t = rows * (1 if table is None else table.shape[1])
+    if (not _sizes_covered(q, k_rows, v_rows) or not (usable(k_rows) and usable(v_rows)) or 0 in q.shape[:2] or not q.shape[1] <= t <= NO_WINDOW // 2
+            or (table is not None and (rows % 8 or not k_rows.shape[0])) or (tree is not None and not tree.is_contiguous())):
+        return ForwardPlan(False, False, scale)
+    if not usable(q):
+        return ForwardPlan(True, False, scale)
+    return plan_forward(q, k_rows, v_rows, t=t, lengths=prefix_lengths, cached=True, tree=tree, table=table, page=rows if table is not None else 0,
+                        window=window, sink_tokens=sink_tokens, sinks=sinks, scale=scale, max_keys=max_keys)
 
 
 def cached_attention(q, k_rows, v_rows, table, prefix_lengths, *, tree: torch.Tensor | None = None, window: int | None = None,
@@ -114,19 +125,17 @@ def cached_attention(q, k_rows, v_rows, table, prefix_lengths, *, tree: torch.Te
                      max_keys: int | None = None) -> torch.Tensor:
     """See the module docstring; returns [B, N, H, Dv] in ``q.dtype``.  ``max_keys`` (a bound on ``prefix_lengths + N``) only tunes how
     the work is split and never costs correctness."""
-    scale = _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale)
+    plan = _plans.get((meta(q), meta(k_rows), meta(v_rows), meta(table), meta(prefix_lengths), meta(tree), meta(sinks), window, sink_tokens, scale,
+                       max_keys), _plan, q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale, max_keys)
+    _no_gradient(q, k_rows, v_rows, sinks)
     if q.shape[0] == 0 or q.shape[1] == 0:
         return q.new_zeros(*q.shape[:3], v_rows.shape[3])
-    if not kernel_supported(q, k_rows, v_rows, table):
-        return cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, tree=tree, window=window, sink_tokens=sink_tokens,
-                                          sinks=sinks, scale=scale)
+    if not plan.covered or not B.kernels_enabled() or (k_rows.data_ptr() | v_rows.data_ptr()) % 16:
+        return cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, tree=None if tree is None else tree.contiguous(),
+                                          window=window, sink_tokens=sink_tokens, sinks=sinks, scale=scale)
+    if not plan.ready or q.data_ptr() % 16:
+        return cached_attention(in_place(q), k_rows, v_rows, table, prefix_lengths, tree=tree, window=window, sink_tokens=sink_tokens,
+                                sinks=sinks, scale=scale, max_keys=max_keys)
     with on_device(q.device):
-        q = q if usable(q) else q.contiguous()
-        i32 = lambda x: None if x is None else x.to(torch.int32).contiguous()  # noqa: E731
-        tbl = i32(table)
-        page = k_rows.shape[1] if tbl is not None else 0
-        t = page * tbl.shape[1] if tbl is not None else k_rows.shape[1]
-        return launch_forward(q, k_rows, v_rows, t=t, lengths=i32(prefix_lengths), cached=True,
-                              tree=None if tree is None else tree.contiguous(), table=tbl, page=page, window=window,
-                              sink_tokens=int(sink_tokens), sinks=None if sinks is None else sinks.float().contiguous(), scale=scale,
-                              want_lse=False, max_keys=max_keys)[0]
+        lengths, tbl, sk = converted(plan, prefix_lengths, table, sinks)
+        return launch_forward(plan, q, k_rows, v_rows, lengths, tree, tbl, sk, False)[0]

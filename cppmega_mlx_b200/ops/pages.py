@@ -17,27 +17,37 @@ acceptance and compaction of the pool on them.  The reference's manager only han
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from . import _backend as B
-from .window_attention import on_device
+from .window_attention import Plans, _raw_stream, entry, meta, on_device
 
 MAX_POOLS = 32          # of one launch
 MAX_PAIRS = 65535
 MAX_MOVES = 2048        # rows of one sequence in one call
 
 
-def _pools(pools, rank: int, what: str) -> list[torch.Tensor]:
-    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+_POOL = struct.Struct("Q4q")                     # cmb_page_pool
+_plans = Plans()
+
+
+def _pools(pools) -> tuple[torch.Tensor, ...]:
+    return (pools,) if isinstance(pools, torch.Tensor) else tuple(pools)
+
+
+def _check_pools(pools, rank: int, what: str) -> None:
     if not pools:
         raise ValueError(f"{what}: no pools")
     for p in pools:
         if p.dim() < rank or p.shape[0] != pools[0].shape[0] or p.device != pools[0].device:
             raise ValueError(f"{what}: pools have at least {rank} dimensions, one number of pages and one device")
-        if p.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{what}: pools are written in place and cannot require a gradient")
-    return pools
+
+
+def _check_grad(pools, what: str) -> None:
+    if torch.is_grad_enabled() and any(p.requires_grad for p in pools):
+        raise ValueError(f"{what}: pools are written in place and cannot require a gradient")
 
 
 def _dense(t: torch.Tensor, first: int) -> bool:
@@ -57,12 +67,24 @@ def _indexes(x, what: str) -> torch.Tensor:
     return t
 
 
-def copy_pages(pools, src, dst) -> None:
-    """See the module docstring."""
-    pools = _pools(pools, 2, "copy_pages")
-    src, dst = _indexes(src, "copy_pages: src"), _indexes(dst, "copy_pages: dst")
+def _plan_copy(pools, src, dst):
+    """(whether the kernel serves the call, (page stride, bytes of a page) of every pool that has any)."""
+    _check_pools(pools, 2, "copy_pages")
     if src.dim() != 1 or src.shape != dst.shape or src.device != dst.device:
         raise ValueError(f"copy_pages: src and dst are one list each, got {tuple(src.shape)} and {tuple(dst.shape)}")
+    dev = pools[0].device
+    if src.device.type != "cpu" and src.device != dev:
+        raise ValueError(f"copy_pages: indexes on {src.device}, pools on {dev}")
+    covered = dev.type == "cuda" and all(_dense(p, 1) for p in pools) and src.shape[0] <= MAX_PAIRS
+    return covered, tuple((p.stride(0) * p.element_size(), 0, 0, (p.numel() // p.shape[0]) * p.element_size()) if p.numel() else None for p in pools)
+
+
+def copy_pages(pools, src, dst) -> None:
+    """See the module docstring."""
+    pools = _pools(pools)
+    src, dst = _indexes(src, "copy_pages: src"), _indexes(dst, "copy_pages: dst")
+    covered, shapes = _plans.get((*map(meta, pools), meta(src), meta(dst)), _plan_copy, pools, src, dst)
+    _check_grad(pools, "copy_pages")
     dev, n = pools[0].device, pools[0].shape[0]
     if src.device.type == "cpu":
         used = [(s, d) for s, d in zip(src.tolist(), dst.tolist()) if (s, d) != (-1, -1)]
@@ -76,30 +98,28 @@ def copy_pages(pools, src, dst) -> None:
             return
         if len(used) < src.shape[0]:
             src, dst = torch.tensor([s for s, _ in used]), torch.tensor(to)
-    elif src.device != dev:
-        raise ValueError(f"copy_pages: indexes on {src.device}, pools on {dev}")
     if src.shape[0] == 0 or n == 0:
         return
-    if not B.on_gpu(*pools) or not all(_dense(p, 1) for p in pools) or src.shape[0] > MAX_PAIRS:
+    if not covered or not B.kernels_enabled():
         s, d = src.to(dev, torch.int64), dst.to(dev, torch.int64)
-        if src.device.type != "cpu":       # unused places copy page 0 to itself
+        if src.device.type != "cpu":       # unused places are left out
             pad = (s == -1) & (d == -1)
             s, d = (s[~pad], d[~pad]) if bool(pad.any()) else (s, d)
         for p in pools:
             p[d] = p[s]
         return
-    lib = B.load_library()
     with on_device(dev):
-        s, d = (x.to(dev, torch.int32, non_blocking=True).contiguous() for x in (src, dst))
-        for at in range(0, len(pools), MAX_POOLS):
-            part = [p for p in pools[at:at + MAX_POOLS] if p.numel()]
-            if not part:
-                continue
-            bases = (ctypes.c_void_p * len(part))(*(p.data_ptr() for p in part))
-            lp = (ctypes.c_longlong * (4 * len(part)))(*(x for p in part for x in (
-                p.stride(0) * p.element_size(), 0, 0, p[0].numel() * p.element_size())))
-            B.check(lib.cmb_copy_pages(bases, lp, len(part), B.ptr(s), B.ptr(d), s.shape[0], n, B.ptr(B.status_buffer(dev)),
-                                       B.stream_ptr()), "copy_pages")
+        if src.dtype != torch.int32 or src.device != dev or not src.is_contiguous():
+            src = src.to(dev, torch.int32, non_blocking=True).contiguous()
+        if dst.dtype != torch.int32 or dst.device != dev or not dst.is_contiguous():
+            dst = dst.to(dev, torch.int32, non_blocking=True).contiguous()
+        packed = [_POOL.pack(p.data_ptr(), *x) for p, x in zip(pools, shapes) if x is not None]
+        fn = entry("cmb_copy_pages", ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                   ctypes.c_void_p)
+        for at in range(0, len(packed), MAX_POOLS):
+            part = packed[at:at + MAX_POOLS]
+            B.check(fn(b"".join(part), len(part), src.data_ptr(), dst.data_ptr(), src.shape[0], n, B.status_buffer(dev).data_ptr(),
+                       _raw_stream(dev.index)), "copy_pages")
 
 
 def compact_rows_reference(pools, table, start, path, counts) -> None:
@@ -114,14 +134,12 @@ def compact_rows_reference(pools, table, start, path, counts) -> None:
         p[table[b, to // page].long(), :, to % page] = p[table[b, fro // page].long(), :, fro % page]
 
 
-def compact_rows(pools, table, start, path, counts) -> None:
-    """See the module docstring.  table [B, W], start [B], path [B, P], counts [B], int32 / int64 on the pools' device."""
-    pools = _pools(pools, 4, "compact_rows")
+def _plan_compact(pools, table, start, path, counts):
+    """(whether the kernel serves the call, (strides, bytes of a row) of every pool, the entry's sizes)."""
+    _check_pools(pools, 4, "compact_rows")
     dev = pools[0].device
     if any(p.shape[:3] != pools[0].shape[:3] for p in pools):
         raise ValueError("compact_rows: pools differ in pages, layers or page size")
-    table, start, path, counts = (_indexes(x, f"compact_rows: {n}") for x, n in
-                                  ((table, "table"), (start, "start"), (path, "path"), (counts, "counts")))
     b = table.shape[0]
     if table.dim() != 2 or path.dim() != 2 or path.shape[0] != b or start.shape != (b,) or counts.shape != (b,):
         raise ValueError(f"compact_rows: table {tuple(table.shape)}, start {tuple(start.shape)}, path {tuple(path.shape)} and counts "
@@ -130,9 +148,26 @@ def compact_rows(pools, table, start, path, counts) -> None:
         raise ValueError(f"compact_rows: indexes and pools are on one device ({dev})")
     if path.shape[1] > MAX_MOVES:
         raise ValueError(f"compact_rows: at most {MAX_MOVES} rows of a sequence, got {path.shape[1]}")
-    if b == 0 or path.shape[1] == 0 or pools[0].numel() == 0:
-        return
     n, layers, page = pools[0].shape[:3]
+    covered = (dev.type == "cuda" and all(_dense(p, 3) for p in pools) and b <= 65535 and min(len(pools), MAX_POOLS) * layers <= 65535
+               and table.shape[1] > 0)
+    size = [p.element_size() for p in pools]
+    shapes = tuple((p.stride(0) * e, p.stride(1) * e, p.stride(2) * e, p.numel() // max(1, n * layers * page) * e) for p, e in zip(pools, size))
+    return covered, shapes, struct.pack("6i", b, table.shape[1], path.shape[1], page, n, layers)
+
+
+def compact_rows(pools, table, start, path, counts) -> None:
+    """See the module docstring.  table [B, W], start [B], path [B, P], counts [B], int32 / int64 on the pools' device."""
+    pools = _pools(pools)
+    table, start, path, counts = (_indexes(table, "compact_rows: table"), _indexes(start, "compact_rows: start"),
+                                  _indexes(path, "compact_rows: path"), _indexes(counts, "compact_rows: counts"))
+    covered, shapes, ip = _plans.get((*map(meta, pools), meta(table), meta(start), meta(path), meta(counts)), _plan_compact, pools, table, start,
+                                     path, counts)
+    _check_grad(pools, "compact_rows")
+    dev = pools[0].device
+    if path.shape[0] == 0 or path.shape[1] == 0 or any(p.numel() == 0 for p in pools):
+        return
+    n, page = pools[0].shape[0], pools[0].shape[2]
     if dev.type == "cpu":
         i = torch.arange(path.shape[1])
         use = i < counts[:, None]
@@ -145,18 +180,16 @@ def compact_rows(pools, table, start, path, counts) -> None:
         need &= (counts > 0)[:, None]
         if bool(((table < 0) | (table >= n))[need].any()):
             raise ValueError(f"compact_rows: a page outside the pool of {n}")
-    if not B.on_gpu(*pools) or not all(_dense(p, 3) for p in pools) or b > 65535 or len(pools[:MAX_POOLS]) * layers > 65535:
+    if not covered or not B.kernels_enabled():
         compact_rows_reference(pools, table, start, path, counts)
         return
-    lib = B.load_library()
     with on_device(dev):
-        table, start, path, counts = (x.to(torch.int32).contiguous() for x in (table, start, path, counts))
-        ip = (ctypes.c_int * 6)(b, table.shape[1], path.shape[1], page, n, layers)
-        for at in range(0, len(pools), MAX_POOLS):
-            part = pools[at:at + MAX_POOLS]
-            bases = (ctypes.c_void_p * len(part))(*(p.data_ptr() for p in part))
-            lp = (ctypes.c_longlong * (4 * len(part)))(*(x for p in part for x in (
-                p.stride(0) * p.element_size(), p.stride(1) * p.element_size(), p.stride(2) * p.element_size(),
-                p[0, 0, 0].numel() * p.element_size())))
-            B.check(lib.cmb_compact_rows(bases, lp, len(part), B.ptr(table), B.ptr(start), B.ptr(path), B.ptr(counts), ip,
-                                         B.ptr(B.status_buffer(dev)), B.stream_ptr()), "compact_rows")
+        table, start, path, counts = (x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+                                      for x in (table, start, path, counts))
+        packed = [_POOL.pack(p.data_ptr(), *x) for p, x in zip(pools, shapes)]
+        fn = entry("cmb_compact_rows", ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                   ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p)
+        for at in range(0, len(packed), MAX_POOLS):
+            part = packed[at:at + MAX_POOLS]
+            B.check(fn(b"".join(part), len(part), table.data_ptr(), start.data_ptr(), path.data_ptr(), counts.data_ptr(), ip,
+                       B.status_buffer(dev).data_ptr(), _raw_stream(dev.index)), "compact_rows")

@@ -22,6 +22,8 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import struct
+from typing import NamedTuple
 
 import torch
 
@@ -105,20 +107,30 @@ def window_attention_reference(q, k, v, *, window: int | None = None, sink_token
 
 # ------------------------------------------------------------------------------------------------------------ kernel path
 @contextlib.contextmanager
+def _other_device(device: torch.device):
+    with torch.cuda.device(device):
+        yield
+
+
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """Kernels run on the current device's current stream: make it the tensors' device for the call."""
-    if device.index == torch.cuda.current_device():
-        yield
-    else:
-        with torch.cuda.device(device):
-            yield
+    return _HERE if device.index == torch.cuda.current_device() else _other_device(device)
 
 
 def usable(t: torch.Tensor) -> bool:
-    """A layout that the kernels read in place: unit inner stride, other strides (of dimensions longer than 1) positive
-    multiples of 8 elements, 16-byte aligned."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
+    """A layout that the kernels read in place (its address apart, which must be a multiple of 16 bytes): unit inner stride, other
+    strides (of dimensions longer than 1) positive multiples of 8 elements."""
+    return t.stride(-1) == 1 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+
+
+def in_place(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a dense copy of it where the kernels cannot read it as it lies."""
+    if usable(t):
+        return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t.contiguous()
 
 
 def strides3(t: torch.Tensor) -> tuple[int, int, int]:
@@ -128,9 +140,13 @@ def strides3(t: torch.Tensor) -> tuple[int, int, int]:
 
 def kernel_covers(q, k, v) -> bool:
     """Types, head sizes and devices of the kernels (layouts apart)."""
+    return B.on_gpu(q, k, v) and _sizes_covered(q, k, v)
+
+
+def _sizes_covered(q, k, v) -> bool:
     dq, dv = q.shape[3], v.shape[3]
-    return (B.on_gpu(q, k, v) and q.dtype == k.dtype == v.dtype == torch.bfloat16 and dq % 8 == 0 and dv % 8 == 0
-            and dq <= MAX_HEAD_DIM and dv <= MAX_HEAD_DIM and q.shape[2] // k.shape[2] <= MAX_GROUP and k.shape[2] <= 65535)
+    return (q.is_cuda and q.dtype == k.dtype == v.dtype == torch.bfloat16 and dq % 8 == 0 and dv % 8 == 0 and dq <= MAX_HEAD_DIM
+            and dv <= MAX_HEAD_DIM and q.shape[2] // k.shape[2] <= MAX_GROUP and k.shape[2] <= 65535 and q.shape[0] <= 65535)
 
 
 def choose_splits(ctas: int, tiles: int) -> int:
@@ -153,13 +169,66 @@ def sink_split(s: int, t: int, window: int, sink_tokens: int, g: int) -> tuple[i
     return tiles, max(1, min(64, -(-s // (window + 128))))
 
 
-def launch_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page: int, window, sink_tokens, sinks, scale, want_lse: bool,
-                   max_keys: int | None = None):
-    """``cmb_window_fwd`` on checked arguments in usable layouts; (o, lse or None)."""
-    lib = B.load_library()
+def meta(t):
+    """What a call's preparation depends on of a tensor: nothing of its address or contents."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+class Plans:
+    """Prepared calls by their tensors' layouts and their options (checks done, arguments packed); forgotten when there are many."""
+
+    def __init__(self, most: int = 1024):
+        self.most, self.plans = most, {}
+
+    def get(self, key, make, *args):
+        plan = self.plans.get(key)
+        if plan is None:
+            plan = make(*args)
+            if len(self.plans) >= self.most:
+                self.plans.clear()
+            self.plans[key] = plan
+        return plan
+
+
+_CALL, _AT = struct.Struct("18i12qd"), struct.Struct("12Q")               # cmb_window_call, cmb_window_ptrs
+_BWD_CALL, _BWD_AT = struct.Struct("12i24qd"), struct.Struct("16Q")       # cmb_window_bwd_call, cmb_window_bwd_ptrs
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_entries: dict[str, object] = {}
+
+
+def entry(name: str, *argtypes):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(B.load_library(), name)
+        fn.argtypes, fn.restype = argtypes, ctypes.c_int
+        _entries[name] = fn
+    return fn
+
+
+def addr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+class ForwardPlan(NamedTuple):
+    covered: bool              # by the kernel, as far as types and sizes go
+    ready: bool                # the layouts are read in place
+    scale: float
+    call: bytes = b""
+    out_shape: tuple = ()
+    rows: int = 0              # B S H
+    ws: int = 0                # floats of scratch; the (max, sum) pairs begin at ws_ml
+    ws_ml: int = 0
+    convert: tuple = (False, False, False)    # lengths, table, sinks need another type or layout
+    window: int = 0
+    sink_tokens: int = 0
+    bwd: dict | None = None
+
+
+def plan_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page: int, window, sink_tokens, sinks, scale,
+                 max_keys: int | None = None) -> ForwardPlan:
+    """Arguments of ``cmb_window_fwd`` for checked tensors in usable layouts."""
     b, s, h, dq = q.shape
     hk, dv = v.shape[2], v.shape[3]
-    dev = q.device
     w = NO_WINDOW if window is None else min(int(window), NO_WINDOW)
     g = h // hk
     blocks = row_blocks(s, g)
@@ -172,63 +241,99 @@ def launch_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page:
     box_k = 32 if one_tile else 64
     if table is not None:
         box_k = min(128 if one_tile else 64, page & -page)
-    out = torch.empty(b, s, h, dv, dtype=torch.bfloat16, device=dev)
-    lse = torch.empty(b, h, s, dtype=torch.float32, device=dev) if want_lse else None
-    ws = torch.empty(b * s * h * splits * (dv + 2), dtype=torch.float32, device=dev) if splits > 1 else None
-    ml = None if ws is None else ws[b * s * h * splits * dv:]
-    ip = (ctypes.c_int * 16)(b, s, t, h, hk, dq, dv, w, min(sink_tokens, NO_WINDOW), int(cached),
-                             s if tree is not None and tree.dim() == 2 else 0, 0 if table is None else table.shape[1], page,
-                             k.shape[0] if table is not None else 0, box_k, splits)
-    lp = (ctypes.c_longlong * 12)(*strides3(q), *strides3(k), *strides3(v), *strides3(out))
-    B.check(lib.cmb_window_fwd(B.ptr(q), B.ptr(k), B.ptr(v), B.ptr(lengths), B.ptr(tree), B.ptr(table), B.ptr(sinks), B.ptr(out),
-                               B.ptr(lse), B.ptr(ws), B.ptr(ml), ip, lp, ctypes.c_float(scale), B.ptr(B.status_buffer(dev)),
-                               B.stream_ptr()), "window_fwd")
+    out_shape = (b, s, h, dv)
+    o = tuple(x if n > 1 else 0 for n, x in zip(out_shape, (s * h * dv, h * dv, dv)))
+    sinks_bf16 = sinks is not None and sinks.dtype == torch.bfloat16
+    rows = b * s * h
+    call = _CALL.pack(b, s, t, h, hk, dq, dv, w, min(int(sink_tokens), NO_WINDOW), int(cached),
+                      s if tree is not None and tree.dim() == 2 else 0, 0 if table is None else table.shape[1], page,
+                      k.shape[0] if table is not None else 0, box_k, splits, int(sinks_bf16), 0, *strides3(q), *strides3(k), *strides3(v),
+                      *o, scale)
+    plain = lambda x: x is not None and (x.dtype != torch.int32 or not x.is_contiguous())  # noqa: E731
+    return ForwardPlan(True, True, scale, call, out_shape, rows, rows * splits * (dv + 2) if splits > 1 else 0, rows * splits * dv,
+                       (plain(lengths), plain(table), sinks is not None and (sinks.dtype not in (torch.bfloat16, torch.float32)
+                                                                            or not sinks.is_contiguous())), w, int(sink_tokens), {})
+
+
+def launch_forward(plan: ForwardPlan, q, k, v, lengths, tree, table, sinks, want_lse: bool):
+    """(o, lse or None) of a plan whose tensors are converted; the current device is theirs."""
+    dev = q.device
+    out = q.new_empty(plan.out_shape)
+    b, s, h, _ = plan.out_shape
+    lse = q.new_empty((b, h, s), dtype=torch.float32) if want_lse else None
+    ws = q.new_empty(plan.ws, dtype=torch.float32) if plan.ws else None
+    w0 = addr(ws)
+    at = _AT.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), addr(lengths), addr(tree), addr(table), addr(sinks), out.data_ptr(), addr(lse),
+                  w0, w0 + 4 * plan.ws_ml if w0 else 0, B.status_buffer(dev).data_ptr())
+    B.check(entry("cmb_window_fwd", ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p)(plan.call, at, _raw_stream(dev.index)), "window_fwd")
     return out, lse
+
+
+def converted(plan: ForwardPlan, lengths, table, sinks):
+    a, b, c = plan.convert
+    return (lengths.to(torch.int32).contiguous() if a else lengths, table.to(torch.int32).contiguous() if b else table,
+            sinks.float().contiguous() if c else sinks)
+
+
+def _plan_backward(q, k, v, do, sinks, plan: ForwardPlan, need_q: bool, need_kv: bool, need_s: bool):
+    b, s, h, dq = q.shape
+    t, hk, dv = v.shape[1:]
+    g = h // hk
+    tiles, splits = sink_split(s, t, plan.window, plan.sink_tokens, g)
+    if not need_kv:
+        splits = 1
+    dense = lambda x: tuple(st if n > 1 else 0 for n, st in zip(x.shape, (x.shape[1] * x.shape[2] * x.shape[3], x.shape[2] * x.shape[3], x.shape[3])))  # noqa: E731
+    o = tuple(st if n > 1 else 0 for n, st in zip(plan.out_shape, (s * h * dv, h * dv, dv)))
+    call = _BWD_CALL.pack(b, s, t, h, hk, dq, dv, plan.window, min(plan.sink_tokens, NO_WINDOW), tiles, splits,
+                          int(sinks is not None and sinks.dtype == torch.bfloat16), *strides3(q), *strides3(k), *strides3(v), *o, *strides3(do),
+                          *dense(q), *dense(k), *dense(v), plan.scale)
+    n_stats = 2 * plan.rows
+    n_sink = h * b * -(-s // min(s, 128 // g)) if need_s else 0
+    n_part = b * hk * tiles * splits * 128 * (dq + dv) if splits > 1 else 0
+    return call, n_stats, n_sink, n_part
 
 
 class _WindowAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, sinks, key_lengths, window, sink_tokens, scale):
-        with on_device(q.device):
-            sk = None if sinks is None else sinks.float().contiguous()
-            out, lse = launch_forward(q, k, v, t=k.shape[1], lengths=key_lengths, cached=False, tree=None, table=None, page=0,
-                                      window=window, sink_tokens=sink_tokens, sinks=sk, scale=scale, want_lse=True)
-        ctx.save_for_backward(q, k, v, sinks, key_lengths, out, lse)
-        ctx.args = (window, sink_tokens, scale)
+    def forward(ctx, q, k, v, sinks, lengths, plan):
+        out, lse = launch_forward(plan, q, k, v, lengths, None, None, sinks, True)
+        ctx.save_for_backward(q, k, v, sinks, lengths, out, lse)
+        ctx.plan = plan
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, sinks, lengths, out, lse = ctx.saved_tensors
-        window, sink_tokens, scale = ctx.args
+        plan = ctx.plan
         need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
-        b, s, h, dq_ = q.shape
-        t, hk, dv_ = v.shape[1:]
-        do = do if usable(do) else do.contiguous()
-        lib = B.load_library()
-        with on_device(q.device):
-            f32 = lambda *n: torch.empty(*n, dtype=torch.float32, device=q.device)  # noqa: E731
-            sk = None if sinks is None else sinks.float().contiguous()
-            sink_part = f32(h, b * -(-s // min(s, 128 // (h // hk)))) if sinks is not None and need_s else None
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q or need_s else None
-            dk, dv = ((torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (k, v)) if need_k or need_v else (None, None))
-            w = NO_WINDOW if window is None else min(int(window), NO_WINDOW)
-            tiles, splits = sink_split(s, t, w, sink_tokens, h // hk)
-            part = f32(b * hk * tiles * splits * 128 * (dq_ + dv_)) if splits > 1 and dk is not None else None
-            ip = (ctypes.c_int * 11)(b, s, t, h, hk, dq_, dv_, w, min(sink_tokens, NO_WINDOW), tiles, splits if part is not None else 1)
-            lp = (ctypes.c_longlong * 24)(*(st for x in (q, k, v, out, do, dq, dk, dv) for st in ((0, 0, 0) if x is None else strides3(x))))
-            stats = f32(2 * b * s * h)
-            B.check(lib.cmb_window_bwd(B.ptr(q), B.ptr(k), B.ptr(v), B.ptr(out), B.ptr(do), B.ptr(lengths), B.ptr(sk), B.ptr(lse),
-                                       B.ptr(dq), B.ptr(dk), B.ptr(dv), B.ptr(stats), B.ptr(sink_part), B.ptr(part), ip, lp,
-                                       ctypes.c_float(scale), B.ptr(B.status_buffer(q.device)), B.stream_ptr()), "window_bwd")
-            ds = None if sink_part is None else sink_part.sum(1).to(sinks.dtype)
-        return dq if need_q else None, dk if need_k else None, dv if need_v else None, ds, None, None, None, None
+        need_kv = need_k or need_v
+        do = in_place(do)
+        dev = q.device
+        key = (do.stride(), need_q, need_kv, need_s)
+        prepared = plan.bwd.get(key)
+        if prepared is None:
+            prepared = plan.bwd[key] = _plan_backward(q, k, v, do, sinks, plan, need_q, need_kv, need_s)
+        call, n_stats, n_sink, n_part = prepared
+        with on_device(dev):
+            dq = q.new_empty(q.shape) if need_q or need_s else None
+            dk = k.new_empty(k.shape) if need_kv else None
+            dv = v.new_empty(v.shape) if need_kv else None
+            ds = sinks.new_empty(sinks.shape) if need_s else None
+            n_stats_up = -(-n_stats // 4) * 4                # every part of the scratch begins on 16 bytes
+            ws = q.new_empty(n_stats_up + n_part + n_sink, dtype=torch.float32)
+            w0 = ws.data_ptr()
+            at = _BWD_AT.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), do.data_ptr(), addr(lengths), addr(sinks), lse.data_ptr(),
+                              addr(dq), addr(dk), addr(dv), addr(ds), w0, w0 + 4 * (n_stats_up + n_part) if n_sink else 0,
+                              w0 + 4 * n_stats_up if n_part else 0, B.status_buffer(dev).data_ptr())
+            B.check(entry("cmb_window_bwd", ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p)(call, at, _raw_stream(dev.index)), "window_bwd")
+        return dq if need_q else None, dk if need_k else None, dv if need_v else None, ds, None, None
 
 
-def window_attention(q, k, v, *, window: int | None = None, sink_tokens: int = 0, sinks: torch.Tensor | None = None,
-                     key_lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
-    """See the module docstring; returns [B, S, H, Dv] in ``q.dtype``."""
+_plans = Plans()
+
+
+def _plan(q, k, v, window, sink_tokens, sinks, key_lengths, scale) -> ForwardPlan:
     scale = _check(q, k, v, window, sink_tokens, sinks, scale, "window_attention")
     if q.shape[0] != k.shape[0]:
         raise ValueError(f"window_attention: batches of q ({q.shape[0]}) and k ({k.shape[0]}) differ")
@@ -236,18 +341,27 @@ def window_attention(q, k, v, *, window: int | None = None, sink_tokens: int = 0
         raise ValueError(f"window_attention: {q.shape[1]} queries are the last positions of at least as many keys, got {k.shape[1]}")
     if key_lengths is not None:
         _check_lengths(key_lengths, q.shape[0], q.device, "window_attention: key_lengths")
-    if not kernel_covers(q, k, v) or k.shape[1] > NO_WINDOW // 2 or q.shape[0] > 65535:
+    if not _sizes_covered(q, k, v) or k.shape[1] > NO_WINDOW // 2 or q.shape[0] == 0 or q.shape[1] == 0:
+        return ForwardPlan(False, False, scale)
+    if not (usable(q) and usable(k) and usable(v)):
+        return ForwardPlan(True, False, scale)
+    return plan_forward(q, k, v, t=k.shape[1], lengths=key_lengths, cached=False, tree=None, table=None, page=0, window=window,
+                        sink_tokens=sink_tokens, sinks=sinks, scale=scale)
+
+
+def window_attention(q, k, v, *, window: int | None = None, sink_tokens: int = 0, sinks: torch.Tensor | None = None,
+                     key_lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """See the module docstring; returns [B, S, H, Dv] in ``q.dtype``."""
+    plan = _plans.get((meta(q), meta(k), meta(v), meta(sinks), meta(key_lengths), window, sink_tokens, scale),
+                      _plan, q, k, v, window, sink_tokens, sinks, key_lengths, scale)
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (sinks is not None and sinks.requires_grad))
+    if not plan.covered or not B.kernels_enabled() or (grad and q.shape[2] // k.shape[2] > MAX_GROUP_GRAD):
         return window_attention_reference(q, k, v, window=window, sink_tokens=sink_tokens, sinks=sinks, key_lengths=key_lengths, scale=scale)
-    if q.shape[0] == 0 or q.shape[1] == 0:
-        return q.new_zeros(*q.shape[:3], v.shape[3])
-    q, k, v = (x if usable(x) else x.contiguous() for x in (q, k, v))
-    lengths = None if key_lengths is None else key_lengths.to(torch.int32).contiguous()
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, sinks)):
-        if q.shape[2] // k.shape[2] > MAX_GROUP_GRAD:
-            return window_attention_reference(q, k, v, window=window, sink_tokens=sink_tokens, sinks=sinks, key_lengths=key_lengths,
-                                              scale=scale)
-        return _WindowAttentionFn.apply(q, k, v, sinks, lengths, window, int(sink_tokens), scale)
+    if not plan.ready or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        return window_attention(in_place(q), in_place(k), in_place(v), window=window, sink_tokens=sink_tokens, sinks=sinks,
+                                key_lengths=key_lengths, scale=scale)
     with on_device(q.device):
-        sk = None if sinks is None else sinks.float().contiguous()
-        return launch_forward(q, k, v, t=k.shape[1], lengths=lengths, cached=False, tree=None, table=None, page=0, window=window,
-                              sink_tokens=int(sink_tokens), sinks=sk, scale=scale, want_lse=False)[0]
+        lengths, _, sk = converted(plan, key_lengths, None, sinks)
+        if grad:
+            return _WindowAttentionFn.apply(q, k, v, sk, lengths, plan)
+        return launch_forward(plan, q, k, v, lengths, None, None, sk, False)[0]
