@@ -35,7 +35,7 @@
 // Rows of V that no row may see (past a sequence's end, padding, pages handed on to others) may hold anything, NaN included:
 // a helper warp zeroes them in shared memory before they are multiplied with P's zeros.
 //
-// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 TMA producer, 9 / 10 scores and 12 / 13 products of stream 0 / 1, 11 the V helper.  Every wait is
+// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 and 14 TMA producers, 9 / 10 scores and 12 / 13 products of stream 0 / 1, 11 the V helper.  Every wait is
 // bounded (sm100.cuh).
 #include <cstring>
 
@@ -43,7 +43,7 @@
 
 namespace cmb {
 
-constexpr int WA_THREADS = 512;          // 14 warps with a role, in whole warp groups
+constexpr int WA_THREADS = 480;
 constexpr float WA_RESCALE = 8.f;        // log2 units a tile's maximum may exceed the reference before O is rescaled
 constexpr int WA_CTL = 3072;             // barriers (first 1 KB), (max, sum) of every row and stream (2 KB)
 
@@ -72,18 +72,20 @@ struct WindowParams {
 
 template <int DB, bool KEYS>
 struct WindowCfg {
-  static constexpr int BN = KEYS ? 128 : 64;             // keys of a tile
-  static constexpr int BUFS = KEYS ? 1 : 2;              // score buffers of a stream
+  static constexpr int BN = 64;                          // keys of a tile
+  static constexpr int BUFS = 2;                         // score buffers of a stream
+  static constexpr int CW = KEYS ? 16 : 32;              // keys of the chunks that a softmax thread works in
   static constexpr int KBLK = BN * 128;                  // bytes of a [BN keys x 64 columns] block
   static constexpr int Q_BYTES = (KEYS ? 1 : 2) * DB * WA_BLK;
-  static constexpr int NK = KEYS ? (DB == 2 ? 3 : 4) : (DB == 2 ? 5 : 8);
+  static constexpr int NK = DB == 2 ? (KEYS ? 6 : 5) : (KEYS ? 10 : 8);
   static constexpr int NV = NK;
   static constexpr int STAGE = DB * KBLK;
   static constexpr int SMEM_BYTES = Q_BYTES + (NK + NV) * STAGE + WA_CTL;
   static constexpr int PART_PITCH = DB * 64 + 4;         // floats; rows 16 bytes apart in banks
-  static_assert(SMEM_BYTES <= 232448, "shared memory");
+  static_assert(NK == NV && NK % 2 == 0 || !KEYS, "KEYS: a stream's stages keep their parity");
+  static_assert(SMEM_BYTES <= 232448 && (13 + 2 * NK + 3 * NV) * 8 + 8 <= 512, "shared memory");
   static_assert(!KEYS || 256 * PART_PITCH * 4 <= (NK + NV) * STAGE, "partial results reuse the rings");
-  // TMEM: stream s has O at 128 s and its scores at 256 + 128 s (+ 64 for ROWS' second buffer); P is written over the scores
+  // TMEM: stream s has O at 128 s and its score buffers at 256 + 128 s and 64 columns on; P is written over the scores
   static constexpr int O_STEP = 128, S_COL = 256, S_STEP = 128;
 };
 
@@ -192,6 +194,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   if (threadIdx.x == 0) {
     const uint32_t readers = !KEYS && two ? 2 : 1;     // MMA warps that read each tile
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
     mbar_init(q_full, 1);
     for (int i = 0; i < NK; ++i) {
       mbar_init(&k_full[i], 1);
@@ -225,71 +230,80 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // KEYS keeps 128 scores of a row in registers: 256 x 176 + 256 x 80 = the 512 x 128 that the block was launched with
   if (warp >= 8) {
-  if constexpr (KEYS) wa_fewer_registers<80>();
-  if (warp == 8) {
-    // ---------------------------------------------------------------- TMA producer (a box per lane)
-    if (lane == 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-    }
+  if (warp == 8 || warp == 14) {
+    // ---------------------------------------------------------------- TMA producers of keys (and queries) and of values: one thread
+    // of the warp issues (copies issued lane by lane cost 500 clocks each, and one thread for both was the bound of short
+    // windows), all look up pages, 32 boxes at a time and a batch ahead
     if (NT > 0) {
-      if (elect_one()) {
-        const uint32_t q_box = p.box_q * p.g * 128;
+      const bool is_k = warp == 8;
+      const CUtensorMap* map = is_k ? &tmK : &tmV;
+      uint8_t* ring = is_k ? ks : vs;
+      uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
+      int* pages = reinterpret_cast<int*>(ctl + (is_k ? 512 : 768));     // [2 batches][32 boxes]
+      const int per_tile = BN / p.box_k, batch = 32 / per_tile;     // boxes of a tile, tiles of a batch of lookups
+      const bool paged = p.table != nullptr;
+      auto look_up = [&](int i0) {           // the page of this lane's box, of the batch that begins at tile i0
+        const int i = i0 + lane / per_tile;
+        if (!paged || i >= t1) return 0;
+        const WaTile<BN> t(R, i);
+        const int j = t.k0 + (lane % per_tile) * p.box_k;
+        return j < t.k1() ? p.table[static_cast<long long>(b) * p.table_w + j / p.page] : 0;
+      };
+      int next = look_up(t0);
+      if (is_k && elect_one()) {
         const int nq = KEYS ? p.copies : (two ? 2 : 1);
-        mbar_arrive_expect_tx(q_full, q_box * nq * DB);
+        mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.box_q * p.g * 128) * nq * DB);
         for (int t = 0; t < nq; ++t)
           for (int kb = 0; kb < DB; ++kb)
             tma_load_5d(KEYS ? qs + kb * WA_BLK + t * p.copy_rows * 128 : qs + (t * DB + kb) * WA_BLK, &tmQ, q_full, kb * 64, 0,
                         KEYS ? s_first : s_first + t * p.box_q, hk, b);
       }
-      __syncwarp();
-      // lane i moves box i / DB of each tile, column block i % DB; BN / box_k boxes of <= 2 column blocks fit in 32 lanes
-      // (box_k >= 8).
-      const int my_box = lane / DB, my_kb = lane % DB;
-      auto page_of = [&](int i) {
-        if (i >= t1) return 0;
-        const WaTile t = R.tile(i);
-        const int j = t.k0 + my_box * p.box_k;
-        if (j >= t.k1 || p.table == nullptr) return b;
-        int id = p.table[static_cast<long long>(b) * p.table_w + j / p.page];
-        if (id < 0 || id >= p.num_pages) {
-          if (status != nullptr && atomicCAS(status, 0, ST_BAD_ARGUMENT) == 0) {
-            status[1] = b;
-            status[2] = j / p.page;
-            status[3] = id;
+      WaTile<BN> t(R, t0);
+      int kst = 0, kph = 1, row = paged ? t.k0 % p.page : t.k0;     // stage (keys and values run through as many), its phase, row in the page
+      for (int i0 = t0, odd = 0; i0 < t1; i0 += batch, odd ^= 32) {
+        if (paged) {
+          if (next < 0 || next >= p.num_pages) {     // reported, and read as page 0: the copies stay inside the pool
+            if (status != nullptr && atomicCAS(status, 0, ST_BAD_ARGUMENT) == 0) {
+              status[1] = b;
+              status[2] = i0 + lane / per_tile;
+              status[3] = next;
+            }
+            next = 0;
           }
-          id = 0;
+          pages[odd + lane] = next;
+          __syncwarp();
+          next = look_up(i0 + batch);
         }
-        return id;
-      };
-      auto load = [&](int i, uint8_t* ring, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int depth, int page) {
-        const int n = i - t0, st = n % depth;
-        const WaTile t = R.tile(i);
-        const int boxes = (t.k1 - t.k0 + p.box_k - 1) / p.box_k;
         bool ok = true;
-        if (elect_one()) {
-          ok = wa_wait(&empty[st], ((n / depth) & 1) ^ 1, abort_flag, status, ST_TIMEOUT_EMPTY);
-          if (ok) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(boxes) * p.box_k * 128 * DB);
+        if (elect_one()) {             // (always the same thread)
+          const int* page = pages + odd;
+          for (int i = i0; i < t1 && i < i0 + batch && ok; ++i) {
+            const int boxes = (t.keys() + p.box_k - 1) / p.box_k;
+            const uint32_t bytes = static_cast<uint32_t>(boxes) * p.box_k * 128 * DB;
+            ok = wa_wait(&empty[kst], kph, abort_flag, status, ST_TIMEOUT_EMPTY);
+            if (ok) {
+              mbar_arrive_expect_tx(&full[kst], bytes);
+              uint8_t* dst = ring + kst * Cfg::STAGE;
+              for (int m = 0; m < boxes; ++m) {
+                const int outer = paged ? page[m] : b;
+#pragma unroll
+                for (int kb = 0; kb < DB; ++kb) tma_load_4d(dst + kb * Cfg::KBLK, map, &full[kst], kb * 64, row, hk, outer);
+                dst += p.box_k * 128;
+                row += p.box_k;
+                if (paged && row == p.page) row = 0;
+              }
+            }
+            if (++kst == NK) {
+              kst = 0;
+              kph ^= 1;
+            }
+            t.next();
+            if (t.left == 0) row = paged ? t.k0 % p.page : t.k0;    // the window's first tile
+            page += per_tile;
+          }
         }
-        if (!__all_sync(0xffffffffu, ok)) return false;
-        const int j = t.k0 + my_box * p.box_k;
-        if (my_box < boxes)
-          tma_load_4d(ring + st * Cfg::STAGE + my_kb * Cfg::KBLK + my_box * p.box_k * 128, map, &full[st], my_kb * 64,
-                      p.table != nullptr ? j % p.page : j, hk, page);
-        return true;
-      };
-      // The keys run a tile ahead of the values: the next scores are wanted before this tile's product, and a stage of values
-      // is free later than one of keys.  Pages are looked up a tile before they are needed.
-      int page0 = page_of(t0), page1 = page_of(t0 + 1);
-      bool ok = load(t0, ks, &tmK, k_full, k_empty, NK, page0);
-      for (int i = t0; i < t1 && ok; ++i) {
-        const int page2 = page_of(i + 2);
-        if (i + 1 < t1) ok = load(i + 1, ks, &tmK, k_full, k_empty, NK, page1);
-        ok = ok && load(i, vs, &tmV, v_full, v_empty, NV, page0);
-        page0 = page1;
-        page1 = page2;
+        if (!__all_sync(0xffffffffu, ok)) break;
       }
     }
   } else if (warp == 11) {
@@ -300,16 +314,17 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const unsigned long long* tree = p.tree + static_cast<long long>(b) * p.tree_sb;
       for (int m = 0; m < p.S; ++m) nodes_any |= tree[m];
     }
+    WaTile<BN> t(R, t0);
+    int st = 0, ph = 0;
     for (int i = t0; i < t1; ++i) {
-      const int n = i - t0, st = n % NV;
-      const WaTile t = R.tile(i);
-      if (!wa_warp_wait(&v_full[st], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
-      const bool tail = t.k1 - t.k0 < BN, head = i >= R.n_s && t.k0 < R.wtrue;
-      const bool drafted = p.tree != nullptr && t.k1 > prefix;
+      if (!wa_warp_wait(&v_full[st], ph, abort_flag, status, ST_TIMEOUT_FULL)) break;
+      const int k1 = t.k1();
+      const bool tail = k1 - t.k0 < BN, head = t.in_window() && t.k0 < R.wtrue;
+      const bool drafted = p.tree != nullptr && k1 > prefix;
       if (tail || head || drafted) {
         for (int r = lane; r < BN; r += 32) {
           const int j = t.k0 + r;
-          const bool seen = j < t.k1 && (j >= R.wtrue || j < p.ns) &&
+          const bool seen = j < k1 && (j >= R.wtrue || j < p.ns) &&
                             (!drafted || j < prefix || (j - prefix < 64 && ((nodes_any >> (j - prefix)) & 1ull)));
           if (!seen) {
 #pragma unroll
@@ -322,8 +337,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         fence_proxy_async_smem();
       }
       wa_warp_arrive(&v_ready[st]);
+      t.next();
+      if (++st == NV) {
+        st = 0;
+        ph ^= 1;
+      }
     }
-  } else if (warp < 14) {
+  } else {
     // ---------------------------------------------------------------- MMA issuers: a thread each for the scores (warps 9, 10)
     // and the products (12, 13) of each stream.  One thread for both would hold a finished P back behind the scores of two tiles
     // later: an issuing thread advances no faster than the tensor pipe takes its instructions.
@@ -334,39 +354,48 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const uint32_t s_col = tmem_base + Cfg::S_COL + st * Cfg::S_STEP, o_col = tmem_base + Cfg::O_STEP * st;
       const int first = t0 + (KEYS ? st : 0), step = KEYS ? 2 : 1;
       int c = 0;                                       // tiles of this stream so far
+      WaTile<BN> t(R, first);
+      int stage = KEYS ? st : 0, phase = 0;
+      auto walk = [&] {
+        for (int f = 0; f < step; ++f) t.next();
+        stage += step;
+        if (stage >= NK) {
+          stage -= NK;
+          phase ^= 1;
+        }
+      };
       if (scores) {
         const uint64_t q_desc = make_smem_desc_sw128(smem_u32(qs) + (KEYS ? 0 : st * DB * WA_BLK), 16, 1024);
         const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ks), 16, 1024);
         bool ok = first >= t1 || wa_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
         for (int i = first; i < t1 && ok; i += step, ++c) {
-          const int n = i - t0, kst = n % NK, buf = c % BUFS;
-          const WaTile t = R.tile(i);
-          const uint32_t idesc_s = make_idesc(128, ((t.k1 - t.k0 + 15) >> 4) * 16, 1, 1, 0, 0);
-          const uint64_t kd = k_desc + static_cast<uint32_t>(kst * (Cfg::STAGE >> 4));
+          const int buf = c & 1;
+          const uint32_t idesc_s = make_idesc(128, (t.keys() + 15) & ~15, 1, 1, 0, 0);
+          const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
           const uint32_t d = s_col + buf * 64;
           // the scores take the place of an earlier tile's P, once the product has read it
-          if (c >= BUFS && !wa_wait(&pv_done[st * 2 + buf], (c / BUFS - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
-          if (!wa_wait(&k_full[kst], (n / NK) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
+          if (c >= 2 && !wa_wait(&pv_done[st * 2 + buf], ((c >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
+          if (!wa_wait(&k_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
           tc_fence_after();
 #pragma unroll
           for (int kb = 0; kb < DB; ++kb)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               umma_f16(d, q_desc + ((kb * WA_BLK + k * 32) >> 4), kd + ((kb * Cfg::KBLK + k * 32) >> 4), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&k_empty[kst]);
+          umma_commit(&k_empty[stage]);
           umma_commit(&s_full[st * 2 + buf]);
+          walk();
         }
       } else {
         constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
         const uint64_t v_desc = make_smem_desc_sw128(smem_u32(vs), Cfg::KBLK, 1024);
         for (int i = first; i < t1; i += step, ++c) {
-          const int n = i - t0, vst = n % NV, buf = c % BUFS;
-          const WaTile t = R.tile(i);
-          const int k16 = (t.k1 - t.k0 + 15) >> 4;
-          const uint64_t vd = v_desc + static_cast<uint32_t>(vst * (Cfg::STAGE >> 4));
+          const int buf = c & 1;
+          const int k16 = (t.keys() + 15) >> 4;
+          const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
           const uint32_t a = s_col + buf * 64;
-          if (!wa_wait(&v_ready[vst], (n / NV) & 1, abort_flag, status, ST_TIMEOUT_FULL)) break;
-          if (!wa_wait(&p_full[st * 2 + buf], (c / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
+          if (!wa_wait(&v_ready[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
+          if (!wa_wait(&p_full[st * 2 + buf], (c >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
           tc_fence_after();
           umma_f16_ts(o_col, a, vd, idesc_o, c > 0 ? 1u : 0u);
           if (k16 == BN / 16) {
@@ -375,15 +404,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           } else {
             for (int k = 1; k < k16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
           }
-          umma_commit(&v_empty[vst]);
+          umma_commit(&v_empty[stage]);
           umma_commit(&pv_done[st * 2 + buf]);
+          walk();
         }
       }
     }
   }
   } else {
     // ---------------------------------------------------------------- softmax and epilogue (a warp group per stream)
-    if constexpr (KEYS) wa_more_registers<176>();
     const int st = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
@@ -392,9 +421,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int copy = KEYS ? row / p.copy_rows : 0;
     const int rr = KEYS ? row - copy * p.copy_rows : row;          // row within the tile
     const WindowRow w = window_row(p, rr, KEYS ? s_first : s_first + st * p.box_q, hk, b, klim, prefix);
-    const int c_first = KEYS ? copy * (BN / 32 / p.copies) : 0;          // this thread's 32-key chunks of a tile
-    constexpr int CH = BN / 32;
-    const int c_count = KEYS ? CH / p.copies : CH;
+    constexpr int CW = Cfg::CW, CH = BN / CW;
+    const int c_count = KEYS ? CH / p.copies : CH, c_first = KEYS ? copy * c_count : 0;      // this thread's chunks of a tile
     const bool warp_ok = __any_sync(0xffffffffu, w.ok);
     // what every row of the warp sees (rows that are not ok are never read): most tiles need no mask
     const int all_upto = __reduce_min_sync(0xffffffffu, w.ok ? w.plim : 0x7fffffff);
@@ -407,9 +435,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       auto scores_in = [&](int at) {         // tile `at` of this stream: are its scores there?
         return wa_warp_wait(&s_full[st * 2 + at % BUFS], (at / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       };
-      uint32_t x[CH][32];                    // the scores of this thread's chunks
+      uint32_t x[CH][CW];                    // the scores of this thread's chunks
       auto load = [&](int e, int chunks, int at) {
-        if (e < c_count && c_first + e < chunks) tmem_ld_x32(s_base + (at % BUFS) * 64 + (c_first + e) * 32, x[e]);
+        if (e < c_count && c_first + e < chunks) {
+          const uint32_t a = s_base + (at % BUFS) * 64 + (c_first + e) * CW;
+          if constexpr (CW == 32) tmem_ld_x32(a, x[e]);
+          else tmem_ld_x16(a, x[e]);
+        }
       };
       for (int i = first; i < t1 && !warp_ok; i += step, ++c) {    // no rows: this warp only keeps step
         if (!scores_in(c)) {
@@ -418,8 +450,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         wa_warp_arrive(&p_full[st * 2 + c % BUFS]);
       }
-      WaTile t = R.tile(first);
-      int chunks = (t.k1 - t.k0 + 31) >> 5;  // 32-key chunks that the tile has
+      WaTile<BN> t(R, first);
+      int chunks = (t.keys() + CW - 1) / CW; // chunks that the tile has
       if (warp_ok && first < t1) {
         ok = scores_in(0);
         tc_fence_after();
@@ -431,14 +463,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int i = first; i < t1 && warp_ok && ok; i += step, ++c) {
         const int buf = c % BUFS;
         const uint32_t s_addr = s_base + buf * 64;
-        const bool whole = t.k1 - t.k0 == BN && t.k1 - 1 <= all_upto && (t.k0 >= all_from || t.k1 <= p.ns);
+        const int k1 = t.k1();
+        const bool whole = k1 - t.k0 == BN && k1 - 1 <= all_upto && (t.k0 >= all_from || k1 <= p.ns);
         if (!whole) {                        // what is masked may be NaN: selected, not added to
 #pragma unroll
           for (int e = 0; e < CH; ++e) {
             if (e < c_count && c_first + e < chunks) {
-              const unsigned word = window_word(p, w, t.k0 + (c_first + e) * 32, t.k1, prefix);
+              const unsigned word = window_word(p, w, t.k0 + (c_first + e) * CW, k1, prefix);
 #pragma unroll
-              for (int i2 = 0; i2 < 32; ++i2) x[e][i2] = (word >> i2) & 1u ? x[e][i2] : 0xff800000u;
+              for (int i2 = 0; i2 < CW; ++i2) x[e][i2] = (word >> i2) & 1u ? x[e][i2] : 0xff800000u;
             }
           }
         }
@@ -449,7 +482,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         for (int e = 0; e < CH; ++e) {
           if (e < c_count && c_first + e < chunks) {
 #pragma unroll
-            for (int i2 = 0; i2 < 32; i2 += 16)
+            for (int i2 = 0; i2 < CW; i2 += 16)
 #pragma unroll
               for (int u = 0; u < 8; ++u)
                 m8[u] = fmaxf(fmaxf(m8[u], __uint_as_float(x[e][i2 + 2 * u])), __uint_as_float(x[e][i2 + 2 * u + 1]));
@@ -465,9 +498,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             l_sum *= alpha;
           }
           if (c > 0) {
-            // O is rescaled when the previous tile's product has completed (KEYS: these scores were issued after it)
-            if (BUFS > 1 &&
-                !wa_warp_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) {
+            // O is rescaled when the previous tile's product has completed
+            if (!wa_warp_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) {
               ok = false;
               break;
             }
@@ -488,32 +520,31 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
         float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto probs = [&](int e) {
-          // P of chunk ch is columns 16 ch .. 16 ch + 15 of the scores, all read by now (the row's lane is this thread's)
+          // P of chunk ch is columns CW / 2 ch .. of the scores, all read by now (the row's lane is this thread's)
           if (e < c_count && c_first + e < chunks) {
-            uint32_t w16[16];
+            uint32_t w16[CW / 2];
 #pragma unroll
-            for (int i2 = 0; i2 < 16; ++i2) {
+            for (int i2 = 0; i2 < CW / 2; ++i2) {
               float2 v = fma2(make_float2(__uint_as_float(x[e][2 * i2]), __uint_as_float(x[e][2 * i2 + 1])), c2, neg_m);
               v.x = exp2f(v.x);
               v.y = exp2f(v.y);
               acc[i2 & 1] = add2(acc[i2 & 1], v);
               w16[i2] = pack_bf16x2(v.x, v.y);
             }
-            tmem_st_x16(s_addr + (c_first + e) * 16, w16);
+            if constexpr (CW == 32) tmem_st_x16(s_addr + (c_first + e) * 16, w16);
+            else tmem_st_x8(s_addr + (c_first + e) * 8, w16);
           }
         };
         const bool more = i + step < t1;
-        const WaTile tn = R.tile(i + step);
-        const int chunks_n = (tn.k1 - tn.k0 + 31) >> 5;
+        for (int f = 0; f < step; ++f) t.next();
+        const int chunks_n = (t.keys() + CW - 1) / CW;
 #pragma unroll
         for (int e = 0; e < CH; ++e) probs(e);
         if (KEYS && p.copies > 1) {          // the other copies' chunks count nothing here
-          uint32_t z[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) z[e] = 0u;
+          const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
           for (int ch = 0; ch < CH; ++ch)
-            if (ch < chunks && (ch < c_first || ch >= c_first + c_count)) tmem_st_x16(s_addr + ch * 16, z);
+            if (ch < chunks && (ch < c_first || ch >= c_first + c_count)) tmem_st_x8(s_addr + ch * 8, z);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -529,7 +560,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
         tmem_wait_ld();
-        t = tn;
         chunks = chunks_n;
       }
       // (the product before the last completes before it: one thread issued both)
@@ -701,24 +731,33 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams
   const long long bs = row / p.H;
   const int s = static_cast<int>(bs % p.S);
   const long long b = bs / p.S;
+  // lane i holds the (max, sum) of splits i and i + 32, then their weights; the partial outputs are fetched eight at a time
   const float2* ml = p.ws_ml + row * p.splits;
-  float top = -INFINITY;
-  for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, ml[i].x);
-  top = warp_max(top);
-  float l = 0.f;
+  const float2 none = make_float2(-INFINITY, 0.f);
+  const float2 v0 = lane < p.splits ? ml[lane] : none, v1 = lane + 32 < p.splits ? ml[lane + 32] : none;
+  float top = warp_max(fmaxf(v0.x, v1.x));
+  const float w0 = v0.x > -INFINITY ? exp2f(v0.x - top) : (v0.y == v0.y ? 0.f : v0.y);
+  const float w1 = v1.x > -INFINITY ? exp2f(v1.x - top) : (v1.y == v1.y ? 0.f : v1.y);
+  float l = warp_sum((w0 != 0.f ? w0 * v0.y : 0.f) + (w1 != 0.f ? w1 * v1.y : 0.f));
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < p.splits; ++i) {
-    const float2 v = ml[i];
-    const float wt = v.x > -INFINITY ? exp2f(v.x - top) : (v.y == v.y ? 0.f : v.y);
-    if (wt != 0.f) {
-      l += v.y * wt;
-      if (lane * 4 < p.Dv) {
-        const float4 a = *reinterpret_cast<const float4*>(p.ws_o + (row * p.splits + i) * p.Dv + lane * 4);
-        o.x = fmaf(a.x, wt, o.x);
-        o.y = fmaf(a.y, wt, o.y);
-        o.z = fmaf(a.z, wt, o.z);
-        o.w = fmaf(a.w, wt, o.w);
-      }
+  const bool in = lane * 4 < p.Dv;
+  const float* src = p.ws_o + row * p.splits * p.Dv + lane * 4;
+  for (int i0 = 0; i0 < p.splits; i0 += 8) {
+    float4 a[8];
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = i0 + i;
+      w[i] = __shfl_sync(0xffffffffu, at < 32 ? w0 : w1, at & 31);
+      a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in && at < p.splits && w[i] != 0.f) a[i] = *reinterpret_cast<const float4*>(src + static_cast<long long>(at) * p.Dv);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      o.x = fmaf(a[i].x, w[i], o.x);
+      o.y = fmaf(a[i].y, w[i], o.y);
+      o.z = fmaf(a[i].z, w[i], o.z);
+      o.w = fmaf(a[i].w, w[i], o.w);
     }
   }
   float f = 1.f;
@@ -824,7 +863,7 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
   p.splits = a.splits;
   p.lengths = static_cast<const int*>(at->lengths);
   p.sinks.p = at->sinks; p.sinks.bf16 = a.sinks_bf16;
-  if (B <= 0 || p.S <= 0 || p.Hk <= 0 || p.H <= 0 || p.H % p.Hk || p.T < 0 || p.splits < 1) return 1;
+  if (B <= 0 || p.S <= 0 || p.Hk <= 0 || p.H <= 0 || p.H % p.Hk || p.T < 0 || p.splits < 1 || p.splits > 64) return 1;
   p.g = p.H / p.Hk;
   if (p.g > 128 || p.Hk > 65535 || static_cast<long long>(B) * p.splits > 65535) return 1;
   if (Dq <= 0 || Dq > 128 || Dq % 8 || p.Dv <= 0 || p.Dv > 128 || p.Dv % 8) return 1;
@@ -832,13 +871,12 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
   if (p.cached && (p.lengths == nullptr || p.T < p.S)) return 1;
   if (!p.cached && (p.tree != nullptr || p.table != nullptr || p.T < p.S)) return 1;
   if (p.tree != nullptr && p.S > 64) return 1;
-  if (p.box_k != 8 && p.box_k != 16 && p.box_k != 32 && p.box_k != 64 && p.box_k != 128) return 1;
+  if (p.box_k != 8 && p.box_k != 16 && p.box_k != 32 && p.box_k != 64) return 1;
   if (p.table != nullptr && (p.page <= 0 || p.page % p.box_k || p.num_pages <= 0 || p.table_w <= 0 ||
                              static_cast<long long>(p.table_w) * p.page < p.T))
     return 1;
   const long long rows = static_cast<long long>(p.S) * p.g;
   const bool keys = rows <= 128;
-  if (!keys && p.box_k > 64) return 1;                     // a tile of 64 keys
   if (p.splits > 1 && (at->ws_o == nullptr || at->ws_ml == nullptr)) return 1;
   if ((a.o_sb | a.o_ss | a.o_sh) & 7 || (reinterpret_cast<uintptr_t>(at->out) & 15)) return 1;
   p.copies = 1;

@@ -22,11 +22,6 @@ struct WaSinks {
   }
 };
 
-// Keys [k0, k1) of one tile.
-struct WaTile {
-  int k0, k1;
-};
-
 // The key tiles of a block of rows whose positions lie in [pmin, pmax]: the visible first tokens [0, send), then the window
 // [wlo, kend), BN keys a tile.  Keys of the two ranges are disjoint.
 template <int BN>
@@ -46,12 +41,25 @@ struct WaRange {
     n_s = (send + BN - 1) / BN;
     n_t = n_s + (kend > wlo ? (kend - wlo + BN - 1) / BN : 0);
   }
-  __host__ __device__ WaTile tile(int i) const {
-    WaTile t;
-    t.k0 = i < n_s ? BN * i : wlo + BN * (i - n_s);
-    const int end = i < n_s ? send : kend;
-    t.k1 = t.k0 + BN < end ? t.k0 + BN : end;
-    return t;
+};
+// One tile, keys [k0, k1), and the way to the next: a few dependent instructions a step, because the issuing threads walk alone.
+template <int BN>
+struct WaTile {
+  int k0, end;       // end of the range that the tile is in
+  int left, wlo, kend;    // tiles of the first range from this one on (<= 0: in the window)
+  __host__ __device__ WaTile(const WaRange<BN>& r, int i) : left(r.n_s - i), wlo(r.wlo), kend(r.kend) {
+    k0 = left > 0 ? BN * i : r.wlo + BN * (i - r.n_s);
+    end = left > 0 ? r.send : r.kend;
+  }
+  __host__ __device__ int keys() const { return end - k0 < BN ? end - k0 : BN; }
+  __host__ __device__ int k1() const { return k0 + keys(); }
+  __host__ __device__ bool in_window() const { return left <= 0; }
+  __host__ __device__ void next() {
+    k0 += BN;
+    if (--left == 0) {
+      k0 = wlo;
+      end = kend;
+    }
   }
 };
 
@@ -74,6 +82,11 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -112,15 +125,6 @@ __device__ __forceinline__ bool wa_warp_wait(uint64_t* bar, uint32_t parity, vol
 __device__ __forceinline__ void wa_warp_arrive(uint64_t* bar) {      // one arrival for the warp's work so far
   __syncwarp();
   if (elect_one()) mbar_arrive(bar);
-}
-// Registers of a warp group, moved between the groups of a block: the sum never exceeds what the block was launched with.
-template <int N>
-__device__ __forceinline__ void wa_more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void wa_fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 // Two fp32 operations of one instruction (a pair of registers each).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {

@@ -185,7 +185,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         uint8_t* t2 = t1 + DB * WB_SBLK;
         for (int kb = 0; kb < DB; ++kb) {
           if (MODE == WB_DQ) {
-            const int k0 = R.tile(n).k0;
+            const int k0 = WaTile<64>(R, n).k0;
             tma_load_4d(t1 + kb * WB_SBLK, &tmT1, &t_full[st], kb * 64, k0, hk, b);
             tma_load_4d(t2 + kb * WB_SBLK, &tmT2, &t_full[st], kb * 64, k0, hk, b);
           } else {
@@ -215,9 +215,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         aux[st * WB_SUB + lane] = v[0];
         aux[st * WB_SUB + 32 + lane] = v[1];
       } else {
-        const WaTile t = R.tile(n);
-        if (t.k1 - t.k0 < WB_SUB) {
-          for (int r = t.k1 - t.k0 + (lane >> 3); r < WB_SUB; r += 4)
+        const WaTile<64> t(R, n);
+        if (t.keys() < WB_SUB) {
+          for (int r = t.keys() + (lane >> 3); r < WB_SUB; r += 4)
 #pragma unroll
             for (int kb = 0; kb < DB; ++kb)
               *reinterpret_cast<uint4*>(ts + st * Cfg::STAGE + kb * WB_SBLK + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -297,11 +297,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       unsigned words[2] = {0u, 0u};
       if (row_ok) {
         if (MODE == WB_DQ) {
-          const WaTile t = R.tile(n);
+          const WaTile<64> t(R, n);
           const int pos = off + qi;
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            words[i] = wa_mask_word(t.k0 + 32 * i, min(pos, klim - 1), pos - p.window + 1, p.ns, t.k1);
+            words[i] = wa_mask_word(t.k0 + 32 * i, min(pos, klim - 1), pos - p.window + 1, p.ns, t.k1());
         } else {     // the columns [lo, hi) of this key: rows at or behind it, inside its window
           const int j = row0 + row, q0 = (n_first + n) * p.sub_q;
           const int first = min(max(j - off - q0, 0), p.sub_q);

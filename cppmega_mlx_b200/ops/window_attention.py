@@ -150,7 +150,7 @@ def _sizes_covered(q, k, v) -> bool:
 
 
 def choose_splits(ctas: int, tiles: int) -> int:
-    """How many ways to split the key axis of ``ctas`` thread blocks whose rows see about ``tiles`` 128-key tiles: enough blocks for
+    """How many ways to split the key axis of ``ctas`` thread blocks whose rows see about ``tiles`` 64-key tiles: enough blocks for
     every SM, two tiles (one per stream of the kernel) or more to a block."""
     return max(1, min(NUM_SMS // max(1, ctas), (tiles + 1) // 2, 64))
 
@@ -234,13 +234,10 @@ def plan_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page: i
     blocks = row_blocks(s, g)
     span = s if tree is not None or blocks == 1 else 2 * (128 // g)
     reach = min(t if max_keys is None else min(t, max_keys), w + span)
-    splits = choose_splits(b * hk * blocks, -(-reach // 128) + -(-min(sink_tokens, t) // 128))
+    splits = choose_splits(b * hk * blocks, -(-reach // 64) + -(-min(sink_tokens, t) // 64))
     if b * splits > 65535:
         splits = 1
-    one_tile = s * g <= 128                                # the kernel's form for few rows: 128 keys a tile, else 64
-    box_k = 32 if one_tile else 64
-    if table is not None:
-        box_k = min(128 if one_tile else 64, page & -page)
+    box_k = 64 if table is None else min(64, page & -page)     # key rows of one copy; a tile is 64 keys
     out_shape = (b, s, h, dv)
     o = tuple(x if n > 1 else 0 for n, x in zip(out_shape, (s * h * dv, h * dv, dv)))
     sinks_bf16 = sinks is not None and sinks.dtype == torch.bfloat16
