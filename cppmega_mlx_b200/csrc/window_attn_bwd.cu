@@ -78,11 +78,10 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   uint64_t* r_full = reinterpret_cast<uint64_t*>(ctl);
   uint64_t* t_full = r_full + 1;             // [WB_NS] landed
   uint64_t* t_ready = t_full + WB_NS;        // [WB_NS] cleaned, row statistics fetched
-  uint64_t* t_empty = t_ready + WB_NS;       // [WB_NS]
+  uint64_t* t_empty = t_ready + WB_NS;       // [WB_NS] gradient products done
   uint64_t* x_full = t_empty + WB_NS;        // [2] scores
   uint64_t* a_full = x_full + 2;             // [2] P, dS written
-  uint64_t* g_done = a_full + 2;             // [2] gradient products
-  uint64_t* all_done = g_done + 2;           // every product (a phase bit of g_done could not tell the last from one two earlier)
+  uint64_t* all_done = a_full + 2;           // every product
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* aux = reinterpret_cast<float2*>(ctl + 1024);          // [WB_NS][64]
@@ -135,7 +134,6 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(&x_full[i], 1);
       mbar_init(&a_full[i], 4);
-      mbar_init(&g_done[i], 1);
     }
     mbar_init(all_done, 1);
     *abort_flag = 0;
@@ -239,7 +237,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         const int st = n % WB_NS, buf = n & 1;
         if (!wa_wait(&t_ready[st], (n / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_FULL)) return false;
         // the buffer holds P and dS of sub-tile n - 2 until its gradient products have read them
-        if (n >= 2 && !wa_wait(&g_done[buf], ((n >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
+        if (n >= 2 && !wa_wait(&t_empty[(n - 2) % WB_NS], ((n - 2) / WB_NS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
         tc_fence_after();
         const uint32_t x = tmem_base + Cfg::X_COL + buf * 128;
         const uint64_t t1 = td + static_cast<uint32_t>(st * (Cfg::STAGE >> 4)), t2 = t1 + ((DB * WB_SBLK) >> 4);
@@ -270,7 +268,6 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
           umma_f16_ts(tmem_base + Cfg::O1_COL, x + 64 + k * 8, t1 + ((k * 2048) >> 4), idesc_g, (n > 0 || k > 0) ? 1u : 0u);
         }
         umma_commit(&t_empty[st]);
-        umma_commit(&g_done[buf]);
         if (n == NT - 1) umma_commit(all_done);
       }
     }
@@ -290,6 +287,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       lse2 = v.x;
       delta = v.y;
     }
+    const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     float row_dot = 0.f;                   // SINKS: sum_j p_ij dP_ij over this warp group's keys
     for (int n = st_id; n < NT; n += 2) {
@@ -348,20 +346,20 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
           float4 a;
           if (MODE == WB_DKV) a = a4[e];
           else a = make_float4(lse2, delta, lse2, delta);
-          float p0 = exp2f(fmaf(__uint_as_float(x1[2 * e]), p.scale_log2, -a.x));
-          float p1 = exp2f(fmaf(__uint_as_float(x1[2 * e + 1]), p.scale_log2, -a.z));
-          float d0 = p0 * (__uint_as_float(x2[2 * e]) - a.y);
-          float d1 = p1 * (__uint_as_float(x2[2 * e + 1]) - a.w);
+          float2 pr = fma2(make_float2(__uint_as_float(x1[2 * e]), __uint_as_float(x1[2 * e + 1])), c2, make_float2(-a.x, -a.z));
+          pr.x = exp2f(pr.x);
+          pr.y = exp2f(pr.y);
+          float2 d = mul2(pr, add2(make_float2(__uint_as_float(x2[2 * e]), __uint_as_float(x2[2 * e + 1])), make_float2(-a.y, -a.w)));
           if (!full) {      // selected, not multiplied: what is masked may be NaN
             const bool v0 = (words[i] >> (2 * e)) & 1u, v1 = (words[i] >> (2 * e + 1)) & 1u;
-            p0 = v0 ? p0 : 0.f;
-            d0 = v0 ? d0 : 0.f;
-            p1 = v1 ? p1 : 0.f;
-            d1 = v1 ? d1 : 0.f;
+            pr.x = v0 ? pr.x : 0.f;
+            d.x = v0 ? d.x : 0.f;
+            pr.y = v1 ? pr.y : 0.f;
+            d.y = v1 ? d.y : 0.f;
           }
-          if (SINKS) row_dot += fmaf(p0, delta, d0) + fmaf(p1, delta, d1);
-          pw[e] = pack_bf16x2(p0, p1);
-          dw[e] = pack_bf16x2(d0, d1);
+          if (SINKS) row_dot += fmaf(pr.x, delta, d.x) + fmaf(pr.y, delta, d.y);
+          if (MODE == WB_DKV) pw[e] = pack_bf16x2(pr.x, pr.y);
+          dw[e] = pack_bf16x2(d.x, d.y);
         }
         if (MODE == WB_DKV) tmem_st_x16(x_addr + 16 * i, pw);
         tmem_st_x16(x_addr + 64 + 16 * i, dw);
