@@ -12,13 +12,17 @@
 //
 //   S = Q.K^T       tcgen05.mma 128 x n x 16, fp32 in TMEM (n = the tile's keys, rounded up to 16: the few first tokens and the
 //                   last tile cost what they hold)
-//   P = exp2(S c - m)   one row per thread, its scores in registers (setmaxnreg), P written back to TMEM as bf16.  P's rounding (half
+//   P = exp2(S c - m)   one row per thread, its scores in registers, P written back over S in TMEM as bf16.  P's rounding (half
 //                   a step, 2^-8) is that of the product's operand type; the row's sum is of the unrounded values in fp32.
 //   O += P.V        A from TMEM (from shared memory, P and its reads would cost half as much shared-memory bandwidth again as
 //                   the K, V and Q reads that already take most of it), V read MN-major in place, accumulator resident in TMEM
 //
-// The running maximum m moves only when a tile exceeds it by 2^8 (numerator and denominator share it, so the result does not
-// depend on when); O is rescaled in TMEM only then.  Two streams (softmax warp group + MMA-issuing warp each) share the CTA so
+// The reference m need not be the maximum: bf16 and fp32 share the exponent range, so P, its sum and O keep their precision at any m
+// that neither overflows nor loses the largest terms.  m is the maximum of the first tile with a key, and moves (O rescaled in
+// TMEM) when a tile's sum comes out above 2^40; terms 2^126 below m are nothing beside the first tile's, which reach 1.  So the common
+// tile needs no maximum at all.
+//
+// Two streams (a softmax warp group and two issuing threads each) share the CTA so
 // that one stream's products run under the other's exponentials:
 //
 //   ROWS   the streams are two row tiles that share every key tile (long sequences: the bound is the exponentials and the
@@ -44,7 +48,7 @@
 namespace cmb {
 
 constexpr int WA_THREADS = 480;
-constexpr float WA_RESCALE = 8.f;        // log2 units a tile's maximum may exceed the reference before O is rescaled
+constexpr float WA_FAR = 1099511627776.f;   // 2^40: a tile's row sum above which the reference moves
 constexpr int WA_CTL = 3072;             // barriers (first 1 KB), (max, sum) of every row and stream (2 KB)
 
 struct WindowParams {
@@ -241,7 +245,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       uint8_t* ring = is_k ? ks : vs;
       uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
       int* pages = reinterpret_cast<int*>(ctl + (is_k ? 512 : 768));     // [2 batches][32 boxes]
-      const int per_tile = BN / p.box_k, batch = 32 / per_tile;     // boxes of a tile, tiles of a batch of lookups
+      const int box_log = __ffs(p.box_k) - 1, box_bytes = p.box_k * 128;     // (a power of two)
+      const int per_tile = BN >> box_log, batch = 32 / per_tile;    // boxes of a tile, tiles of a batch of lookups
       const bool paged = p.table != nullptr;
       auto look_up = [&](int i0) {           // the page of this lane's box, of the batch that begins at tile i0
         const int i = i0 + lane / per_tile;
@@ -279,17 +284,16 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (elect_one()) {             // (always the same thread)
           const int* page = pages + odd;
           for (int i = i0; i < t1 && i < i0 + batch && ok; ++i) {
-            const int boxes = (t.keys() + p.box_k - 1) / p.box_k;
-            const uint32_t bytes = static_cast<uint32_t>(boxes) * p.box_k * 128 * DB;
+            const int boxes = (t.keys() + p.box_k - 1) >> box_log;
             ok = wa_wait(&empty[kst], kph, abort_flag, status, ST_TIMEOUT_EMPTY);
             if (ok) {
-              mbar_arrive_expect_tx(&full[kst], bytes);
+              mbar_arrive_expect_tx(&full[kst], static_cast<uint32_t>(boxes * box_bytes) * DB);
               uint8_t* dst = ring + kst * Cfg::STAGE;
               for (int m = 0; m < boxes; ++m) {
                 const int outer = paged ? page[m] : b;
 #pragma unroll
                 for (int kb = 0; kb < DB; ++kb) tma_load_4d(dst + kb * Cfg::KBLK, map, &full[kst], kb * 64, row, hk, outer);
-                dst += p.box_k * 128;
+                dst += box_bytes;
                 row += p.box_k;
                 if (paged && row == p.page) row = 0;
               }
@@ -475,51 +479,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
           }
         }
-        float m8[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < CH; ++e) {
-          if (e < c_count && c_first + e < chunks) {
-#pragma unroll
-            for (int i2 = 0; i2 < CW; i2 += 16)
-#pragma unroll
-              for (int u = 0; u < 8; ++u)
-                m8[u] = fmaxf(fmaxf(m8[u], __uint_as_float(x[e][i2 + 2 * u])), __uint_as_float(x[e][i2 + 2 * u + 1]));
-          }
-        }
-        const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * p.scale_log2;
-        const bool moved = mx > m_ref + WA_RESCALE || (m_ref == -INFINITY && mx > -INFINITY);
-        if (__any_sync(0xffffffffu, moved)) {
-          float alpha = 1.f;
-          if (moved) {
-            alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
-            m_ref = mx;
-            l_sum *= alpha;
-          }
-          if (c > 0) {
-            // O is rescaled when the previous tile's product has completed
-            if (!wa_warp_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-#pragma unroll 1
-            for (int cc = 0; cc < DB * 2; ++cc) {
-              uint32_t o[32];
-              tmem_ld_x32(o_addr + cc * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st_x32(o_addr + cc * 32, o);
-            }
-          }
-        }
-        // a row without a key yet: exp2(-inf - 0) = 0
-        const float2 neg_m = m_ref == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m_ref, -m_ref);
         const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
-        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto probs = [&](int e) {
+        float2 acc[2];
+        auto probs = [&](int e, float2 neg_m) {
           // P of chunk ch is columns CW / 2 ch .. of the scores, all read by now (the row's lane is this thread's)
           if (e < c_count && c_first + e < chunks) {
             uint32_t w16[CW / 2];
@@ -535,11 +497,69 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             else tmem_st_x8(s_addr + (c_first + e) * 8, w16);
           }
         };
+        auto tile_sum = [&] {
+          // a row without a key yet: exp2(-inf - 0) = 0
+          const float2 neg_m = m_ref == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m_ref, -m_ref);
+          acc[0] = acc[1] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < CH; ++e) probs(e, neg_m);
+          return (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+        };
+        // P, with a reference that rises to the row's largest score so far
+        auto lift = [&] {
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < CH; ++e) {
+            if (e < c_count && c_first + e < chunks) {
+#pragma unroll
+              for (int i2 = 0; i2 < CW; ++i2) m4[i2 & 3] = fmaxf(m4[i2 & 3], __uint_as_float(x[e][i2]));
+            }
+          }
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+          float alpha = 1.f;
+          if (mx > m_ref) {
+            alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
+            m_ref = mx;
+            l_sum *= alpha;
+          }
+          if (c > 0) {
+            // O is rescaled when the previous tile's product has completed
+            if (!wa_warp_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
+            tc_fence_after();
+#pragma unroll 1
+            for (int cc = 0; cc < DB * 2; ++cc) {
+              uint32_t o[32];
+              tmem_ld_x32(o_addr + cc * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st_x32(o_addr + cc * 32, o);
+            }
+          }
+          return true;
+        };
+        const bool first_keys = __any_sync(0xffffffffu, w.ok && m_ref == -INFINITY);     // a row without a reference yet
+        float sum = 0.f;
+        if constexpr (KEYS) {                // few tiles: the first one counts
+          bool seek = first_keys;
+          for (int pass = 0;; ++pass) {
+            if (seek && !(ok = lift())) break;
+            sum = tile_sum();
+            seek = pass == 0 && __any_sync(0xffffffffu, w.ok && !(sum < WA_FAR));
+            if (!seek) break;
+          }
+        } else {                             // many: the loop without the maximum is straight
+          sum = tile_sum();
+          if (first_keys || __any_sync(0xffffffffu, w.ok && !(sum < WA_FAR))) {
+            ok = lift();
+            sum = tile_sum();
+          }
+        }
+        if (!ok) break;
+        l_sum += sum;
         const bool more = i + step < t1;
         for (int f = 0; f < step; ++f) t.next();
         const int chunks_n = (t.keys() + CW - 1) / CW;
-#pragma unroll
-        for (int e = 0; e < CH; ++e) probs(e);
         if (KEYS && p.copies > 1) {          // the other copies' chunks count nothing here
           const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
@@ -558,7 +578,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int e = 0; e < CH; ++e) load(e, chunks_n, c + 1);
         }
-        l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
         tmem_wait_ld();
         chunks = chunks_n;
       }
