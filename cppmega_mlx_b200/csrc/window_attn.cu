@@ -39,22 +39,20 @@
 // Rows of V that no row may see (past a sequence's end, padding, pages handed on to others) may hold anything, NaN included:
 // a helper warp zeroes them in shared memory before they are multiplied with P's zeros.
 //
-// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 and 14 TMA producers, 9 / 10 scores and 12 / 13 products of stream 0 / 1, 11 the V helper.  Every wait is
-// bounded (sm100.cuh).
+// Every wait is bounded (sm100.cuh).
 #include <cstring>
+#include <type_traits>
 
 #include "window_attn.h"
 
 namespace cmb {
 
-constexpr int WA_THREADS = 480;
 constexpr float WA_FAR = 1099511627776.f;   // 2^40: a tile's row sum above which the reference moves
-constexpr int WA_CTL = 3072;             // barriers (first 1 KB), (max, sum) of every row and stream (2 KB)
+constexpr int WA_CTL = 1024;             // barriers and looked-up pages
 
 struct WindowParams {
   int S, T, H, Hk, g;                    // queries, keys per sequence (cache capacity), heads
   int box_q;                             // queries in a row tile's TMA box
-  int copies, copy_rows;                 // KEYS: how often a tile holds its rows, and 128 / copies
   int Dv;
   float scale_log2;                      // softmax scale * log2(e)
   int window, ns;
@@ -74,23 +72,33 @@ struct WindowParams {
   int* status;
 };
 
-template <int DB, bool KEYS>
+// COPIES: 0 for ROWS, else KEYS with the rows so many times in a tile.
+template <int DB, int COPIES>
 struct WindowCfg {
+  static constexpr bool KEYS = COPIES > 0;
   static constexpr int BN = 64;                          // keys of a tile
   static constexpr int BUFS = 2;                         // score buffers of a stream
-  static constexpr int CW = KEYS ? 16 : 32;              // keys of the chunks that a softmax thread works in
+  static constexpr int COPY_ROWS = KEYS ? 128 / COPIES : 128;
+  static constexpr int TN = KEYS ? BN / COPIES : BN;     // keys of a tile that a softmax thread takes, in chunks of CW
+  static constexpr int CW = TN < 32 ? TN : 32, CH = TN / CW;
+  static constexpr int STREAMS = KEYS ? 1 : 2;           // of a CTA
+  static constexpr int SOFT = 128 * STREAMS;             // softmax threads
+  // warps: softmax, producer of keys, scores, products, producer of values, V helper (KEYS: the products' warp helps, so that
+  // there are 8 warps of 128 registers)
+  static constexpr int W_K = 4 * STREAMS, W_S = W_K + 1, W_P = W_S + STREAMS, W_V = W_P + STREAMS, W_HELP = W_V + 1;
+  static constexpr int THREADS = (KEYS ? W_HELP : W_HELP + 1) * 32;
+  static constexpr int CTAS = KEYS ? 2 : 1;              // of an SM
   static constexpr int KBLK = BN * 128;                  // bytes of a [BN keys x 64 columns] block
-  static constexpr int Q_BYTES = (KEYS ? 1 : 2) * DB * WA_BLK;
-  static constexpr int NK = DB == 2 ? (KEYS ? 6 : 5) : (KEYS ? 10 : 8);
-  static constexpr int NV = NK;
+  static constexpr int Q_BYTES = STREAMS * DB * WA_BLK;
+  static constexpr int NK = DB == 2 ? (KEYS ? 3 : 5) : (KEYS ? 6 : 8);
+  static constexpr int NV = DB == 2 && KEYS ? 2 : NK;
   static constexpr int STAGE = DB * KBLK;
   static constexpr int SMEM_BYTES = Q_BYTES + (NK + NV) * STAGE + WA_CTL;
   static constexpr int PART_PITCH = DB * 64 + 4;         // floats; rows 16 bytes apart in banks
-  static_assert(NK == NV && NK % 2 == 0 || !KEYS, "KEYS: a stream's stages keep their parity");
-  static_assert(SMEM_BYTES <= 232448 && (13 + 2 * NK + 3 * NV) * 8 + 8 <= 512, "shared memory");
-  static_assert(!KEYS || 256 * PART_PITCH * 4 <= (NK + NV) * STAGE, "partial results reuse the rings");
-  // TMEM: stream s has O at 128 s and its score buffers at 256 + 128 s and 64 columns on; P is written over the scores
-  static constexpr int O_STEP = 128, S_COL = 256, S_STEP = 128;
+  static_assert((SMEM_BYTES + 1024) * CTAS <= 233472 && (13 + 2 * NK + 3 * NV) * 8 + 8 <= 512, "shared memory");
+  static_assert(!KEYS || 128 * PART_PITCH * 4 <= (NK + NV) * STAGE, "partial results reuse the rings");
+  // TMEM: the streams' O, then their score buffers; P is written over the scores
+  static constexpr int O_STEP = 128, S_COL = STREAMS * 128, S_STEP = 128, TMEM_COLS = STREAMS * 256;
 };
 
 // One row's place in the problem.
@@ -141,11 +149,12 @@ __device__ __forceinline__ unsigned window_word(const WindowParams& p, const Win
   return w.ok ? bits : 0u;
 }
 
-template <int DB, bool KEYS>
-__global__ void __launch_bounds__(WA_THREADS, 1)
+template <int DB, int COPIES>
+__global__ void __launch_bounds__(WindowCfg<DB, COPIES>::THREADS, WindowCfg<DB, COPIES>::CTAS)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const WindowParams p) {
-  using Cfg = WindowCfg<DB, KEYS>;
+  using Cfg = WindowCfg<DB, COPIES>;
+  constexpr bool KEYS = Cfg::KEYS;
   constexpr int NK = Cfg::NK, NV = Cfg::NV, BN = Cfg::BN, BUFS = Cfg::BUFS;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {   // swizzled TMA / MMA tiles need 1024-byte aligned buffers
@@ -167,7 +176,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* pv_done = p_full + 4;          // [stream][buffer] P read, O added to
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float2* xml = reinterpret_cast<float2*>(ctl + 1024);   // [2 streams][128 rows] (max, sum)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z / p.splits, split = blockIdx.z - b * p.splits;
@@ -176,10 +184,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   int* status = p.status;
 
   // rows and keys of this CTA
-  const int rows_q = (KEYS ? 1 : 2) * p.box_q;                     // queries of the CTA
+  const int rows_q = Cfg::STREAMS * p.box_q;                     // queries of the CTA
   const int s_first = xt * rows_q;
   const int s_last = min(p.S, s_first + rows_q) - 1;
-  const bool two = KEYS || s_first + p.box_q < p.S;                // is there a second row tile?
+  const bool two = !KEYS && s_first + p.box_q < p.S;               // is there a second row tile?
   int prefix = 0, klim, pmin, pmax;
   if (p.cached) {
     prefix = max(0, min(p.lengths[b], p.T - p.S));                 // out-of-range prefixes are reported below
@@ -197,7 +205,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int NT = t1 - t0;
 
   if (threadIdx.x == 0) {
-    const uint32_t readers = !KEYS && two ? 2 : 1;     // MMA warps that read each tile
+    const uint32_t readers = two ? 2 : 1;     // MMA warps that read each tile
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -226,21 +234,21 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     }
   }
-  if (warp == 8) {
-    tmem_alloc(tmem_slot, 512);
+  if (warp == Cfg::W_K) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  if (warp >= 8) {
-  if (warp == 8 || warp == 14) {
+  if (warp >= Cfg::W_K) {
+  if (warp == Cfg::W_K || warp == Cfg::W_V) {
     // ---------------------------------------------------------------- TMA producers of keys (and queries) and of values: one thread
     // of the warp issues (copies issued lane by lane cost 500 clocks each, and one thread for both was the bound of short
     // windows), all look up pages, 32 boxes at a time and a batch ahead
     if (NT > 0) {
-      const bool is_k = warp == 8;
+      const bool is_k = warp == Cfg::W_K;
       const CUtensorMap* map = is_k ? &tmK : &tmV;
       uint8_t* ring = is_k ? ks : vs;
       uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
@@ -257,15 +265,16 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       };
       int next = look_up(t0);
       if (is_k && elect_one()) {
-        const int nq = KEYS ? p.copies : (two ? 2 : 1);
+        const int nq = KEYS ? COPIES : (two ? 2 : 1);
         mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.box_q * p.g * 128) * nq * DB);
         for (int t = 0; t < nq; ++t)
           for (int kb = 0; kb < DB; ++kb)
-            tma_load_5d(KEYS ? qs + kb * WA_BLK + t * p.copy_rows * 128 : qs + (t * DB + kb) * WA_BLK, &tmQ, q_full, kb * 64, 0,
+            tma_load_5d(KEYS ? qs + kb * WA_BLK + t * Cfg::COPY_ROWS * 128 : qs + (t * DB + kb) * WA_BLK, &tmQ, q_full, kb * 64, 0,
                         KEYS ? s_first : s_first + t * p.box_q, hk, b);
       }
       WaTile<BN> t(R, t0);
-      int kst = 0, kph = 1, row = paged ? t.k0 % p.page : t.k0;     // stage (keys and values run through as many), its phase, row in the page
+      const int stages = is_k ? NK : NV;
+      int kst = 0, kph = 1, row = paged ? t.k0 % p.page : t.k0;     // stage, its phase, row in the page
       for (int i0 = t0, odd = 0; i0 < t1; i0 += batch, odd ^= 32) {
         if (paged) {
           if (next < 0 || next >= p.num_pages) {     // reported, and read as page 0: the copies stay inside the pool
@@ -298,7 +307,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (paged && row == p.page) row = 0;
               }
             }
-            if (++kst == NK) {
+            if (++kst == stages) {
               kst = 0;
               kph ^= 1;
             }
@@ -310,18 +319,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!__all_sync(0xffffffffu, ok)) break;
       }
     }
-  } else if (warp == 11) {
-    // ---------------------------------------------------------------- V helper: rows that nobody sees become zeros
+  } else {
+    // rows of V that nobody sees become zeros
     unsigned long long nodes_any = ~0ull;
-    if (p.tree != nullptr) {       // which drafted places hold a node
+    if (p.tree != nullptr && warp >= Cfg::W_P) {       // which drafted places hold a node
       nodes_any = 0ull;
       const unsigned long long* tree = p.tree + static_cast<long long>(b) * p.tree_sb;
       for (int m = 0; m < p.S; ++m) nodes_any |= tree[m];
     }
-    WaTile<BN> t(R, t0);
-    int st = 0, ph = 0;
-    for (int i = t0; i < t1; ++i) {
-      if (!wa_warp_wait(&v_full[st], ph, abort_flag, status, ST_TIMEOUT_FULL)) break;
+    auto zero_unseen = [&](const WaTile<BN>& t, int st) {
       const int k1 = t.k1();
       const bool tail = k1 - t.k0 < BN, head = t.in_window() && t.k0 < R.wtrue;
       const bool drafted = p.tree != nullptr && k1 > prefix;
@@ -340,81 +346,101 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         fence_proxy_async_smem();
       }
-      wa_warp_arrive(&v_ready[st]);
-      t.next();
-      if (++st == NV) {
-        st = 0;
-        ph ^= 1;
+    };
+    if (warp == Cfg::W_HELP) {
+      // -------------------------------------------------------------- V helper
+      WaTile<BN> t(R, t0);
+      int st = 0, ph = 0;
+      for (int i = t0; i < t1; ++i) {
+        if (!wa_warp_wait(&v_full[st], ph, abort_flag, status, ST_TIMEOUT_FULL)) break;
+        zero_unseen(t, st);
+        wa_warp_arrive(&v_ready[st]);
+        t.next();
+        if (++st == NV) {
+          st = 0;
+          ph ^= 1;
+        }
       }
-    }
-  } else {
-    // ---------------------------------------------------------------- MMA issuers: a thread each for the scores (warps 9, 10)
-    // and the products (12, 13) of each stream.  One thread for both would hold a finished P back behind the scores of two tiles
-    // later: an issuing thread advances no faster than the tensor pipe takes its instructions.
-    const bool scores = warp < 11;
-    const int st = scores ? warp - 9 : warp - 12;
-    if ((st == 0 || two) && elect_one()) {
-      // one descriptor each, advanced by adding to its address field (16-byte units)
-      const uint32_t s_col = tmem_base + Cfg::S_COL + st * Cfg::S_STEP, o_col = tmem_base + Cfg::O_STEP * st;
-      const int first = t0 + (KEYS ? st : 0), step = KEYS ? 2 : 1;
-      int c = 0;                                       // tiles of this stream so far
-      WaTile<BN> t(R, first);
-      int stage = KEYS ? st : 0, phase = 0;
-      auto walk = [&] {
-        for (int f = 0; f < step; ++f) t.next();
-        stage += step;
-        if (stage >= NK) {
-          stage -= NK;
-          phase ^= 1;
-        }
-      };
-      if (scores) {
-        const uint64_t q_desc = make_smem_desc_sw128(smem_u32(qs) + (KEYS ? 0 : st * DB * WA_BLK), 16, 1024);
-        const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ks), 16, 1024);
-        bool ok = first >= t1 || wa_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
-        for (int i = first; i < t1 && ok; i += step, ++c) {
-          const int buf = c & 1;
-          const uint32_t idesc_s = make_idesc(128, (t.keys() + 15) & ~15, 1, 1, 0, 0);
-          const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
-          const uint32_t d = s_col + buf * 64;
-          // the scores take the place of an earlier tile's P, once the product has read it
-          if (c >= 2 && !wa_wait(&pv_done[st * 2 + buf], ((c >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
-          if (!wa_wait(&k_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kb = 0; kb < DB; ++kb)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16(d, q_desc + ((kb * WA_BLK + k * 32) >> 4), kd + ((kb * Cfg::KBLK + k * 32) >> 4), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&k_empty[stage]);
-          umma_commit(&s_full[st * 2 + buf]);
-          walk();
-        }
-      } else {
-        constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
-        const uint64_t v_desc = make_smem_desc_sw128(smem_u32(vs), Cfg::KBLK, 1024);
-        for (int i = first; i < t1; i += step, ++c) {
-          const int buf = c & 1;
-          const int k16 = (t.keys() + 15) >> 4;
-          const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
-          const uint32_t a = s_col + buf * 64;
-          if (!wa_wait(&v_ready[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
-          if (!wa_wait(&p_full[st * 2 + buf], (c >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
-          tc_fence_after();
-          umma_f16_ts(o_col, a, vd, idesc_o, c > 0 ? 1u : 0u);
-          if (k16 == BN / 16) {
-#pragma unroll
-            for (int k = 1; k < BN / 16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
-          } else {
-            for (int k = 1; k < k16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
+    } else {
+      // ---------------------------------------------------------------- MMA issuers: a thread each for the scores (W_S)
+      // and the products (W_P) of each stream.  One thread for both would hold a finished P back behind the scores of two tiles
+      // later: an issuing thread advances no faster than the tensor pipe takes its instructions.
+      const bool scores = warp < Cfg::W_P;
+      const int st = scores ? warp - Cfg::W_S : warp - Cfg::W_P;
+      if (st == 0 || two) {
+        // one descriptor each, advanced by adding to its address field (16-byte units)
+        const uint32_t s_col = tmem_base + Cfg::S_COL + st * Cfg::S_STEP, o_col = tmem_base + Cfg::O_STEP * st;
+        int c = 0;                                       // tiles so far
+        WaTile<BN> t(R, t0);
+        const int stages = scores ? NK : NV;
+        int stage = 0, phase = 0;
+        auto walk = [&] {
+          t.next();
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
           }
-          umma_commit(&v_empty[stage]);
-          umma_commit(&pv_done[st * 2 + buf]);
-          walk();
+        };
+        if (scores && elect_one()) {
+          const uint64_t q_desc = make_smem_desc_sw128(smem_u32(qs) + st * DB * WA_BLK, 16, 1024);
+          const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ks), 16, 1024);
+          bool ok = t0 >= t1 || wa_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
+          for (int i = t0; i < t1 && ok; ++i, ++c) {
+            const int buf = c & 1;
+            const uint32_t idesc_s = make_idesc(128, (t.keys() + 15) & ~15, 1, 1, 0, 0);
+            const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
+            const uint32_t d = s_col + buf * 64;
+            // the scores take the place of an earlier tile's P, once the product has read it
+            if (c >= 2 && !wa_wait(&pv_done[st * 2 + buf], ((c >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
+            if (!wa_wait(&k_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kb = 0; kb < DB; ++kb)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16(d, q_desc + ((kb * WA_BLK + k * 32) >> 4), kd + ((kb * Cfg::KBLK + k * 32) >> 4), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
+            umma_commit(&k_empty[stage]);
+            umma_commit(&s_full[st * 2 + buf]);
+            walk();
+          }
+        } else if (!scores && (KEYS || elect_one())) {
+          constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
+          const uint64_t v_desc = make_smem_desc_sw128(smem_u32(vs), Cfg::KBLK, 1024);
+          for (int i = t0; i < t1; ++i, ++c) {
+            const int buf = c & 1;
+            const int k16 = (t.keys() + 15) >> 4;
+            const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
+            const uint32_t a = s_col + buf * 64;
+            if constexpr (KEYS) {              // all of the warp
+              if (!wa_warp_wait(&v_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
+              zero_unseen(t, stage);
+              __syncwarp();
+            } else {
+              if (!wa_wait(&v_ready[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
+            }
+            bool ok = true;
+            if (!KEYS || elect_one()) {
+              ok = wa_wait(&p_full[st * 2 + buf], (c >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+              if (ok) {
+                tc_fence_after();
+                umma_f16_ts(o_col, a, vd, idesc_o, c > 0 ? 1u : 0u);
+                if (k16 == BN / 16) {
+#pragma unroll
+                  for (int k = 1; k < BN / 16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
+                } else {
+                  for (int k = 1; k < k16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
+                }
+                umma_commit(&v_empty[stage]);
+                umma_commit(&pv_done[st * 2 + buf]);
+              }
+            }
+            if (KEYS ? !__all_sync(0xffffffffu, ok) : !ok) break;
+            walk();
+          }
         }
       }
     }
-  }
+    }
   } else {
     // ---------------------------------------------------------------- softmax and epilogue (a warp group per stream)
     const int st = warp >> 2, quarter = warp & 3;
@@ -422,11 +448,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_base = tmem_base + lane_addr + Cfg::S_COL + st * Cfg::S_STEP, o_addr = tmem_base + lane_addr + Cfg::O_STEP * st;
     const bool active = st == 0 || two;
-    const int copy = KEYS ? row / p.copy_rows : 0;
-    const int rr = KEYS ? row - copy * p.copy_rows : row;          // row within the tile
-    const WindowRow w = window_row(p, rr, KEYS ? s_first : s_first + st * p.box_q, hk, b, klim, prefix);
-    constexpr int CW = Cfg::CW, CH = BN / CW;
-    const int c_count = KEYS ? CH / p.copies : CH, c_first = KEYS ? copy * c_count : 0;      // this thread's chunks of a tile
+    const int copy = row / Cfg::COPY_ROWS;
+    const int rr = row - copy * Cfg::COPY_ROWS;         // row within the tile
+    const WindowRow w = window_row(p, rr, s_first + st * p.box_q, hk, b, klim, prefix);
+    constexpr int CW = Cfg::CW, CH = Cfg::CH;
+    const int first_key = copy * Cfg::TN;    // of a tile's keys, this thread's TN begin here
     const bool warp_ok = __any_sync(0xffffffffu, w.ok);
     // what every row of the warp sees (rows that are not ok are never read): most tiles need no mask
     const int all_upto = __reduce_min_sync(0xffffffffu, w.ok ? w.plim : 0x7fffffff);
@@ -435,36 +461,36 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool ok = active;
     int c = 0;
     if (active) {
-      const int first = t0 + (KEYS ? st : 0), step = KEYS ? 2 : 1;
       auto scores_in = [&](int at) {         // tile `at` of this stream: are its scores there?
         return wa_warp_wait(&s_full[st * 2 + at % BUFS], (at / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       };
       uint32_t x[CH][CW];                    // the scores of this thread's chunks
-      auto load = [&](int e, int chunks, int at) {
-        if (e < c_count && c_first + e < chunks) {
-          const uint32_t a = s_base + (at % BUFS) * 64 + (c_first + e) * CW;
+      // (a short tile's last columns hold anything and are masked; wide: more keys than the first chunk's)
+      auto load = [&](int at, bool wide) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+          if (e > 0 && !wide) continue;
+          const uint32_t a = s_base + (at % BUFS) * 64 + first_key + e * CW;
           if constexpr (CW == 32) tmem_ld_x32(a, x[e]);
           else tmem_ld_x16(a, x[e]);
         }
       };
-      for (int i = first; i < t1 && !warp_ok; i += step, ++c) {    // no rows: this warp only keeps step
+      for (int i = t0; i < t1 && !warp_ok; ++i, ++c) {    // no rows: this warp only keeps step
         if (!scores_in(c)) {
           ok = false;
           break;
         }
         wa_warp_arrive(&p_full[st * 2 + c % BUFS]);
       }
-      WaTile<BN> t(R, first);
-      int chunks = (t.keys() + CW - 1) / CW; // chunks that the tile has
-      if (warp_ok && first < t1) {
+      WaTile<BN> t(R, t0);
+      bool wide = CH == 1 || t.keys() > CW;
+      if (warp_ok && t0 < t1) {
         ok = scores_in(0);
         tc_fence_after();
-#pragma unroll
-        for (int e = 0; e < CH; ++e)
-          if (ok) load(e, chunks, 0);
+        if (ok) load(0, wide);
         tmem_wait_ld();
       }
-      for (int i = first; i < t1 && warp_ok && ok; i += step, ++c) {
+      for (int i = t0; i < t1 && warp_ok && ok; ++i, ++c) {
         const int buf = c % BUFS;
         const uint32_t s_addr = s_base + buf * 64;
         const int k1 = t.k1();
@@ -472,49 +498,44 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!whole) {                        // what is masked may be NaN: selected, not added to
 #pragma unroll
           for (int e = 0; e < CH; ++e) {
-            if (e < c_count && c_first + e < chunks) {
-              const unsigned word = window_word(p, w, t.k0 + (c_first + e) * CW, k1, prefix);
+            const unsigned word = window_word(p, w, t.k0 + first_key + e * CW, k1, prefix);
 #pragma unroll
-              for (int i2 = 0; i2 < CW; ++i2) x[e][i2] = (word >> i2) & 1u ? x[e][i2] : 0xff800000u;
-            }
+            for (int i2 = 0; i2 < CW; ++i2) x[e][i2] = (word >> i2) & 1u ? x[e][i2] : 0xff800000u;
           }
         }
         const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
         float2 acc[2];
         auto probs = [&](int e, float2 neg_m) {
-          // P of chunk ch is columns CW / 2 ch .. of the scores, all read by now (the row's lane is this thread's)
-          if (e < c_count && c_first + e < chunks) {
-            uint32_t w16[CW / 2];
+          // P of a chunk takes half its scores' columns, all read by now (the row's lane is this thread's)
+          uint32_t w16[CW / 2];
 #pragma unroll
-            for (int i2 = 0; i2 < CW / 2; ++i2) {
-              float2 v = fma2(make_float2(__uint_as_float(x[e][2 * i2]), __uint_as_float(x[e][2 * i2 + 1])), c2, neg_m);
-              v.x = exp2f(v.x);
-              v.y = exp2f(v.y);
-              acc[i2 & 1] = add2(acc[i2 & 1], v);
-              w16[i2] = pack_bf16x2(v.x, v.y);
-            }
-            if constexpr (CW == 32) tmem_st_x16(s_addr + (c_first + e) * 16, w16);
-            else tmem_st_x8(s_addr + (c_first + e) * 8, w16);
+          for (int i2 = 0; i2 < CW / 2; ++i2) {
+            float2 v = fma2(make_float2(__uint_as_float(x[e][2 * i2]), __uint_as_float(x[e][2 * i2 + 1])), c2, neg_m);
+            v.x = exp2f(v.x);
+            v.y = exp2f(v.y);
+            acc[i2 & 1] = add2(acc[i2 & 1], v);
+            w16[i2] = pack_bf16x2(v.x, v.y);
           }
+          const uint32_t a = s_addr + (first_key + e * CW) / 2;
+          if constexpr (CW == 32) tmem_st_x16(a, w16);
+          else tmem_st_x8(a, w16);
         };
         auto tile_sum = [&] {
           // a row without a key yet: exp2(-inf - 0) = 0
           const float2 neg_m = m_ref == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m_ref, -m_ref);
           acc[0] = acc[1] = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int e = 0; e < CH; ++e) probs(e, neg_m);
+          for (int e = 0; e < CH; ++e)
+            if (e == 0 || wide) probs(e, neg_m);
           return (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
         };
         // P, with a reference that rises to the row's largest score so far
         auto lift = [&] {
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < CH; ++e) {
-            if (e < c_count && c_first + e < chunks) {
+          for (int e = 0; e < CH; ++e)
 #pragma unroll
-              for (int i2 = 0; i2 < CW; ++i2) m4[i2 & 3] = fmaxf(m4[i2 & 3], __uint_as_float(x[e][i2]));
-            }
-          }
+            for (int i2 = 0; i2 < CW && (e == 0 || wide); ++i2) m4[i2 & 3] = fmaxf(m4[i2 & 3], __uint_as_float(x[e][i2]));
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
           float alpha = 1.f;
           if (mx > m_ref) {
@@ -557,14 +578,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         if (!ok) break;
         l_sum += sum;
-        const bool more = i + step < t1;
-        for (int f = 0; f < step; ++f) t.next();
-        const int chunks_n = (t.keys() + CW - 1) / CW;
-        if (KEYS && p.copies > 1) {          // the other copies' chunks count nothing here
+        const bool more = i + 1 < t1;
+        t.next();
+        const bool wide_n = CH == 1 || t.keys() > CW;
+        if constexpr (COPIES > 1) {          // the other copies' keys count nothing here
           const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
-          for (int ch = 0; ch < CH; ++ch)
-            if (ch < chunks && (ch < c_first || ch >= c_first + c_count)) tmem_st_x8(s_addr + ch * 8, z);
+          for (int ch = 0; ch < 4; ++ch)
+            if (ch * 16 / Cfg::TN != copy) tmem_st_x8(s_addr + ch * 8, z);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -575,11 +596,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             break;
           }
           tc_fence_after();
-#pragma unroll
-          for (int e = 0; e < CH; ++e) load(e, chunks_n, c + 1);
+          load(c + 1, wide_n);
         }
         tmem_wait_ld();
-        chunks = chunks_n;
+        wide = wide_n;
       }
       // (the product before the last completes before it: one thread issued both)
       if (c > 0 && ok)
@@ -587,8 +607,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_after();
     }
     const float LN2 = 0.6931471805599453f;
-    if (!KEYS) {
-      // -------------------------------------------------------------- ROWS: a thread writes its row
+    if constexpr (COPIES <= 1) {
+      // -------------------------------------------------------------- a thread writes its row
       if (active && ok) {
         float inv = 0.f;
         const bool in = rr / p.g < p.box_q && w.s < p.S;       // a padding node's row is written too (zeros)
@@ -643,16 +663,17 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     } else {
-      // -------------------------------------------------------------- KEYS: join the streams and copies, then write
+      // -------------------------------------------------------------- join the copies, then write
       // The rings are free: both streams' last products have completed, and they read every tile that was fetched.
       float* part = reinterpret_cast<float*>(ks);
+      float2* xml = reinterpret_cast<float2*>(qs);           // (reference, sum) of every row: the queries have been read
       if (c == 0) m_ref = -INFINITY;
-      xml[st * 128 + row] = make_float2(w.ok ? m_ref : -INFINITY, l_sum);
-      if (named_bar_and(1, 256, ok)) {
+      xml[row] = make_float2(w.ok ? m_ref : -INFINITY, l_sum);
+      if (named_bar_and(1, Cfg::SOFT, ok)) {
         float top = -INFINITY;
-        for (int q = 0; q < 2 * p.copies; ++q) top = fmaxf(top, xml[(q & 1) * 128 + (q >> 1) * p.copy_rows + rr].x);
+        for (int q = 0; q < COPIES; ++q) top = fmaxf(top, xml[q * Cfg::COPY_ROWS + rr].x);
         const float wt = w.ok && m_ref > -INFINITY ? exp2f(m_ref - top) : (l_sum == l_sum ? 0.f : l_sum);
-        float* mine = part + (st * 128 + row) * Cfg::PART_PITCH;
+        float* mine = part + row * Cfg::PART_PITCH;
 #pragma unroll
         for (int cc = 0; cc < DB * 2; ++cc) {
           uint32_t o[32];
@@ -671,15 +692,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         }
       }
-      if (named_bar_and(1, 256, ok)) {
+      if (named_bar_and(1, Cfg::SOFT, ok)) {
         const int vec = p.Dv / 8;                                  // 16-byte output pieces of a row
         const int rows = min(p.box_q, p.S - s_first) * p.g;
-        for (int it = threadIdx.x; it < rows * vec; it += 256) {
+        for (int it = threadIdx.x; it < rows * vec; it += Cfg::SOFT) {
           const int r = it / vec, col = (it - r * vec) * 8;
           float top = -INFINITY, l = 0.f, f8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          for (int q = 0; q < 2 * p.copies; ++q) top = fmaxf(top, xml[(q & 1) * 128 + (q >> 1) * p.copy_rows + r].x);
-          for (int q = 0; q < 2 * p.copies; ++q) {
-            const int pr = (q & 1) * 128 + (q >> 1) * p.copy_rows + r;
+          for (int q = 0; q < COPIES; ++q) top = fmaxf(top, xml[q * Cfg::COPY_ROWS + r].x);
+          for (int q = 0; q < COPIES; ++q) {
+            const int pr = q * Cfg::COPY_ROWS + r;
             const float2 ml = xml[pr];
             l += ml.x > -INFINITY ? ml.y * exp2f(ml.x - top) : (ml.y == ml.y ? 0.f : ml.y);
             const float4 a = *reinterpret_cast<const float4*>(part + pr * Cfg::PART_PITCH + col);
@@ -725,13 +746,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == Cfg::W_K) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
   }
 }
 
-// Joins the splits of a row: a warp per (sequence, query, head), four output columns per lane.
+// Joins the splits of a row (sequence, query, head), four output columns per lane: a warp, or with more than 8 splits a block of
+// four warps that share them (61 nodes, 16 heads, 37 splits: 13.8 us with a warp each).
 struct CombineParams {
   int S, H, splits, Dv;
   long long rows;
@@ -742,8 +764,11 @@ struct CombineParams {
   long long o_sb, o_ss, o_sh;
   float* lse;
 };
+template <bool SHARED>
 __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams p) {
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  __shared__ float4 parts[3][32];
+  const int warp = threadIdx.x >> 5;
+  const long long row = SHARED ? blockIdx.x : static_cast<long long>(blockIdx.x) * 4 + warp;
   if (row >= p.rows) return;
   const int lane = threadIdx.x & 31;
   const int h = static_cast<int>(row % p.H);
@@ -761,7 +786,7 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool in = lane * 4 < p.Dv;
   const float* src = p.ws_o + row * p.splits * p.Dv + lane * 4;
-  for (int i0 = 0; i0 < p.splits; i0 += 8) {
+  for (int i0 = SHARED ? 8 * warp : 0; i0 < p.splits; i0 += SHARED ? 32 : 8) {
     float4 a[8];
     float w[8];
 #pragma unroll
@@ -777,6 +802,16 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams
       o.y = fmaf(a[i].y, w[i], o.y);
       o.z = fmaf(a[i].z, w[i], o.z);
       o.w = fmaf(a[i].w, w[i], o.w);
+    }
+  }
+  if constexpr (SHARED) {
+    if (warp > 0) parts[warp - 1][lane] = o;
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const float4 a = parts[i][lane];
+      o.x += a.x; o.y += a.y; o.z += a.z; o.w += a.w;
     }
   }
   float f = 1.f;
@@ -843,16 +878,16 @@ int make_tmap_grouped(CUtensorMap* out, const void* base, int D, int S, int Hk, 
 
 namespace {
 
-template <int DB, bool KEYS>
+template <int DB, int COPIES>
 int launch_window_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const cmb::WindowParams& p, int B,
                       cudaStream_t stream) {
-  using Cfg = cmb::WindowCfg<DB, KEYS>;
-  auto kern = cmb::window_fwd_kernel<DB, KEYS>;
+  using Cfg = cmb::WindowCfg<DB, COPIES>;
+  auto kern = cmb::window_fwd_kernel<DB, COPIES>;
   static std::atomic<unsigned long long> attr_done{0};
   if (cmb_host::set_smem_limit_once_per_device(attr_done, reinterpret_cast<const void*>(kern), Cfg::SMEM_BYTES)) return 103;
-  const int per = (KEYS ? 1 : 2) * p.box_q;
+  const int per = Cfg::STREAMS * p.box_q;
   dim3 grid((p.S + per - 1) / per, p.Hk, B * p.splits);
-  kern<<<grid, cmb::WA_THREADS, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, p);
+  kern<<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? 0 : 104;
 }
 
@@ -898,14 +933,13 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
   const bool keys = rows <= 128;
   if (p.splits > 1 && (at->ws_o == nullptr || at->ws_ml == nullptr)) return 1;
   if ((a.o_sb | a.o_ss | a.o_sh) & 7 || (reinterpret_cast<uintptr_t>(at->out) & 15)) return 1;
-  p.copies = 1;
+  int copies = 0;
   if (keys) {
     p.box_q = p.S;
-    p.copies = rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
+    copies = rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
   } else {
     p.box_q = 128 / p.g < p.S ? 128 / p.g : p.S;
   }
-  p.copy_rows = 128 / p.copies;
   p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
   p.out = static_cast<__nv_bfloat16*>(at->out); p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
   p.lse = static_cast<float*>(at->lse);
@@ -921,16 +955,26 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
   if (rc) return rc + 20000;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = Dq > 64 || p.Dv > 64;
-  if (wide) rc = keys ? launch_window_fwd<2, true>(tq, tk, tv, p, B, st) : launch_window_fwd<2, false>(tq, tk, tv, p, B, st);
-  else rc = keys ? launch_window_fwd<1, true>(tq, tk, tv, p, B, st) : launch_window_fwd<1, false>(tq, tk, tv, p, B, st);
+  auto launch = [&](auto db) {
+    constexpr int DB = decltype(db)::value;
+    switch (copies) {
+      case 0: return launch_window_fwd<DB, 0>(tq, tk, tv, p, B, st);
+      case 1: return launch_window_fwd<DB, 1>(tq, tk, tv, p, B, st);
+      case 2: return launch_window_fwd<DB, 2>(tq, tk, tv, p, B, st);
+      default: return launch_window_fwd<DB, 4>(tq, tk, tv, p, B, st);
+    }
+  };
+  rc = wide ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 1>{});
   if (rc || p.splits == 1) return rc;
   cmb::CombineParams c{};
   c.S = p.S; c.H = p.H; c.splits = p.splits; c.Dv = p.Dv;
   c.rows = static_cast<long long>(B) * p.S * p.H;
   c.ws_o = p.ws_o; c.ws_ml = p.ws_ml; c.sinks = p.sinks;
   c.out = p.out; c.o_sb = p.o_sb; c.o_ss = p.o_ss; c.o_sh = p.o_sh; c.lse = p.lse;
-  const long long blocks = (c.rows + 3) / 4;
+  const bool shared = p.splits > 8;
+  const long long blocks = shared ? c.rows : (c.rows + 3) / 4;
   if (blocks > 0x7fffffffll) return 1;
-  cmb::window_combine_kernel<<<static_cast<unsigned>(blocks), 128, 0, st>>>(c);
+  if (shared) cmb::window_combine_kernel<true><<<static_cast<unsigned>(blocks), 128, 0, st>>>(c);
+  else cmb::window_combine_kernel<false><<<static_cast<unsigned>(blocks), 128, 0, st>>>(c);
   return cudaGetLastError() == cudaSuccess ? 0 : 104;
 }

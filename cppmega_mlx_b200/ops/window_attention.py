@@ -149,10 +149,10 @@ def _sizes_covered(q, k, v) -> bool:
             and dv <= MAX_HEAD_DIM and q.shape[2] // k.shape[2] <= MAX_GROUP and k.shape[2] <= 65535 and q.shape[0] <= 65535)
 
 
-def choose_splits(ctas: int, tiles: int) -> int:
+def choose_splits(ctas: int, tiles: int, small: bool) -> int:
     """How many ways to split the key axis of ``ctas`` thread blocks whose rows see about ``tiles`` 64-key tiles: enough blocks for
-    every SM, two tiles (one per stream of the kernel) or more to a block."""
-    return max(1, min(NUM_SMS // max(1, ctas), (tiles + 1) // 2, 64))
+    every SM (two on an SM where a block is ``small``: up to 128 rows), a tile or more to a block."""
+    return max(1, min((2 if small else 1) * NUM_SMS // max(1, ctas), tiles if small else (tiles + 1) // 2, 64))
 
 
 def row_blocks(s: int, g: int) -> int:
@@ -234,7 +234,7 @@ def plan_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page: i
     blocks = row_blocks(s, g)
     span = s if tree is not None or blocks == 1 else 2 * (128 // g)
     reach = min(t if max_keys is None else min(t, max_keys), w + span)
-    splits = choose_splits(b * hk * blocks, -(-reach // 64) + -(-min(sink_tokens, t) // 64))
+    splits = choose_splits(b * hk * blocks, -(-reach // 64) + -(-min(sink_tokens, t) // 64), s * g <= 128)
     if b * splits > 65535:
         splits = 1
     box_k = 64 if table is None else min(64, page & -page)     # key rows of one copy; a tile is 64 keys
