@@ -8,7 +8,7 @@
 // Row i stands at position P_i and sees key j when j <= P_i, j is a valid key, and P_i - j < window or j < ns; drafted node n
 // stands at prefix + (number of its ancestors) and sees of the other nodes only those in its 64-bit word.
 //
-// Work of a CTA: 128-row tiles (window_attn.h: g heads x 128 / g queries) against tiles of 64 or 128 keys.
+// Work of a CTA: a 128-row tile (window_attn.h: g heads x 128 / g queries) against tiles of 64 keys.
 //
 //   S = Q.K^T       tcgen05.mma 128 x n x 16, fp32 in TMEM (n = the tile's keys, rounded up to 16: the few first tokens and the
 //                   last tile cost what they hold)
@@ -22,22 +22,20 @@
 // TMEM) when a tile's sum comes out above 2^40; terms 2^126 below m are nothing beside the first tile's, which reach 1.  So the common
 // tile needs no maximum at all.
 //
-// Two streams (a softmax warp group and two issuing threads each) share the CTA so
-// that one stream's products run under the other's exponentials:
+// Two CTAs share an SM (8 warps, half the TMEM and 113 KB of shared memory each): one's products run under the other's
+// exponentials, and its start and end under the other's tiles.  Against one CTA an SM with two row tiles that shared the key tiles,
+// this fetches every key tile twice from L2 and still gains where the tiles are many (2 x 4096 queries, 16 heads over 4 of 128, a window of 1024: 104 -> 94 us),
+// and more where they are few (128 single tokens over a window of 1024: 50 -> 37 us).  Tiles of 64 keys leave room for two score
+// buffers, so that the next scores run under this tile's exponentials: with one buffer of 128 every tile waited for its product and
+// the next scores, 2000 of 5200 clocks.
 //
-//   ROWS   the streams are two row tiles that share every key tile (long sequences: the bound is the exponentials and the
-//          tensor pipe, so key tiles should be fetched once for as many rows as fit).  Tiles of 64 keys, so that a stream has two
-//          score buffers and the next scores run under this tile's exponentials: with one buffer of 128 (P lies over S, and O and
-//          S of two streams fill the TMEM) every tile waited for its product and the next scores, 2000 of 5200 clocks.
-//   KEYS   the streams are the even and odd key tiles of one row tile, joined at the end (<= 128 rows: decode, small trees; the
-//          bound is reading the cache, so the shared memory goes to tiles in flight).  With <= 32 (64) rows the tile holds
-//          them four (two) times in its TMEM lane quarters and each copy takes a quarter (half) of a tile's keys, because a
-//          warp can only read its own quarter of the lanes: otherwise one warp would do all the exponentials.
+// With <= 32 (64) rows the tile holds them four (two) times in its TMEM lane quarters and each copy takes a quarter (half) of a tile's
+// keys, because a warp can only read its own quarter of the lanes: otherwise one warp would do all the exponentials.
 //
 // Few row tiles are split over the key axis as well (grid), partial results joined by window_combine_kernel.
 //
 // Rows of V that no row may see (past a sequence's end, padding, pages handed on to others) may hold anything, NaN included:
-// a helper warp zeroes them in shared memory before they are multiplied with P's zeros.
+// the products' warp zeroes them in shared memory before they are multiplied with P's zeros.
 //
 // Every wait is bounded (sm100.cuh).
 #include <cstring>
@@ -72,33 +70,25 @@ struct WindowParams {
   int* status;
 };
 
-// COPIES: 0 for ROWS, else KEYS with the rows so many times in a tile.
 template <int DB, int COPIES>
 struct WindowCfg {
-  static constexpr bool KEYS = COPIES > 0;
   static constexpr int BN = 64;                          // keys of a tile
-  static constexpr int BUFS = 2;                         // score buffers of a stream
-  static constexpr int COPY_ROWS = KEYS ? 128 / COPIES : 128;
-  static constexpr int TN = KEYS ? BN / COPIES : BN;     // keys of a tile that a softmax thread takes, in chunks of CW
+  static constexpr int BUFS = 2;                         // score buffers
+  static constexpr int COPY_ROWS = 128 / COPIES;
+  static constexpr int TN = BN / COPIES;                 // keys of a tile that a softmax thread takes, in chunks of CW
   static constexpr int CW = TN < 32 ? TN : 32, CH = TN / CW;
-  static constexpr int STREAMS = KEYS ? 1 : 2;           // of a CTA
-  static constexpr int SOFT = 128 * STREAMS;             // softmax threads
-  // warps: softmax, producer of keys, scores, products, producer of values, V helper (KEYS: the products' warp helps, so that
-  // there are 8 warps of 128 registers)
-  static constexpr int W_K = 4 * STREAMS, W_S = W_K + 1, W_P = W_S + STREAMS, W_V = W_P + STREAMS, W_HELP = W_V + 1;
-  static constexpr int THREADS = (KEYS ? W_HELP : W_HELP + 1) * 32;
-  static constexpr int CTAS = KEYS ? 2 : 1;              // of an SM
+  // warps: 0-3 softmax, then the producer of keys, scores, products, producer of values
+  static constexpr int W_K = 4, W_S = 5, W_P = 6, W_V = 7, THREADS = 256, CTAS = 2;      // CTAs of an SM
   static constexpr int KBLK = BN * 128;                  // bytes of a [BN keys x 64 columns] block
-  static constexpr int Q_BYTES = STREAMS * DB * WA_BLK;
-  static constexpr int NK = DB == 2 ? (KEYS ? 3 : 5) : (KEYS ? 6 : 8);
-  static constexpr int NV = DB == 2 && KEYS ? 2 : NK;
+  static constexpr int Q_BYTES = DB * WA_BLK;
+  static constexpr int NK = DB == 2 ? 3 : 6, NV = DB == 2 ? 2 : 6;
   static constexpr int STAGE = DB * KBLK;
   static constexpr int SMEM_BYTES = Q_BYTES + (NK + NV) * STAGE + WA_CTL;
   static constexpr int PART_PITCH = DB * 64 + 4;         // floats; rows 16 bytes apart in banks
-  static_assert((SMEM_BYTES + 1024) * CTAS <= 233472 && (13 + 2 * NK + 3 * NV) * 8 + 8 <= 512, "shared memory");
-  static_assert(!KEYS || 128 * PART_PITCH * 4 <= (NK + NV) * STAGE, "partial results reuse the rings");
-  // TMEM: the streams' O, then their score buffers; P is written over the scores
-  static constexpr int O_STEP = 128, S_COL = STREAMS * 128, S_STEP = 128, TMEM_COLS = STREAMS * 256;
+  static_assert((SMEM_BYTES + 1024) * CTAS <= 233472 && (9 + 2 * NK + 2 * NV) * 8 + 8 <= 512, "shared memory");
+  static_assert(128 * PART_PITCH * 4 <= (NK + NV) * STAGE, "partial results reuse the rings");
+  // TMEM: O, then the score buffers; P is written over the scores
+  static constexpr int S_COL = 128, TMEM_COLS = 256;
 };
 
 // One row's place in the problem.
@@ -154,7 +144,6 @@ __global__ void __launch_bounds__(WindowCfg<DB, COPIES>::THREADS, WindowCfg<DB, 
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const WindowParams p) {
   using Cfg = WindowCfg<DB, COPIES>;
-  constexpr bool KEYS = Cfg::KEYS;
   constexpr int NK = Cfg::NK, NV = Cfg::NV, BN = Cfg::BN, BUFS = Cfg::BUFS;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {   // swizzled TMA / MMA tiles need 1024-byte aligned buffers
@@ -169,12 +158,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* k_full = q_full + 1;           // [NK]
   uint64_t* k_empty = k_full + NK;         // [NK]
   uint64_t* v_full = k_empty + NK;         // [NV] landed
-  uint64_t* v_ready = v_full + NV;         // [NV] unseen rows zeroed
-  uint64_t* v_empty = v_ready + NV;        // [NV]
-  uint64_t* s_full = v_empty + NV;         // [stream][buffer]
-  uint64_t* p_full = s_full + 4;           // [stream][buffer] P written
-  uint64_t* pv_done = p_full + 4;          // [stream][buffer] P read, O added to
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
+  uint64_t* v_empty = v_full + NV;         // [NV]
+  uint64_t* s_full = v_empty + NV;         // [buffer]
+  uint64_t* p_full = s_full + BUFS;        // [buffer] P written
+  uint64_t* pv_done = p_full + BUFS;       // [buffer] P read, O added to
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + BUFS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -184,10 +172,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   int* status = p.status;
 
   // rows and keys of this CTA
-  const int rows_q = Cfg::STREAMS * p.box_q;                     // queries of the CTA
-  const int s_first = xt * rows_q;
-  const int s_last = min(p.S, s_first + rows_q) - 1;
-  const bool two = !KEYS && s_first + p.box_q < p.S;               // is there a second row tile?
+  const int s_first = xt * p.box_q;
+  const int s_last = min(p.S, s_first + p.box_q) - 1;
   int prefix = 0, klim, pmin, pmax;
   if (p.cached) {
     prefix = max(0, min(p.lengths[b], p.T - p.S));                 // out-of-range prefixes are reported below
@@ -205,21 +191,19 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int NT = t1 - t0;
 
   if (threadIdx.x == 0) {
-    const uint32_t readers = two ? 2 : 1;     // MMA warps that read each tile
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
     mbar_init(q_full, 1);
     for (int i = 0; i < NK; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], readers);
+      mbar_init(&k_empty[i], 1);
     }
     for (int i = 0; i < NV; ++i) {
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_ready[i], 1);
-      mbar_init(&v_empty[i], readers);
+      mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < BUFS; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
@@ -265,12 +249,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       };
       int next = look_up(t0);
       if (is_k && elect_one()) {
-        const int nq = KEYS ? COPIES : (two ? 2 : 1);
-        mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.box_q * p.g * 128) * nq * DB);
-        for (int t = 0; t < nq; ++t)
+        mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.box_q * p.g * 128) * COPIES * DB);
+        for (int t = 0; t < COPIES; ++t)
           for (int kb = 0; kb < DB; ++kb)
-            tma_load_5d(KEYS ? qs + kb * WA_BLK + t * Cfg::COPY_ROWS * 128 : qs + (t * DB + kb) * WA_BLK, &tmQ, q_full, kb * 64, 0,
-                        KEYS ? s_first : s_first + t * p.box_q, hk, b);
+            tma_load_5d(qs + kb * WA_BLK + t * Cfg::COPY_ROWS * 128, &tmQ, q_full, kb * 64, 0, s_first, hk, b);
       }
       WaTile<BN> t(R, t0);
       const int stages = is_k ? NK : NV;
@@ -319,15 +301,52 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!__all_sync(0xffffffffu, ok)) break;
       }
     }
+  } else if (warp == Cfg::W_S) {
+    // ---------------------------------------------------------------- scores (one thread issues).  Scores and products have a thread
+    // each: one for both would hold a finished P back behind the scores of two tiles later, because an issuing thread advances no
+    // faster than the tensor pipe takes its instructions.
+    if (NT > 0 && elect_one()) {
+      // one descriptor each, advanced by adding to its address field (16-byte units)
+      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(qs), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(ks), 16, 1024);
+      bool ok = wa_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
+      WaTile<BN> t(R, t0);
+      for (int c = 0, stage = 0, phase = 0; c < NT && ok; ++c) {
+        const int buf = c & 1;
+        const uint32_t idesc_s = make_idesc(128, (t.keys() + 15) & ~15, 1, 1, 0, 0);
+        const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
+        const uint32_t d = tmem_base + Cfg::S_COL + buf * 64;
+        // the scores take the place of an earlier tile's P, once the product has read it
+        if (c >= 2 && !wa_wait(&pv_done[buf], ((c >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
+        if (!wa_wait(&k_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kb = 0; kb < DB; ++kb)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(d, q_desc + ((kb * WA_BLK + k * 32) >> 4), kd + ((kb * Cfg::KBLK + k * 32) >> 4), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&k_empty[stage]);
+        umma_commit(&s_full[buf]);
+        t.next();
+        if (++stage == NK) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
   } else {
-    // rows of V that nobody sees become zeros
+    // ---------------------------------------------------------------- products: the warp zeroes the rows of V that nobody sees, one
+    // thread issues
+    constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
+    const uint64_t v_desc = make_smem_desc_sw128(smem_u32(vs), Cfg::KBLK, 1024);
     unsigned long long nodes_any = ~0ull;
-    if (p.tree != nullptr && warp >= Cfg::W_P) {       // which drafted places hold a node
+    if (p.tree != nullptr) {       // which drafted places hold a node
       nodes_any = 0ull;
       const unsigned long long* tree = p.tree + static_cast<long long>(b) * p.tree_sb;
       for (int m = 0; m < p.S; ++m) nodes_any |= tree[m];
     }
-    auto zero_unseen = [&](const WaTile<BN>& t, int st) {
+    WaTile<BN> t(R, t0);
+    for (int c = 0, stage = 0, phase = 0; c < NT; ++c) {
+      if (!wa_warp_wait(&v_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
       const int k1 = t.k1();
       const bool tail = k1 - t.k0 < BN, head = t.in_window() && t.k0 < R.wtrue;
       const bool drafted = p.tree != nullptr && k1 > prefix;
@@ -340,117 +359,49 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int kb = 0; kb < DB; ++kb)
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(vs + st * Cfg::STAGE + kb * Cfg::KBLK + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<uint4*>(vs + stage * Cfg::STAGE + kb * Cfg::KBLK + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
       }
-    };
-    if (warp == Cfg::W_HELP) {
-      // -------------------------------------------------------------- V helper
-      WaTile<BN> t(R, t0);
-      int st = 0, ph = 0;
-      for (int i = t0; i < t1; ++i) {
-        if (!wa_warp_wait(&v_full[st], ph, abort_flag, status, ST_TIMEOUT_FULL)) break;
-        zero_unseen(t, st);
-        wa_warp_arrive(&v_ready[st]);
-        t.next();
-        if (++st == NV) {
-          st = 0;
-          ph ^= 1;
+      __syncwarp();
+      bool ok = true;
+      if (elect_one()) {           // (always the same thread)
+        const int buf = c & 1;
+        const int k16 = (t.keys() + 15) >> 4;
+        const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
+        const uint32_t a = tmem_base + Cfg::S_COL + buf * 64;
+        ok = wa_wait(&p_full[buf], (c >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+        if (ok) {
+          tc_fence_after();
+          umma_f16_ts(tmem_base, a, vd, idesc_o, c > 0 ? 1u : 0u);
+          if (k16 == BN / 16) {
+#pragma unroll
+            for (int k = 1; k < BN / 16; ++k) umma_f16_ts(tmem_base, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
+          } else {
+            for (int k = 1; k < k16; ++k) umma_f16_ts(tmem_base, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
+          }
+          umma_commit(&v_empty[stage]);
+          umma_commit(&pv_done[buf]);
         }
       }
-    } else {
-      // ---------------------------------------------------------------- MMA issuers: a thread each for the scores (W_S)
-      // and the products (W_P) of each stream.  One thread for both would hold a finished P back behind the scores of two tiles
-      // later: an issuing thread advances no faster than the tensor pipe takes its instructions.
-      const bool scores = warp < Cfg::W_P;
-      const int st = scores ? warp - Cfg::W_S : warp - Cfg::W_P;
-      if (st == 0 || two) {
-        // one descriptor each, advanced by adding to its address field (16-byte units)
-        const uint32_t s_col = tmem_base + Cfg::S_COL + st * Cfg::S_STEP, o_col = tmem_base + Cfg::O_STEP * st;
-        int c = 0;                                       // tiles so far
-        WaTile<BN> t(R, t0);
-        const int stages = scores ? NK : NV;
-        int stage = 0, phase = 0;
-        auto walk = [&] {
-          t.next();
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-          }
-        };
-        if (scores && elect_one()) {
-          const uint64_t q_desc = make_smem_desc_sw128(smem_u32(qs) + st * DB * WA_BLK, 16, 1024);
-          const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ks), 16, 1024);
-          bool ok = t0 >= t1 || wa_wait(q_full, 0, abort_flag, status, ST_TIMEOUT_FULL);
-          for (int i = t0; i < t1 && ok; ++i, ++c) {
-            const int buf = c & 1;
-            const uint32_t idesc_s = make_idesc(128, (t.keys() + 15) & ~15, 1, 1, 0, 0);
-            const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
-            const uint32_t d = s_col + buf * 64;
-            // the scores take the place of an earlier tile's P, once the product has read it
-            if (c >= 2 && !wa_wait(&pv_done[st * 2 + buf], ((c >> 1) - 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
-            if (!wa_wait(&k_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
-            tc_fence_after();
-#pragma unroll
-            for (int kb = 0; kb < DB; ++kb)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16(d, q_desc + ((kb * WA_BLK + k * 32) >> 4), kd + ((kb * Cfg::KBLK + k * 32) >> 4), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
-            umma_commit(&k_empty[stage]);
-            umma_commit(&s_full[st * 2 + buf]);
-            walk();
-          }
-        } else if (!scores && (KEYS || elect_one())) {
-          constexpr uint32_t idesc_o = make_idesc(128, DB * 64, 1, 1, 0, 1);
-          const uint64_t v_desc = make_smem_desc_sw128(smem_u32(vs), Cfg::KBLK, 1024);
-          for (int i = t0; i < t1; ++i, ++c) {
-            const int buf = c & 1;
-            const int k16 = (t.keys() + 15) >> 4;
-            const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (Cfg::STAGE >> 4));
-            const uint32_t a = s_col + buf * 64;
-            if constexpr (KEYS) {              // all of the warp
-              if (!wa_warp_wait(&v_full[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
-              zero_unseen(t, stage);
-              __syncwarp();
-            } else {
-              if (!wa_wait(&v_ready[stage], phase, abort_flag, status, ST_TIMEOUT_FULL)) break;
-            }
-            bool ok = true;
-            if (!KEYS || elect_one()) {
-              ok = wa_wait(&p_full[st * 2 + buf], (c >> 1) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
-              if (ok) {
-                tc_fence_after();
-                umma_f16_ts(o_col, a, vd, idesc_o, c > 0 ? 1u : 0u);
-                if (k16 == BN / 16) {
-#pragma unroll
-                  for (int k = 1; k < BN / 16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
-                } else {
-                  for (int k = 1; k < k16; ++k) umma_f16_ts(o_col, a + k * 8, vd + ((k * 2048) >> 4), idesc_o, 1u);
-                }
-                umma_commit(&v_empty[stage]);
-                umma_commit(&pv_done[st * 2 + buf]);
-              }
-            }
-            if (KEYS ? !__all_sync(0xffffffffu, ok) : !ok) break;
-            walk();
-          }
-        }
+      if (!__all_sync(0xffffffffu, ok)) break;
+      t.next();
+      if (++stage == NV) {
+        stage = 0;
+        phase ^= 1;
       }
     }
-    }
+  }
   } else {
-    // ---------------------------------------------------------------- softmax and epilogue (a warp group per stream)
-    const int st = warp >> 2, quarter = warp & 3;
-    const int row = quarter * 32 + lane;
+    // ---------------------------------------------------------------- softmax and epilogue
+    const int quarter = warp, row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_base = tmem_base + lane_addr + Cfg::S_COL + st * Cfg::S_STEP, o_addr = tmem_base + lane_addr + Cfg::O_STEP * st;
-    const bool active = st == 0 || two;
+    const uint32_t s_base = tmem_base + lane_addr + Cfg::S_COL, o_addr = tmem_base + lane_addr;
     const int copy = row / Cfg::COPY_ROWS;
     const int rr = row - copy * Cfg::COPY_ROWS;         // row within the tile
-    const WindowRow w = window_row(p, rr, s_first + st * p.box_q, hk, b, klim, prefix);
+    const WindowRow w = window_row(p, rr, s_first, hk, b, klim, prefix);
     constexpr int CW = Cfg::CW, CH = Cfg::CH;
     const int first_key = copy * Cfg::TN;    // of a tile's keys, this thread's TN begin here
     const bool warp_ok = __any_sync(0xffffffffu, w.ok);
@@ -458,11 +409,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int all_upto = __reduce_min_sync(0xffffffffu, w.ok ? w.plim : 0x7fffffff);
     const int all_from = __reduce_max_sync(0xffffffffu, w.ok ? w.lo : -0x7fffffff);
     float m_ref = -INFINITY, l_sum = 0.f;
-    bool ok = active;
+    bool ok = true;
     int c = 0;
-    if (active) {
-      auto scores_in = [&](int at) {         // tile `at` of this stream: are its scores there?
-        return wa_warp_wait(&s_full[st * 2 + at % BUFS], (at / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+    {
+      auto scores_in = [&](int at) {         // tile `at`: are its scores there?
+        return wa_warp_wait(&s_full[at % BUFS], (at / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       };
       uint32_t x[CH][CW];                    // the scores of this thread's chunks
       // (a short tile's last columns hold anything and are masked; wide: more keys than the first chunk's)
@@ -480,7 +431,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           ok = false;
           break;
         }
-        wa_warp_arrive(&p_full[st * 2 + c % BUFS]);
+        wa_warp_arrive(&p_full[c % BUFS]);
       }
       WaTile<BN> t(R, t0);
       bool wide = CH == 1 || t.keys() > CW;
@@ -545,7 +496,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           if (c > 0) {
             // O is rescaled when the previous tile's product has completed
-            if (!wa_warp_wait(&pv_done[st * 2 + (buf ^ 1)], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
+            if (!wa_warp_wait(&pv_done[buf ^ 1], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) return false;
             tc_fence_after();
 #pragma unroll 1
             for (int cc = 0; cc < DB * 2; ++cc) {
@@ -561,7 +512,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         };
         const bool first_keys = __any_sync(0xffffffffu, w.ok && m_ref == -INFINITY);     // a row without a reference yet
         float sum = 0.f;
-        if constexpr (KEYS) {                // few tiles: the first one counts
+        if constexpr (COPIES > 1) {          // few tiles: the first one counts
           bool seek = first_keys;
           for (int pass = 0;; ++pass) {
             if (seek && !(ok = lift())) break;
@@ -589,7 +540,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         tmem_wait_st();
         tc_fence_before();
-        wa_warp_arrive(&p_full[st * 2 + buf]);
+        wa_warp_arrive(&p_full[buf]);
         if (more) {
           if (!scores_in(c + 1)) {
             ok = false;
@@ -603,13 +554,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       // (the product before the last completes before it: one thread issued both)
       if (c > 0 && ok)
-        ok = wa_warp_wait(&pv_done[st * 2 + (c - 1) % BUFS], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
+        ok = wa_warp_wait(&pv_done[(c - 1) % BUFS], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       tc_fence_after();
     }
     const float LN2 = 0.6931471805599453f;
-    if constexpr (COPIES <= 1) {
+    if constexpr (COPIES == 1) {
       // -------------------------------------------------------------- a thread writes its row
-      if (active && ok) {
+      if (ok) {
         float inv = 0.f;
         const bool in = rr / p.g < p.box_q && w.s < p.S;       // a padding node's row is written too (zeros)
         const long long idx = ((static_cast<long long>(b) * p.S + w.s) * p.H + w.h) * p.splits + split;
@@ -664,12 +615,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     } else {
       // -------------------------------------------------------------- join the copies, then write
-      // The rings are free: both streams' last products have completed, and they read every tile that was fetched.
+      // The rings are free: the last product has completed, and the products read every tile that was fetched.
       float* part = reinterpret_cast<float*>(ks);
       float2* xml = reinterpret_cast<float2*>(qs);           // (reference, sum) of every row: the queries have been read
       if (c == 0) m_ref = -INFINITY;
       xml[row] = make_float2(w.ok ? m_ref : -INFINITY, l_sum);
-      if (named_bar_and(1, Cfg::SOFT, ok)) {
+      if (named_bar_and(1, 128, ok)) {
         float top = -INFINITY;
         for (int q = 0; q < COPIES; ++q) top = fmaxf(top, xml[q * Cfg::COPY_ROWS + rr].x);
         const float wt = w.ok && m_ref > -INFINITY ? exp2f(m_ref - top) : (l_sum == l_sum ? 0.f : l_sum);
@@ -692,10 +643,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         }
       }
-      if (named_bar_and(1, Cfg::SOFT, ok)) {
+      if (named_bar_and(1, 128, ok)) {
         const int vec = p.Dv / 8;                                  // 16-byte output pieces of a row
         const int rows = min(p.box_q, p.S - s_first) * p.g;
-        for (int it = threadIdx.x; it < rows * vec; it += Cfg::SOFT) {
+        for (int it = threadIdx.x; it < rows * vec; it += 128) {
           const int r = it / vec, col = (it - r * vec) * 8;
           float top = -INFINITY, l = 0.f, f8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
           for (int q = 0; q < COPIES; ++q) top = fmaxf(top, xml[q * Cfg::COPY_ROWS + r].x);
@@ -885,8 +836,7 @@ int launch_window_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   auto kern = cmb::window_fwd_kernel<DB, COPIES>;
   static std::atomic<unsigned long long> attr_done{0};
   if (cmb_host::set_smem_limit_once_per_device(attr_done, reinterpret_cast<const void*>(kern), Cfg::SMEM_BYTES)) return 103;
-  const int per = Cfg::STREAMS * p.box_q;
-  dim3 grid((p.S + per - 1) / per, p.Hk, B * p.splits);
+  dim3 grid((p.S + p.box_q - 1) / p.box_q, p.Hk, B * p.splits);
   kern<<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? 0 : 104;
 }
@@ -930,16 +880,10 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
                              static_cast<long long>(p.table_w) * p.page < p.T))
     return 1;
   const long long rows = static_cast<long long>(p.S) * p.g;
-  const bool keys = rows <= 128;
   if (p.splits > 1 && (at->ws_o == nullptr || at->ws_ml == nullptr)) return 1;
   if ((a.o_sb | a.o_ss | a.o_sh) & 7 || (reinterpret_cast<uintptr_t>(at->out) & 15)) return 1;
-  int copies = 0;
-  if (keys) {
-    p.box_q = p.S;
-    copies = rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
-  } else {
-    p.box_q = 128 / p.g < p.S ? 128 / p.g : p.S;
-  }
+  p.box_q = 128 / p.g < p.S ? 128 / p.g : p.S;
+  const int copies = rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
   p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
   p.out = static_cast<__nv_bfloat16*>(at->out); p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
   p.lse = static_cast<float*>(at->lse);
@@ -958,7 +902,6 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
   auto launch = [&](auto db) {
     constexpr int DB = decltype(db)::value;
     switch (copies) {
-      case 0: return launch_window_fwd<DB, 0>(tq, tk, tv, p, B, st);
       case 1: return launch_window_fwd<DB, 1>(tq, tk, tv, p, B, st);
       case 2: return launch_window_fwd<DB, 2>(tq, tk, tv, p, B, st);
       default: return launch_window_fwd<DB, 4>(tq, tk, tv, p, B, st);

@@ -149,15 +149,15 @@ def _sizes_covered(q, k, v) -> bool:
             and dv <= MAX_HEAD_DIM and q.shape[2] // k.shape[2] <= MAX_GROUP and k.shape[2] <= 65535 and q.shape[0] <= 65535)
 
 
-def choose_splits(ctas: int, tiles: int, small: bool) -> int:
+def choose_splits(ctas: int, tiles: int) -> int:
     """How many ways to split the key axis of ``ctas`` thread blocks whose rows see about ``tiles`` 64-key tiles: enough blocks for
-    every SM (two on an SM where a block is ``small``: up to 128 rows), a tile or more to a block."""
-    return max(1, min((2 if small else 1) * NUM_SMS // max(1, ctas), tiles if small else (tiles + 1) // 2, 64))
+    every SM, which holds two, and a tile or more to a block."""
+    return max(1, min(2 * NUM_SMS // max(1, ctas), tiles, 64))
 
 
 def row_blocks(s: int, g: int) -> int:
-    """Thread blocks per (sequence, key head): up to 128 rows in one, else two row tiles of 128 // g queries each."""
-    return 1 if s * g <= 128 else -(-s // (2 * (128 // g)))
+    """Thread blocks per (sequence, key head): 128 // g queries each."""
+    return -(-s // (128 // g))
 
 
 def sink_split(s: int, t: int, window: int, sink_tokens: int, g: int) -> tuple[int, int]:
@@ -232,9 +232,9 @@ def plan_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page: i
     w = NO_WINDOW if window is None else min(int(window), NO_WINDOW)
     g = h // hk
     blocks = row_blocks(s, g)
-    span = s if tree is not None or blocks == 1 else 2 * (128 // g)
+    span = s if tree is not None or blocks == 1 else 128 // g
     reach = min(t if max_keys is None else min(t, max_keys), w + span)
-    splits = choose_splits(b * hk * blocks, -(-reach // 64) + -(-min(sink_tokens, t) // 64), s * g <= 128)
+    splits = choose_splits(b * hk * blocks, -(-reach // 64) + -(-min(sink_tokens, t) // 64))
     if b * splits > 65535:
         splits = 1
     box_k = 64 if table is None else min(64, page & -page)     # key rows of one copy; a tile is 64 keys
