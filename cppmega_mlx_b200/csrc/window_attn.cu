@@ -32,7 +32,9 @@
 // With <= 32 (64) rows the tile holds them four (two) times in its TMEM lane quarters and each copy takes a quarter (half) of a tile's
 // keys, because a warp can only read its own quarter of the lanes: otherwise one warp would do all the exponentials.
 //
-// Few row tiles are split over the key axis as well (grid), partial results joined by window_combine_kernel.
+// Few row tiles are split over the key axis as well (grid): up to 8 splits of up to 64 rows are a cluster, which joins
+// their partial results through shared memory; others go through global memory and window_combine_kernel (a cluster of 128-row tiles
+// took 16.1 us where this took 12.7: 60 nodes over 1024 keys).
 //
 // Rows of V that no row may see (past a sequence's end, padding, pages handed on to others) may hold anything, NaN included:
 // the products' warp zeroes them in shared memory before they are multiplied with P's zeros.
@@ -64,8 +66,8 @@ struct WindowParams {
   __nv_bfloat16* out;
   long long o_sb, o_ss, o_sh;
   float* lse;                            // [B, H, S] natural log, +inf where a row sees nothing; may be null
-  int splits;
-  float* ws_o;                           // [B, S, H, splits, Dv]
+  int splits, joined;                    // joined: a row's splits are a cluster, which joins them through shared memory
+  float* ws_o;                           // [B, S, H, splits, Dv], not joined
   float2* ws_ml;                         // [B, S, H, splits] (max, sum)
   int* status;
 };
@@ -154,6 +156,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint8_t* ks = qs + Cfg::Q_BYTES;
   uint8_t* vs = ks + NK * Cfg::STAGE;
   uint8_t* ctl = vs + NV * Cfg::STAGE;
+  // at the end, when the queries and the rings have been read:
+  float2* xml = reinterpret_cast<float2*>(qs);           // [128] (reference, sum) of every row and copy
+  float2* fml = xml + 128;                               // [128] of every row, for the cluster's other splits
+  float* part = reinterpret_cast<float*>(ks);            // [128][PART_PITCH]
   uint64_t* q_full = reinterpret_cast<uint64_t*>(ctl);
   uint64_t* k_full = q_full + 1;           // [NK]
   uint64_t* k_empty = k_full + NK;         // [NK]
@@ -226,6 +232,30 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // a row's end: its head's sink logit joins (reference, sum), and what O is multiplied with
+  auto finish = [&](int h, float& m, float& l) {
+    float f = 1.f;
+    if (p.sinks.p != nullptr) {
+      const float s2 = p.sinks.log2_at(h), top = fmaxf(m, s2);
+      f = m == -INFINITY ? 0.f : exp2f(m - top);
+      l = l * f + exp2f(s2 - top);
+      m = top;
+    }
+    return l > 0.f ? f / l : (l == l ? 0.f : l);
+  };
+  auto put_lse = [&](int s, int h, float m, float l) {
+    p.lse[(static_cast<long long>(b) * p.H + h) * p.S + s] = l == 0.f ? INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  };
+  auto put_row = [&](int s, int h, int col, float m, float l, const float (&f8)[8]) {
+    const float inv = finish(h, m, l);
+    uint4 v;
+    v.x = pack_bf16x2(f8[0] * inv, f8[1] * inv);
+    v.y = pack_bf16x2(f8[2] * inv, f8[3] * inv);
+    v.z = pack_bf16x2(f8[4] * inv, f8[5] * inv);
+    v.w = pack_bf16x2(f8[6] * inv, f8[7] * inv);
+    *reinterpret_cast<uint4*>(p.out + b * p.o_sb + s * p.o_ss + h * p.o_sh + col) = v;
+    if (p.lse != nullptr && col == 0) put_lse(s, h, m, l);
+  };
   if (warp >= Cfg::W_K) {
   if (warp == Cfg::W_K || warp == Cfg::W_V) {
     // ---------------------------------------------------------------- TMA producers of keys (and queries) and of values: one thread
@@ -557,29 +587,22 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = wa_warp_wait(&pv_done[(c - 1) % BUFS], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       tc_fence_after();
     }
-    const float LN2 = 0.6931471805599453f;
     if constexpr (COPIES == 1) {
-      // -------------------------------------------------------------- a thread writes its row
+      // -------------------------------------------------------------- a thread holds a row; the warp writes its rows one after the
+      // other through the rings, which are free (16 bytes of 32 rows at a time left half of every sector to a second write)
       if (ok) {
-        float inv = 0.f;
+        float inv = 1.f;
         const bool in = rr / p.g < p.box_q && w.s < p.S;       // a padding node's row is written too (zeros)
         const long long idx = ((static_cast<long long>(b) * p.S + w.s) * p.H + w.h) * p.splits + split;
         if (p.splits == 1) {
-          float l = l_sum, m = m_ref, f = 1.f;
-          if (p.sinks.p != nullptr && in) {
-            const float s2 = p.sinks.log2_at(w.h);
-            const float top = fmaxf(m, s2);
-            f = m == -INFINITY ? 0.f : exp2f(m - top);
-            l = l * f + exp2f(s2 - top);
-            m = top;
-          }
-          inv = l > 0.f ? f / l : (l == l ? 0.f : l);
-          if (p.lse != nullptr && in)
-            p.lse[(static_cast<long long>(b) * p.H + w.h) * p.S + w.s] = l == 0.f ? INFINITY : (m + log2f(l)) * LN2;
+          float l = l_sum;
+          inv = in ? finish(w.h, m_ref, l) : 0.f;
+          if (p.lse != nullptr && in) put_lse(w.s, w.h, m_ref, l);
         } else if (in) {
           p.ws_ml[idx] = make_float2(m_ref, l_sum);
         }
-        const bool any = __any_sync(0xffffffffu, w.ok) && c > 0;
+        const bool any = __any_sync(0xffffffffu, w.ok) && c > 0, have = any && w.ok;
+        float* mine = part + row * Cfg::PART_PITCH;
 #pragma unroll
         for (int cc = 0; cc < DB * 2; ++cc) {
           uint32_t o[32];
@@ -587,37 +610,54 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_ld_x32(o_addr + cc * 32, o);
             tmem_wait_ld();
           }
-          const bool have = any && w.ok;
-          if (in) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = have ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+          if (p.splits == 1) {
 #pragma unroll
             for (int ch = 0; ch < 4; ++ch) {
-              const int col = cc * 32 + ch * 8;
-              if (col < p.Dv) {
-                float f8[8];
+              uint32_t v[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f8[e] = have ? __uint_as_float(o[8 * ch + e]) : 0.f;
-                if (p.splits == 1) {
-                  uint4 v;
-                  v.x = pack_bf16x2(f8[0] * inv, f8[1] * inv);
-                  v.y = pack_bf16x2(f8[2] * inv, f8[3] * inv);
-                  v.z = pack_bf16x2(f8[4] * inv, f8[5] * inv);
-                  v.w = pack_bf16x2(f8[6] * inv, f8[7] * inv);
-                  *reinterpret_cast<uint4*>(p.out + b * p.o_sb + w.s * p.o_ss + w.h * p.o_sh + col) = v;
-                } else {
-                  float4* dst = reinterpret_cast<float4*>(p.ws_o + idx * p.Dv + col);
-                  dst[0] = make_float4(f8[0], f8[1], f8[2], f8[3]);
-                  dst[1] = make_float4(f8[4], f8[5], f8[6], f8[7]);
-                }
-              }
+              for (int e = 0; e < 4; ++e) v[e] = pack_bf16x2(__uint_as_float(o[8 * ch + 2 * e]), __uint_as_float(o[8 * ch + 2 * e + 1]));
+              reinterpret_cast<uint4*>(mine)[cc * 4 + ch] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          } else {
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch)
+              reinterpret_cast<uint4*>(mine)[cc * 8 + ch] = make_uint4(o[4 * ch], o[4 * ch + 1], o[4 * ch + 2], o[4 * ch + 3]);
+          }
+        }
+        __syncwarp();
+        const unsigned rows_in = __ballot_sync(0xffffffffu, in);
+        const bool last = p.splits == 1;
+        // in 16-byte pieces
+        const int vec = last ? p.Dv / 8 : p.Dv / 4;
+        const long long at = last ? (b * p.o_sb + w.s * p.o_ss + w.h * p.o_sh) / 8 : idx * vec;
+        uint4* dst = last ? reinterpret_cast<uint4*>(p.out) : reinterpret_cast<uint4*>(p.ws_o);
+        const int row_step = 32 / vec, piece_step = 32 - row_step * vec;
+        int r = lane / vec, piece = lane - r * vec;
+        for (int e0 = 0; e0 < vec; e0 += 4) {          // (four loads, then their stores)
+          uint4 v[4];
+          long long to[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            to[e] = __shfl_sync(0xffffffffu, at, r & 31) + piece;
+            if (e0 + e >= vec || !((rows_in >> (r & 31)) & 1u)) to[e] = -1;
+            else v[e] = reinterpret_cast<const uint4*>(part + (quarter * 32 + r) * Cfg::PART_PITCH)[piece];
+            r += row_step;
+            piece += piece_step;
+            if (piece >= vec) {
+              piece -= vec;
+              ++r;
             }
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (to[e] >= 0) dst[to[e]] = v[e];
         }
       }
     } else {
       // -------------------------------------------------------------- join the copies, then write
       // The rings are free: the last product has completed, and the products read every tile that was fetched.
-      float* part = reinterpret_cast<float*>(ks);
-      float2* xml = reinterpret_cast<float2*>(qs);           // (reference, sum) of every row: the queries have been read
       if (c == 0) m_ref = -INFINITY;
       xml[row] = make_float2(w.ok ? m_ref : -INFINITY, l_sum);
       if (named_bar_and(1, 128, ok)) {
@@ -661,23 +701,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           const int ql = r / p.g, s = s_first + ql, h = hk * p.g + (r - ql * p.g);
           if (p.splits == 1) {
-            float m = top, f = 1.f;
-            if (p.sinks.p != nullptr) {
-              const float s2 = p.sinks.log2_at(h);
-              const float t2 = fmaxf(m, s2);
-              f = m == -INFINITY ? 0.f : exp2f(m - t2);
-              l = l * f + exp2f(s2 - t2);
-              m = t2;
-            }
-            const float inv = l > 0.f ? f / l : (l == l ? 0.f : l);
-            uint4 v;
-            v.x = pack_bf16x2(f8[0] * inv, f8[1] * inv);
-            v.y = pack_bf16x2(f8[2] * inv, f8[3] * inv);
-            v.z = pack_bf16x2(f8[4] * inv, f8[5] * inv);
-            v.w = pack_bf16x2(f8[6] * inv, f8[7] * inv);
-            *reinterpret_cast<uint4*>(p.out + b * p.o_sb + s * p.o_ss + h * p.o_sh + col) = v;
-            if (p.lse != nullptr && col == 0)
-              p.lse[(static_cast<long long>(b) * p.H + h) * p.S + s] = l == 0.f ? INFINITY : (m + log2f(l)) * LN2;
+            put_row(s, h, col, top, l, f8);
+          } else if (p.joined) {             // in place: no other thread reads these columns of the row
+            float4* dst = reinterpret_cast<float4*>(part + r * Cfg::PART_PITCH + col);
+            dst[0] = make_float4(f8[0], f8[1], f8[2], f8[3]);
+            dst[1] = make_float4(f8[4], f8[5], f8[6], f8[7]);
+            if (col == 0) fml[r] = make_float2(top, l);
           } else {
             const long long idx = ((static_cast<long long>(b) * p.S + s) * p.H + h) * p.splits + split;
             float4* dst = reinterpret_cast<float4*>(p.ws_o + idx * p.Dv + col);
@@ -688,6 +717,47 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     }
+  }
+
+  if (COPIES > 1 && p.joined) {
+    // ---------------------------------------------------------------- the cluster joins its splits, each CTA some pieces of the rows
+    __syncwarp();
+    cluster_sync_all();
+    const int vec = p.Dv / 8;
+    const int items = min(p.box_q, p.S - s_first) * p.g * vec;
+    for (int it = split * Cfg::THREADS + static_cast<int>(threadIdx.x); it < items; it += p.splits * Cfg::THREADS) {
+      const int r = it / vec, col = (it - r * vec) * 8;
+      float2 ml[8];
+      float4 a[8], d[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        ml[q] = make_float2(-INFINITY, 0.f);
+        a[q] = d[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (q < p.splits) {
+          const float* at = wa_peer(part + r * Cfg::PART_PITCH + col, q);
+          ml[q] = *reinterpret_cast<const float2*>(wa_peer(reinterpret_cast<float*>(fml + r), q));
+          a[q] = *reinterpret_cast<const float4*>(at);
+          d[q] = *reinterpret_cast<const float4*>(at + 4);
+        }
+      }
+      float top = -INFINITY, l = 0.f, f8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) top = fmaxf(top, ml[q].x);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float wt = ml[q].x > -INFINITY ? exp2f(ml[q].x - top) : (ml[q].y == ml[q].y ? 0.f : ml[q].y);
+        if (wt != 0.f) {
+          l = fmaf(ml[q].y, wt, l);
+          f8[0] = fmaf(a[q].x, wt, f8[0]); f8[1] = fmaf(a[q].y, wt, f8[1]);
+          f8[2] = fmaf(a[q].z, wt, f8[2]); f8[3] = fmaf(a[q].w, wt, f8[3]);
+          f8[4] = fmaf(d[q].x, wt, f8[4]); f8[5] = fmaf(d[q].y, wt, f8[5]);
+          f8[6] = fmaf(d[q].z, wt, f8[6]); f8[7] = fmaf(d[q].w, wt, f8[7]);
+        }
+      }
+      const int ql = r / p.g;
+      put_row(s_first + ql, hk * p.g + (r - ql * p.g), col, top, l, f8);
+    }
+    cluster_sync_all();          // no CTA's shared memory goes before the others have read it
   }
 
   // ---------------------------------------------------------------- teardown
@@ -703,8 +773,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-// Joins the splits of a row (sequence, query, head), four output columns per lane: a warp, or with more than 8 splits a block of
-// four warps that share them (61 nodes, 16 heads, 37 splits: 13.8 us with a warp each).
+// Joins the splits of a row (sequence, query, head): a block of four warps that share them, four output columns per lane (61 nodes,
+// 16 heads, 37 splits: 5.2 us; 13.8 us with one warp).
 struct CombineParams {
   int S, H, splits, Dv;
   long long rows;
@@ -715,12 +785,10 @@ struct CombineParams {
   long long o_sb, o_ss, o_sh;
   float* lse;
 };
-template <bool SHARED>
 __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams p) {
   __shared__ float4 parts[3][32];
   const int warp = threadIdx.x >> 5;
-  const long long row = SHARED ? blockIdx.x : static_cast<long long>(blockIdx.x) * 4 + warp;
-  if (row >= p.rows) return;
+  const long long row = blockIdx.x;
   const int lane = threadIdx.x & 31;
   const int h = static_cast<int>(row % p.H);
   const long long bs = row / p.H;
@@ -737,7 +805,7 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool in = lane * 4 < p.Dv;
   const float* src = p.ws_o + row * p.splits * p.Dv + lane * 4;
-  for (int i0 = SHARED ? 8 * warp : 0; i0 < p.splits; i0 += SHARED ? 32 : 8) {
+  for (int i0 = 8 * warp; i0 < p.splits; i0 += 32) {
     float4 a[8];
     float w[8];
 #pragma unroll
@@ -755,15 +823,13 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams
       o.w = fmaf(a[i].w, w[i], o.w);
     }
   }
-  if constexpr (SHARED) {
-    if (warp > 0) parts[warp - 1][lane] = o;
-    __syncthreads();
-    if (warp > 0) return;
+  if (warp > 0) parts[warp - 1][lane] = o;
+  __syncthreads();
+  if (warp > 0) return;
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const float4 a = parts[i][lane];
-      o.x += a.x; o.y += a.y; o.z += a.z; o.w += a.w;
-    }
+  for (int i = 0; i < 3; ++i) {
+    const float4 a = parts[i][lane];
+    o.x += a.x; o.y += a.y; o.z += a.z; o.w += a.w;
   }
   float f = 1.f;
   if (p.sinks.p != nullptr) {
@@ -837,8 +903,17 @@ int launch_window_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   static std::atomic<unsigned long long> attr_done{0};
   if (cmb_host::set_smem_limit_once_per_device(attr_done, reinterpret_cast<const void*>(kern), Cfg::SMEM_BYTES)) return 103;
   dim3 grid((p.S + p.box_q - 1) / p.box_q, p.Hk, B * p.splits);
-  kern<<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : 104;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(Cfg::THREADS);
+  config.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  config.stream = stream;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim = {1, 1, static_cast<unsigned>(p.splits)};
+  config.attrs = &cluster;
+  config.numAttrs = p.joined ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kern, tq, tk, tv, p) == cudaSuccess ? 0 : 104;
 }
 
 }  // namespace
@@ -855,7 +930,7 @@ struct cmb_window_ptrs {
 };
 // q [B,S,H,Dq]; k / v rows [outer, rows, Hk, Dq | Dv] with outer = B (contiguous, rows = T) or pages of a pool (table
 // [B, table_w], rows = page size); bf16 with unit inner stride.  Dq, Dv <= 128 and multiples of 8; H / Hk <= 128.  ws_o / ws_ml
-// are needed for splits > 1 only.  Returns 0, 1 for arguments that the kernel does not cover.
+// are needed for more than 8 splits, and for 2 or more where S H / Hk > 64.  Returns 0, 1 for arguments that the kernel does not cover.
 extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs* at, void* stream) {
   const cmb_window_call& a = *call;
   cmb::WindowParams p{};
@@ -880,7 +955,8 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
                              static_cast<long long>(p.table_w) * p.page < p.T))
     return 1;
   const long long rows = static_cast<long long>(p.S) * p.g;
-  if (p.splits > 1 && (at->ws_o == nullptr || at->ws_ml == nullptr)) return 1;
+  p.joined = p.splits > 1 && p.splits <= 8 && rows <= 64;
+  if (p.splits > 1 && !p.joined && (at->ws_o == nullptr || at->ws_ml == nullptr)) return 1;
   if ((a.o_sb | a.o_ss | a.o_sh) & 7 || (reinterpret_cast<uintptr_t>(at->out) & 15)) return 1;
   p.box_q = 128 / p.g < p.S ? 128 / p.g : p.S;
   const int copies = rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
@@ -908,16 +984,13 @@ extern "C" int cmb_window_fwd(const cmb_window_call* call, const cmb_window_ptrs
     }
   };
   rc = wide ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 1>{});
-  if (rc || p.splits == 1) return rc;
+  if (rc || p.splits == 1 || p.joined) return rc;
   cmb::CombineParams c{};
   c.S = p.S; c.H = p.H; c.splits = p.splits; c.Dv = p.Dv;
   c.rows = static_cast<long long>(B) * p.S * p.H;
   c.ws_o = p.ws_o; c.ws_ml = p.ws_ml; c.sinks = p.sinks;
   c.out = p.out; c.o_sb = p.o_sb; c.o_ss = p.o_ss; c.o_sh = p.o_sh; c.lse = p.lse;
-  const bool shared = p.splits > 8;
-  const long long blocks = shared ? c.rows : (c.rows + 3) / 4;
-  if (blocks > 0x7fffffffll) return 1;
-  if (shared) cmb::window_combine_kernel<true><<<static_cast<unsigned>(blocks), 128, 0, st>>>(c);
-  else cmb::window_combine_kernel<false><<<static_cast<unsigned>(blocks), 128, 0, st>>>(c);
+  if (c.rows > 0x7fffffffll) return 1;
+  cmb::window_combine_kernel<<<static_cast<unsigned>(c.rows), 128, 0, st>>>(c);
   return cudaGetLastError() == cudaSuccess ? 0 : 104;
 }

@@ -122,6 +122,11 @@ __device__ __forceinline__ bool wa_warp_wait(uint64_t* bar, uint32_t parity, vol
   __syncwarp();
   return ok;
 }
+__device__ __forceinline__ float* wa_peer(float* mine, int rank) {      // the same place in a cluster CTA's shared memory
+  float* at;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(at) : "l"(mine), "r"(rank));
+  return at;
+}
 __device__ __forceinline__ void wa_warp_arrive(uint64_t* bar) {      // one arrival for the warp's work so far
   __syncwarp();
   if (elect_one()) mbar_arrive(bar);

@@ -31,6 +31,8 @@ from . import _backend as B
 
 NO_WINDOW = 1 << 30
 NUM_SMS = 148
+JOIN_ROWS = 64         # as the kernel has it
+JOIN_TILES = 32        # 4 tiles for each of 8 blocks take as long as a second kernel that joins more of them (8 heads over 2048 keys: 9.4, 10.4 us)
 MAX_HEAD_DIM = 128
 MAX_GROUP = 128
 MAX_GROUP_GRAD = 64        # the backward's sub-tiles hold 64 rows
@@ -149,10 +151,11 @@ def _sizes_covered(q, k, v) -> bool:
             and dv <= MAX_HEAD_DIM and q.shape[2] // k.shape[2] <= MAX_GROUP and k.shape[2] <= 65535 and q.shape[0] <= 65535)
 
 
-def choose_splits(ctas: int, tiles: int) -> int:
+def choose_splits(ctas: int, tiles: int, rows: int) -> int:
     """How many ways to split the key axis of ``ctas`` thread blocks whose rows see about ``tiles`` 64-key tiles: enough blocks for
-    every SM, which holds two, and a tile or more to a block."""
-    return max(1, min(2 * NUM_SMS // max(1, ctas), tiles, 64))
+    every SM, which holds two, and a tile or more to a block.  Up to 8 of up to 64 ``rows`` are joined within the kernel, so few tiles
+    get no more there."""
+    return max(1, min(2 * NUM_SMS // max(1, ctas), tiles, 8 if rows <= JOIN_ROWS and tiles <= JOIN_TILES else 64))
 
 
 def row_blocks(s: int, g: int) -> int:
@@ -234,7 +237,7 @@ def plan_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page: i
     blocks = row_blocks(s, g)
     span = s if tree is not None or blocks == 1 else 128 // g
     reach = min(t if max_keys is None else min(t, max_keys), w + span)
-    splits = choose_splits(b * hk * blocks, -(-reach // 64) + -(-min(sink_tokens, t) // 64))
+    splits = choose_splits(b * hk * blocks, -(-reach // 64) + -(-min(sink_tokens, t) // 64), s * g)
     if b * splits > 65535:
         splits = 1
     box_k = 64 if table is None else min(64, page & -page)     # key rows of one copy; a tile is 64 keys
@@ -247,7 +250,7 @@ def plan_forward(q, k, v, *, t: int, lengths, cached: bool, tree, table, page: i
                       k.shape[0] if table is not None else 0, box_k, splits, int(sinks_bf16), 0, *strides3(q), *strides3(k), *strides3(v),
                       *o, scale)
     plain = lambda x: x is not None and (x.dtype != torch.int32 or not x.is_contiguous())  # noqa: E731
-    return ForwardPlan(True, True, scale, call, out_shape, rows, rows * splits * (dv + 2) if splits > 1 else 0, rows * splits * dv,
+    return ForwardPlan(True, True, scale, call, out_shape, rows, rows * splits * (dv + 2) if splits > 8 or (splits > 1 and s * g > JOIN_ROWS) else 0, rows * splits * dv,
                        (plain(lengths), plain(table), sinks is not None and (sinks.dtype not in (torch.bfloat16, torch.float32)
                                                                             or not sinks.is_contiguous())), w, int(sink_tokens), {})
 
