@@ -588,8 +588,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_after();
     }
     if constexpr (COPIES == 1) {
-      // -------------------------------------------------------------- a thread holds a row; the warp writes its rows one after the
-      // other through the rings, which are free (16 bytes of 32 rows at a time left half of every sector to a second write)
+      // -------------------------------------------------------------- a thread holds a row; it leaves through the rings, which are
+      // free: the last product has completed, and the products read every tile that was fetched
       if (ok) {
         float inv = 1.f;
         const bool in = rr / p.g < p.box_q && w.s < p.S;       // a padding node's row is written too (zeros)
@@ -626,34 +626,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               reinterpret_cast<uint4*>(mine)[cc * 8 + ch] = make_uint4(o[4 * ch], o[4 * ch + 1], o[4 * ch + 2], o[4 * ch + 3]);
           }
         }
-        __syncwarp();
-        const unsigned rows_in = __ballot_sync(0xffffffffu, in);
-        const bool last = p.splits == 1;
-        // in 16-byte pieces
-        const int vec = last ? p.Dv / 8 : p.Dv / 4;
-        const long long at = last ? (b * p.o_sb + w.s * p.o_ss + w.h * p.o_sh) / 8 : idx * vec;
-        uint4* dst = last ? reinterpret_cast<uint4*>(p.out) : reinterpret_cast<uint4*>(p.ws_o);
-        const int row_step = 32 / vec, piece_step = 32 - row_step * vec;
-        int r = lane / vec, piece = lane - r * vec;
-        for (int e0 = 0; e0 < vec; e0 += 4) {          // (four loads, then their stores)
-          uint4 v[4];
-          long long to[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            to[e] = __shfl_sync(0xffffffffu, at, r & 31) + piece;
-            if (e0 + e >= vec || !((rows_in >> (r & 31)) & 1u)) to[e] = -1;
-            else v[e] = reinterpret_cast<const uint4*>(part + (quarter * 32 + r) * Cfg::PART_PITCH)[piece];
-            r += row_step;
-            piece += piece_step;
-            if (piece >= vec) {
-              piece -= vec;
-              ++r;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (to[e] >= 0) dst[to[e]] = v[e];
-        }
+        if (p.splits == 1)
+          wa_write_rows(reinterpret_cast<const uint8_t*>(part + quarter * 32 * Cfg::PART_PITCH), Cfg::PART_PITCH * 4, p.Dv / 8,
+                        p.out + b * p.o_sb + w.s * p.o_ss + w.h * p.o_sh, in);
+        else
+          wa_write_rows(reinterpret_cast<const uint8_t*>(part + quarter * 32 * Cfg::PART_PITCH), Cfg::PART_PITCH * 4, p.Dv / 4,
+                        p.ws_o + idx * p.Dv, in);
       }
     } else {
       // -------------------------------------------------------------- join the copies, then write

@@ -122,6 +122,35 @@ __device__ __forceinline__ bool wa_warp_wait(uint64_t* bar, uint32_t parity, vol
   __syncwarp();
   return ok;
 }
+// Writes the warp's 32 rows of `vec` 16-byte pieces, staged in shared memory `pitch` bytes apart, each to its lane's `to` (rows of lanes
+// that are not `in` are left out): whole lines, where every lane writing its own row leaves half of each sector to a second write.
+__device__ __forceinline__ void wa_write_rows(const uint8_t* rows, int pitch, int vec, void* to, bool in) {
+  if (vec <= 0) return;
+  __syncwarp();
+  const int lane = threadIdx.x & 31;
+  const unsigned rows_in = __ballot_sync(0xffffffffu, in);
+  const int row_step = 32 / vec, piece_step = 32 - row_step * vec;
+  int r = lane / vec, piece = lane - r * vec;
+  for (int e0 = 0; e0 < vec; e0 += 4) {          // (four loads, then their stores)
+    uint4 v[4];
+    uint4* at[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      at[e] = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), r & 31)) + piece;
+      if (e0 + e >= vec || !((rows_in >> (r & 31)) & 1u)) at[e] = nullptr;
+      else v[e] = *reinterpret_cast<const uint4*>(rows + r * pitch + piece * 16);
+      r += row_step;
+      piece += piece_step;
+      if (piece >= vec) {
+        piece -= vec;
+        ++r;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (at[e] != nullptr) *at[e] = v[e];
+  }
+}
 __device__ __forceinline__ float* wa_peer(float* mine, int rank) {      // the same place in a cluster CTA's shared memory
   float* at;
   asm("mapa.u64 %0, %1, %2;" : "=l"(at) : "l"(mine), "r"(rank));

@@ -11,9 +11,6 @@
 // The sinks' gradient, -sum_i p_i,sink (do_i . o_i), would feel the rounding of o to bf16 (the sum has few outputs and both signs), so
 // DQ adds up do_i . o_i = sum_j p_ij dP_ij itself, in fp32, where sinks are trained.
 //
-// Rows that see few keys have an o as large as single values, and dP - delta cancels: there o's rounding would be most of dS's error.
-// Where a row tile sees at most one sub-tile of keys, DQ (launched first) takes delta from sum_j p_ij dP_ij too, and leaves it for DKV.
-//
 // dK and dQ carry the softmax scale once, at the end.  P and dS are rounded to bf16 (half a step, 2^-8: the operand type of the
 // gradient products) and written back over S and dP in TMEM, where they are the A operands; dQ, dK, dV accumulate there in fp32.
 // One thread issues every product in order; two warp groups take alternate sub-tiles, so that one's exponentials run under
@@ -21,6 +18,13 @@
 //
 // The first tokens are seen by every later row: their key tiles would run S / (64 / g) sub-tiles where another runs about
 // (window + 128) / (64 / g).  Their rows are split over CTAs, fp32 partial results are summed in a fixed order by window_join_kernel.
+//
+// DKV goes first, and DQ's blocks start beside its last ones (a programmatic launch; the two need nothing of each other): DKV has few
+// long blocks, 256 where 2 x 4096 queries meet 4 key heads, which keep 148 SMs busy for 86% of two waves.  Forward and backward of
+// that call, 16 heads of 128, a window of 1024: 414 -> 388 us; 16384 queries, a window of 2048: 1414 -> 1255 us.
+//
+// What bounds it: the tensor pipe.  A 64-wide sub-tile of DKV takes 1304 clocks of products (DQ 1044) and 1640 (1430) in all; products
+// of N = 64 with both operands in shared memory run at 70% of the full rate.
 //
 // A key that no row sees may hold anything: K rows of no row of the tile are zeroed in shared memory before dQ's product.
 #include "window_attn.h"
@@ -41,8 +45,8 @@ struct WindowBwdParams {
   int window, ns;
   const int* lengths;
   float2* stats;                           // [B, Hk, S * g] (lse * log2 e, delta) of packed rows; lse = +inf: sees nothing
-  __nv_bfloat16 *o1, *o2;                  // DQ: dq, -;  DKV: dk, dv
-  long long o1_sb, o1_ss, o1_sh, o2_sb, o2_ss, o2_sh;
+  __nv_bfloat16 *dq, *dk, *dv;             // DQ's, DKV's results
+  long long dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
   int sink_tiles, sink_splits;             // DKV: the first sink_tiles key tiles are split
   float* part;                             // [B, Hk, sink_tiles, sink_splits, 128, Dq + Dv]
   WaSinks sinks;                           // for SINKS
@@ -124,6 +128,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     NT = min(sub_n, (part + 1) * per) - min(sub_n, part * per);
   }
 
+  if (MODE == WB_DKV) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // DQ's blocks may follow on idle SMs
   if (threadIdx.x == 0) {
     mbar_init(r_full, 1);
     for (int i = 0; i < WB_NS; ++i) {
@@ -316,23 +321,6 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         break;
       }
       tc_fence_after();
-      if (MODE == WB_DQ && NT == 1) {
-        float sum[2] = {0.f, 0.f};
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          uint32_t x1[32], x2[32];
-          tmem_ld_x32(x_addr + 32 * i, x1);
-          tmem_ld_x32(x_addr + 64 + 32 * i, x2);
-          tmem_wait_ld();
-          const unsigned word = i ? words[1] : words[0];
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if ((word >> e) & 1u) sum[e & 1] = fmaf(exp2f(fmaf(__uint_as_float(x1[e]), p.scale_log2, -lse2)), __uint_as_float(x2[e]), sum[e & 1]);
-        }
-        delta = sum[0] + sum[1];
-        if (row_ok)
-          p.stats[(static_cast<long long>(b) * p.Hk + hk) * p.S * p.g + static_cast<long long>(qi) * p.g + (row - ql * p.g)].y = delta;
-      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t x1[32], x2[32], pw[16], dw[16];
@@ -388,13 +376,18 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       const int D = second ? p.Dv : p.Dq;
       const float mul = second ? 1.f : p.scale;
       const bool in = MODE == WB_DQ ? row_ok : row0 + row < p.T;
-      __nv_bfloat16* dst = second ? p.o2 + b * p.o2_sb + (row0 + row) * p.o2_ss + hk * p.o2_sh
-                                  : (MODE == WB_DQ ? p.o1 + b * p.o1_sb + qi * p.o1_ss + head * p.o1_sh
-                                                   : p.o1 + b * p.o1_sb + (row0 + row) * p.o1_ss + hk * p.o1_sh);
+      __nv_bfloat16* dst = MODE == WB_DQ ? p.dq + b * p.dq_sb + qi * p.dq_ss + head * p.dq_sh + col0
+                           : second      ? p.dv + b * p.dv_sb + (row0 + row) * p.dv_ss + hk * p.dv_sh
+                                         : p.dk + b * p.dk_sb + (row0 + row) * p.dk_ss + hk * p.dk_sh;
       float* fdst = nullptr;
       if (MODE == WB_DKV && split >= 0)
         fdst = p.part + ((((static_cast<long long>(b) * p.Hk + hk) * p.sink_tiles + key_tile) * p.sink_splits + split) * 128 + row) *
                             (p.Dq + p.Dv) + (second ? p.Dq : 0);
+      // through the operands' shared memory, which is free: every product has completed
+      constexpr int PITCH = CHUNKS * (MODE == WB_DQ ? 64 : 128) + 16;
+      static_assert(8 * 32 * PITCH <= Cfg::R_BYTES + WB_NS * Cfg::STAGE, "rows reuse the operands");
+      uint8_t* stage = smem + warp * 32 * PITCH;
+      uint4* mine = reinterpret_cast<uint4*>(stage + lane * PITCH);
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
         uint32_t o[32];
@@ -403,22 +396,23 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
           tmem_wait_ld();
         }
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          const int col = col0 + c * 32 + ch * 8;
-          if (in && col < D) {
-            float f[8];
+        for (int e = 0; e < 32; ++e) o[e] = NT > 0 ? __float_as_uint(__uint_as_float(o[e]) * mul) : 0u;
+        if (MODE == WB_DKV && fdst != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = NT > 0 ? __uint_as_float(o[8 * ch + e]) * mul : 0.f;
-            if (fdst != nullptr) {
-              *reinterpret_cast<float4*>(fdst + col) = make_float4(f[0], f[1], f[2], f[3]);
-              *reinterpret_cast<float4*>(fdst + col + 4) = make_float4(f[4], f[5], f[6], f[7]);
-            } else {
-              *reinterpret_cast<uint4*>(dst + col) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                                               pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-            }
+          for (int ch = 0; ch < 8; ++ch) mine[c * 8 + ch] = make_uint4(o[4 * ch], o[4 * ch + 1], o[4 * ch + 2], o[4 * ch + 3]);
+        } else {
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = pack_bf16x2(__uint_as_float(o[8 * ch + 2 * e]), __uint_as_float(o[8 * ch + 2 * e + 1]));
+            mine[c * 4 + ch] = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
       }
+      const int cols = min(D - col0, CHUNKS * 32);
+      if (MODE == WB_DKV && fdst != nullptr) wa_write_rows(stage, PITCH, cols / 4, fdst, in);
+      else wa_write_rows(stage, PITCH, cols / 8, dst, in);
     }
   }
 
@@ -426,6 +420,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   if (*abort_flag) {
     for (int i = 0; i < 64; ++i) __nanosleep(2000);
   }
+  if (MODE == WB_DQ) asm volatile("griddepcontrol.wait;" ::: "memory");      // done is done for DKV too: what follows reads both
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
@@ -436,7 +431,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
 
 // Row statistics for the kernel above: stats[b, hk, s, hg] = (lse log2 e, do.o).  16 lanes to a row (8 columns each).
 struct StatsParams {
-  int B, S, H, g, Dv;
+  int B, S, T, H, g, Dq, Dv, window, ns;
+  float scale_log2;
+  const int* lengths;
+  const __nv_bfloat16 *q, *k, *v;
+  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
   const __nv_bfloat16* o;
   const __nv_bfloat16* d;
   long long o_sb, o_ss, o_sh, d_sb, d_ss, d_sh;
@@ -444,10 +443,15 @@ struct StatsParams {
   float2* stats;
 };
 constexpr int WS_ROWS = 64;                // queries of a block (one head)
-__global__ void __launch_bounds__(256) window_stats_kernel(const StatsParams p) {
+// Rows that see few keys have an o as large as single values, and dP - delta cancels: there o's rounding would be most of dS's error,
+// and delta is sum_j p_ij dP_ij in fp32.  With 8 keys |o| is a third of a value's size, its rounding 2^-8 of that, and dP - delta as
+// large as dP: a third of dS's own rounding of 2^-8.
+constexpr int WS_FEW = 8;
+__global__ void __launch_bounds__(256, 3) window_stats_kernel(const StatsParams p) {
   const int h = blockIdx.y, b = blockIdx.z, hk = h / p.g, hg = h - hk * p.g, Hk = p.H / p.g;
   const int sub = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const int s0 = blockIdx.x * WS_ROWS;
+  const int klim = p.lengths != nullptr ? max(0, min(p.lengths[b], p.T)) : p.T;
   uint4 a[4], c[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -472,6 +476,60 @@ __global__ void __launch_bounds__(256) window_stats_kernel(const StatsParams p) 
       const float lse = p.lse[(static_cast<long long>(b) * p.H + h) * p.S + s];
       p.stats[((static_cast<long long>(b) * Hk + hk) * p.S + s) * p.g + hg] = make_float2(lse * 1.4426950408889634f, sum);
     }
+  }
+  // the rows that see few keys, once more: four keys' loads at a time, sums handed round so that lane e + 4 i gets key e's
+#pragma unroll 1
+  for (int s = s0 + sub; s < min(s0 + WS_ROWS, p.S); s += 16) {
+    const int pos = p.T - p.S + s, lo = max(0, pos - p.window + 1);
+    const int n1 = min(min(p.ns, lo), klim), n = n1 + max(0, min(pos, klim - 1) - lo + 1);      // keys it sees: first tokens, all
+    if (n > WS_FEW) continue;
+    const unsigned half = 0xffffu << (16 * (sub & 1));
+    const bool in_q = l16 * 8 < p.Dq, in_v = l16 * 8 < p.Dv;
+    const float lse2 = p.lse[(static_cast<long long>(b) * p.H + h) * p.S + s] * 1.4426950408889634f;
+    uint4 xq = make_uint4(0, 0, 0, 0), xd = xq;
+    if (in_q) xq = *reinterpret_cast<const uint4*>(p.q + b * p.q_sb + s * p.q_ss + h * p.q_sh + l16 * 8);
+    if (in_v) xd = *reinterpret_cast<const uint4*>(p.d + b * p.d_sb + s * p.d_ss + h * p.d_sh + l16 * 8);
+    float fq[8], fd[8], sum = 0.f;
+    unpack8_bf16(xq, fq);
+    unpack8_bf16(xd, fd);
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 4) {
+      uint4 xk[4], xv[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + e;
+        const long long j = i < n1 ? i : lo + (i - n1);
+        xk[e] = xv[e] = make_uint4(0, 0, 0, 0);
+        if (i < n && in_q) xk[e] = *reinterpret_cast<const uint4*>(p.k + b * p.k_sb + j * p.k_ss + hk * p.k_sh + l16 * 8);
+        if (i < n && in_v) xv[e] = *reinterpret_cast<const uint4*>(p.v + b * p.v_sb + j * p.v_ss + hk * p.v_sh + l16 * 8);
+      }
+      float x[4], dp[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float fk[8], fv[8];
+        unpack8_bf16(xk[e], fk);
+        unpack8_bf16(xv[e], fv);
+        x[e] = dp[e] = 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          x[e] = fmaf(fq[u], fk[u], x[e]);
+          dp[e] = fmaf(fd[u], fv[u], dp[e]);
+        }
+      }
+      auto spread = [&](float (&y)[4]) {
+        const bool b0 = l16 & 1, b1 = l16 & 2;
+        const float s0 = __shfl_xor_sync(half, b0 ? y[0] : y[1], 1), s1 = __shfl_xor_sync(half, b0 ? y[2] : y[3], 1);
+        const float u0 = (b0 ? y[1] : y[0]) + s0, u1 = (b0 ? y[3] : y[2]) + s1;
+        float t = (b1 ? u1 : u0) + __shfl_xor_sync(half, b1 ? u0 : u1, 2);
+        t += __shfl_xor_sync(half, t, 4);
+        return t + __shfl_xor_sync(half, t, 8);
+      };
+      const float tx = spread(x), td = spread(dp);
+      if (i0 + (l16 & 3) < n) sum = fmaf(exp2f(fmaf(tx, p.scale_log2, -lse2)), td, sum);
+    }
+    sum += __shfl_xor_sync(half, sum, 1);
+    sum += __shfl_xor_sync(half, sum, 2);
+    if (l16 == 0) p.stats[((static_cast<long long>(b) * Hk + hk) * p.S + s) * p.g + hg].y = sum;
   }
 }
 
@@ -525,13 +583,22 @@ __global__ void __launch_bounds__(32) window_sinks_kernel(const float* part, int
 namespace {
 
 template <int MODE, int DB, bool SINKS = false>
-int launch_window_bwd(const CUtensorMap (&m)[4], const cmb::WindowBwdParams& p, int gx, int B, cudaStream_t stream) {
+int launch_window_bwd(const CUtensorMap (&m)[4], const cmb::WindowBwdParams& p, int gx, int B, cudaStream_t stream, bool beside = false) {
   using Cfg = cmb::WindowBwdCfg<DB>;
   auto kern = cmb::window_bwd_kernel<MODE, DB, SINKS>;
   static std::atomic<unsigned long long> attr_done{0};
   if (cmb_host::set_smem_limit_once_per_device(attr_done, reinterpret_cast<const void*>(kern), Cfg::SMEM_BYTES)) return 103;
-  kern<<<dim3(gx, p.Hk, B), cmb::WB_THREADS, Cfg::SMEM_BYTES, stream>>>(m[0], m[1], m[2], m[3], p);
-  return cudaGetLastError() == cudaSuccess ? 0 : 104;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(gx, p.Hk, B);
+  config.blockDim = dim3(cmb::WB_THREADS);
+  config.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kern, m[0], m[1], m[2], m[3], p) == cudaSuccess ? 0 : 104;
 }
 
 }  // namespace
@@ -576,7 +643,11 @@ extern "C" int cmb_window_bwd(const cmb_window_bwd_call* call, const cmb_window_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
   cmb::StatsParams sp{};
-  sp.B = B; sp.S = S; sp.H = H; sp.g = p.g; sp.Dv = Dv;
+  sp.B = B; sp.S = S; sp.T = T; sp.H = H; sp.g = p.g; sp.Dq = Dq; sp.Dv = Dv; sp.window = p.window; sp.ns = p.ns;
+  sp.scale_log2 = p.scale_log2; sp.lengths = p.lengths;
+  sp.q = static_cast<const __nv_bfloat16*>(at->q); sp.q_sb = a.q_sb; sp.q_ss = a.q_ss; sp.q_sh = a.q_sh;
+  sp.k = static_cast<const __nv_bfloat16*>(at->k); sp.k_sb = a.k_sb; sp.k_ss = a.k_ss; sp.k_sh = a.k_sh;
+  sp.v = static_cast<const __nv_bfloat16*>(at->v); sp.v_sb = a.v_sb; sp.v_ss = a.v_ss; sp.v_sh = a.v_sh;
   sp.o = static_cast<const __nv_bfloat16*>(at->o); sp.o_sb = a.o_sb; sp.o_ss = a.o_ss; sp.o_sh = a.o_sh;
   sp.d = static_cast<const __nv_bfloat16*>(at->dO); sp.d_sb = a.do_sb; sp.d_ss = a.do_ss; sp.d_sh = a.do_sh;
   sp.lse = static_cast<const float*>(at->lse); sp.stats = p.stats;
@@ -591,46 +662,42 @@ extern "C" int cmb_window_bwd(const cmb_window_bwd_call* call, const cmb_window_
     if (!rc) rc = cmb_host::make_tmap_rows(&mv, at->v, Dv, T, Hk, B, a.v_ss, a.v_sh, a.v_sb, box_k);
     return rc;
   };
+  CUtensorMap mq, mo, mk, mv;
+  if (at->dk != nullptr) {
+    if (int rc = maps(mq, mo, mk, mv, p.sub_q, 128)) return rc;
+    p.dk = static_cast<__nv_bfloat16*>(at->dk); p.dk_sb = a.dk_sb; p.dk_ss = a.dk_ss; p.dk_sh = a.dk_sh;
+    p.dv = static_cast<__nv_bfloat16*>(at->dv); p.dv_sb = a.dv_sb; p.dv_ss = a.dv_ss; p.dv_sh = a.dv_sh;
+    const CUtensorMap m[4] = {mk, mv, mq, mo};
+    const int gx = key_tiles + p.sink_tiles * (p.sink_splits - 1);
+    const int rc = wide ? launch_window_bwd<cmb::WB_DKV, 2>(m, p, gx, B, st) : launch_window_bwd<cmb::WB_DKV, 1>(m, p, gx, B, st);
+    if (rc) return rc + 10000;
+  }
   if (at->dq != nullptr) {
-    CUtensorMap mq, mo, mk, mv;
-    int rc = maps(mq, mo, mk, mv, p.box_q, cmb::WB_SUB);
-    if (rc) return rc;
-    cmb::WindowBwdParams pq = p;
-    pq.o1 = static_cast<__nv_bfloat16*>(at->dq); pq.o1_sb = a.dq_sb; pq.o1_ss = a.dq_ss; pq.o1_sh = a.dq_sh;
+    if (int rc = maps(mq, mo, mk, mv, p.box_q, cmb::WB_SUB)) return rc;
+    p.dq = static_cast<__nv_bfloat16*>(at->dq); p.dq_sb = a.dq_sb; p.dq_ss = a.dq_ss; p.dq_sh = a.dq_sh;
     const CUtensorMap m[4] = {mq, mo, mk, mv};
     const int gx = (S + p.box_q - 1) / p.box_q;
+    int rc;
     if (at->dsinks != nullptr) {
-      pq.sinks.p = at->sinks; pq.sinks.bf16 = a.sinks_bf16; pq.sink_part = static_cast<float*>(at->sink_part);
-      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2, true>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1, true>(m, pq, gx, B, st);
+      p.sinks.p = at->sinks; p.sinks.bf16 = a.sinks_bf16; p.sink_part = static_cast<float*>(at->sink_part);
+      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2, true>(m, p, gx, B, st, at->dk != nullptr) : launch_window_bwd<cmb::WB_DQ, 1, true>(m, p, gx, B, st, at->dk != nullptr);
       if (rc) return rc + 20000;
-      cmb::window_sinks_kernel<<<H, 32, 0, st>>>(pq.sink_part, B * gx, at->dsinks, a.sinks_bf16);
+      cmb::window_sinks_kernel<<<H, 32, 0, st>>>(p.sink_part, B * gx, at->dsinks, a.sinks_bf16);
       if (cudaGetLastError() != cudaSuccess) return 104;
     } else {
-      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2>(m, pq, gx, B, st) : launch_window_bwd<cmb::WB_DQ, 1>(m, pq, gx, B, st);
+      rc = wide ? launch_window_bwd<cmb::WB_DQ, 2>(m, p, gx, B, st, at->dk != nullptr) : launch_window_bwd<cmb::WB_DQ, 1>(m, p, gx, B, st, at->dk != nullptr);
       if (rc) return rc + 20000;
     }
   }
-  if (at->dk != nullptr) {
-    CUtensorMap mq, mo, mk, mv;
-    int rc = maps(mq, mo, mk, mv, p.sub_q, 128);
-    if (rc) return rc;
-    cmb::WindowBwdParams pk = p;
-    pk.o1 = static_cast<__nv_bfloat16*>(at->dk); pk.o1_sb = a.dk_sb; pk.o1_ss = a.dk_ss; pk.o1_sh = a.dk_sh;
-    pk.o2 = static_cast<__nv_bfloat16*>(at->dv); pk.o2_sb = a.dv_sb; pk.o2_ss = a.dv_ss; pk.o2_sh = a.dv_sh;
-    const CUtensorMap m[4] = {mk, mv, mq, mo};
-    const int gx = key_tiles + p.sink_tiles * (p.sink_splits - 1);
-    rc = wide ? launch_window_bwd<cmb::WB_DKV, 2>(m, pk, gx, B, st) : launch_window_bwd<cmb::WB_DKV, 1>(m, pk, gx, B, st);
-    if (rc) return rc + 10000;
-    if (p.sink_splits > 1 && p.sink_tiles > 0) {
-      cmb::JoinParams j{};
-      j.T = T; j.Hk = Hk; j.Dq = Dq; j.Dv = Dv; j.tiles = p.sink_tiles; j.splits = p.sink_splits; j.part = p.part;
-      j.dk = pk.o1; j.k_sb = pk.o1_sb; j.k_ss = pk.o1_ss; j.k_sh = pk.o1_sh;
-      j.dv = pk.o2; j.v_sb = pk.o2_sb; j.v_ss = pk.o2_ss; j.v_sh = pk.o2_sh;
-      j.n = static_cast<long long>(B) * Hk * p.sink_tiles * 128 * ((Dq + Dv) / 4);
-      if ((j.n + 255) / 256 > 0x7fffffffll) return 1;
-      cmb::window_join_kernel<<<static_cast<unsigned>((j.n + 255) / 256), 256, 0, st>>>(j);
-      if (cudaGetLastError() != cudaSuccess) return 104;
-    }
+  if (at->dk != nullptr && p.sink_splits > 1 && p.sink_tiles > 0) {
+    cmb::JoinParams j{};
+    j.T = T; j.Hk = Hk; j.Dq = Dq; j.Dv = Dv; j.tiles = p.sink_tiles; j.splits = p.sink_splits; j.part = p.part;
+    j.dk = p.dk; j.k_sb = p.dk_sb; j.k_ss = p.dk_ss; j.k_sh = p.dk_sh;
+    j.dv = p.dv; j.v_sb = p.dv_sb; j.v_ss = p.dv_ss; j.v_sh = p.dv_sh;
+    j.n = static_cast<long long>(B) * Hk * p.sink_tiles * 128 * ((Dq + Dv) / 4);
+    if ((j.n + 255) / 256 > 0x7fffffffll) return 1;
+    cmb::window_join_kernel<<<static_cast<unsigned>((j.n + 255) / 256), 256, 0, st>>>(j);
+    if (cudaGetLastError() != cudaSuccess) return 104;
   }
   return 0;
 }
