@@ -444,9 +444,9 @@ struct StatsParams {
 };
 constexpr int WS_ROWS = 64;                // queries of a block (one head)
 // Rows that see few keys have an o as large as single values, and dP - delta cancels: there o's rounding would be most of dS's error,
-// and delta is sum_j p_ij dP_ij in fp32.  With 8 keys |o| is a third of a value's size, its rounding 2^-8 of that, and dP - delta as
-// large as dP: a third of dS's own rounding of 2^-8.
-constexpr int WS_FEW = 8;
+// and delta is sum_j p_ij dP_ij in fp32.  o's rounding (half a step, 2^-8) is 1 / sqrt(keys) of dP's size: with more than 16 keys it
+// adds less than a tenth to what dS's own rounding costs.
+constexpr int WS_FEW = 16;
 __global__ void __launch_bounds__(256, 3) window_stats_kernel(const StatsParams p) {
   const int h = blockIdx.y, b = blockIdx.z, hk = h / p.g, hg = h - hk * p.g, Hk = p.H / p.g;
   const int sub = threadIdx.x >> 4, l16 = threadIdx.x & 15;
