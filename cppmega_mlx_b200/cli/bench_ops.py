@@ -329,6 +329,55 @@ def bench_flash(args) -> list[dict]:
     return rows
 
 
+def bench_window(args) -> list[dict]:
+    """Windowed attention with visible first tokens (``csrc/window_attn.cu``), its backward, attention of drafted tokens over a cache and
+    page movements (``csrc/pages.cu``).  TFLOP/s count the visible pairs: forward 2 (Dq + Dv) each, backward 2.5 times that; GB/s the
+    cache rows that are read, or twice the bytes that are moved."""
+    from cppmega_mlx_b200 import ops
+    pk = peaks()
+    dev = "cuda"
+    rows = []
+
+    def done(row):
+        rows.append(row)
+        print(json.dumps(row), flush=True)
+    for b, s, h, hk, d, w, ns, label in ((2, 4096, 16, 4, 128, 1024, 4, "training step"), (1, 16384, 16, 4, 128, 2048, 16, "long sequence")):
+        if args.only and args.only not in label:
+            continue
+        q, k, v = (torch.randn(b, s, n, d, device=dev).bfloat16().requires_grad_() for n in (h, hk, hk))
+        flops = 4.0 * d * b * h * sum(min(i + 1, w + min(ns, max(0, i + 1 - w))) for i in range(s))
+        fwd = lambda: ops.window_attention(q, k, v, window=w, sink_tokens=ns)  # noqa: E731
+        with torch.no_grad():
+            ms_f = time_cuda(fwd, iters=args.iters, warmup=args.warmup)
+        ms_fb = time_cuda(_fb(fwd, q, k, v), iters=args.iters, warmup=args.warmup)
+        done({"op": f"window attention {label} B{b} S{s} H{h}/{hk} d{d} window {w} first {ns}", "fwd_ms": ms_f, "fwd_tflops": flops / ms_f / 1e9,
+              "fwd_frac_of_measured_peak": flops / ms_f / 1e9 / pk["bf16_tflops"], "fwd_bwd_ms": ms_fb, "fwd_bwd_tflops": 3.5 * flops / ms_fb / 1e9,
+              "fwd_bwd_frac_of_measured_peak": 3.5 * flops / ms_fb / 1e9 / pk["bf16_tflops"]})
+    for b, n, h, hk, d, t, page, w, label in ((1, 1, 16, 4, 128, 901, 16, 512, "one next token"), (128, 1, 16, 4, 64, 8001, 0, 1024, "next tokens"),
+                                             (64, 12, 32, 8, 128, 8204, 64, None, "drafted trees")):
+        if args.only and args.only not in label:
+            continue
+        q = torch.randn(b, n, h, d, device=dev).bfloat16()
+        shape = (b * -(-t // page), page, hk, d) if page else (b, t, hk, d)
+        k, v = (torch.randn(*shape, device=dev).bfloat16() for _ in range(2))
+        table = torch.randperm(shape[0], device=dev).int().view(b, -1) if page else None
+        prefix = torch.full((b,), t - n, dtype=torch.int32, device=dev)
+        tree = ops.tree_words([(i - 1) // 2 for i in range(n)]).to(dev) if n > 1 else None
+        ms = time_cuda(lambda: ops.cached_attention(q, k, v, table, prefix, tree=tree, window=w, sink_tokens=4 if w else 0), iters=args.iters,
+                       warmup=args.warmup)
+        gb = 4e-9 * b * hk * d * min(t, (w or t) + 4)
+        done({"op": f"cached attention {label} B{b} N{n} H{h}/{hk} d{d} T{t} page {page} window {w}", "ms": ms, "gbs": gb / ms * 1e3,
+              "frac_of_measured_peak": gb / ms * 1e3 / pk["hbm_gbs"]})
+    if not args.only or args.only in "page copies":
+        pools = [torch.zeros(1024, 16, 16, 8, 128, device=dev, dtype=torch.bfloat16) for _ in range(2)]
+        at = torch.randperm(1024, device=dev).int()
+        ms = time_cuda(lambda: ops.copy_pages(pools, at[:500], at[500:1000]), iters=args.iters, warmup=args.warmup)
+        gb = 2e-9 * 500 * 2 * pools[0][0].numel() * 2
+        done({"op": "page copies 500 of 1024, 2 pools of 16 layers x 16 x 8 x 128", "ms": ms, "gbs": gb / ms * 1e3,
+              "frac_of_measured_peak": gb / ms * 1e3 / pk["hbm_gbs"]})
+    return rows
+
+
 def bench_fused_local(args) -> list[dict]:
     """The peer-memory kernels of the fused collectives with every "rank" living on this one GPU (the peer pointer tables point at
     local buffers): the ZeRO-1 reduce + AdamW + push kernel over W = 2 gradient / parameter copies, the Muon reduce and push kernels,
@@ -747,7 +796,7 @@ def bench_serving(args) -> list[dict]:
 
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser()
-    ap.add_argument("op", choices=["gemm", "composite", "mxfp8", "m2rnn", "sparse_mla", "flash", "fused_local", "dsa_loss", "linears", "mamba3_step", "decode", "decode_loop", "serving", "decode_trace", "decode_profile", "step_profile", "all"])
+    ap.add_argument("op", choices=["gemm", "composite", "mxfp8", "m2rnn", "sparse_mla", "flash", "window", "fused_local", "dsa_loss", "linears", "mamba3_step", "decode", "decode_loop", "serving", "decode_trace", "decode_profile", "step_profile", "all"])
     ap.add_argument("--json", default=None)
     ap.add_argument("--only", default=None, help="run the single case with this label (small captures under a profiler)")
     ap.add_argument("--iters", type=int, default=10)
@@ -770,6 +819,8 @@ def main(argv=None) -> int:
         rows += bench_mxfp8(args)
     if args.op in ("flash", "all"):
         rows += bench_flash(args)
+    if args.op in ("window", "all"):
+        rows += bench_window(args)
     if args.op in ("fused_local", "all"):
         rows += bench_fused_local(args)
     if args.op in ("m2rnn", "all"):
