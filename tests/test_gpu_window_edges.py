@@ -190,3 +190,42 @@ def test_backward_beside_other_work_on_the_stream():
         for s, w in zip(sums, want):
             assert torch.equal(s, w.float().sum())
     _done()
+
+
+def test_captured_backwards_with_joined_keys_side_by_side():
+    """Two captured training steps whose first tokens' keys are split and joined and whose sinks are trained, replayed on two streams."""
+    from cppmega_mlx_b200 import ops
+
+    def make(seed, s):
+        leaves = [_rand(1, s, n, 64, seed=seed + n).requires_grad_() for n in (4, 2, 1)]
+        leaves[2] = _rand(1, s, 2, 64, seed=seed + 9).requires_grad_()
+        leaves.append(_rand(4, seed=seed + 5).requires_grad_())
+        do = _rand(1, s, 4, 64, seed=seed + 6)
+
+        def step():
+            o = ops.window_attention(*leaves[:3], window=60, sink_tokens=6, sinks=leaves[3])
+            return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+        return leaves, step
+    sides, graphs = [torch.cuda.Stream() for _ in range(2)], []
+    for side, (seed, s) in zip(sides, ((0, 2100), (50, 1500))):
+        leaves, step = make(seed, s)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        with torch.no_grad():
+            leaves[0].mul_(-0.5)
+        graphs.append((g, out, step))
+    want = [step() for _, _, step in graphs]
+    for side in sides:
+        side.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for side, (g, _, _) in zip(sides, graphs):
+            with torch.cuda.stream(side):
+                g.replay()
+    _done()
+    for w, (_, out, _) in zip(want, graphs):
+        assert all(torch.equal(a, b) for a, b in zip(w, out))
