@@ -477,6 +477,7 @@ __global__ void __launch_bounds__(256, 3) window_stats_kernel(const StatsParams 
       p.stats[((static_cast<long long>(b) * Hk + hk) * p.S + s) * p.g + hg] = make_float2(lse * 1.4426950408889634f, sum);
     }
   }
+  if (klim == p.T && min(p.T - p.S + s0 + 1, p.window) > WS_FEW) return;       // no such row in most blocks
   // the rows that see few keys, once more: four keys' loads at a time, sums handed round so that lane e + 4 i gets key e's
 #pragma unroll 1
   for (int s = s0 + sub; s < min(s0 + WS_ROWS, p.S); s += 16) {
