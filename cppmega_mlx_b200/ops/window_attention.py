@@ -272,7 +272,7 @@ def launch_forward(plan: ForwardPlan, q, k, v, lengths, tree, table, sinks, want
 def converted(plan: ForwardPlan, lengths, table, sinks):
     a, b, c = plan.convert
     return (lengths.to(torch.int32).contiguous() if a else lengths, table.to(torch.int32).contiguous() if b else table,
-            sinks.float().contiguous() if c else sinks)
+            (sinks if sinks.dtype == torch.bfloat16 else sinks.float()).contiguous() if c else sinks)     # bf16 stays: the call says so
 
 
 def _plan_backward(q, k, v, do, sinks, plan: ForwardPlan, need_q: bool, need_kv: bool, need_s: bool):
