@@ -237,9 +237,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     float f = 1.f;
     if (p.sinks.p != nullptr) {
       const float s2 = p.sinks.log2_at(h), top = fmaxf(m, s2);
-      f = m == -INFINITY ? 0.f : exp2f(m - top);
-      l = l * f + exp2f(s2 - top);
-      m = top;
+      if (s2 != -INFINITY) {                 // (a logit of -inf is no key: a row that sees nothing keeps its sum of 0)
+        f = m == -INFINITY ? 0.f : exp2f(m - top);
+        l = l * f + exp2f(s2 - top);
+        m = top;
+      }
     }
     return l > 0.f ? f / l : (l == l ? 0.f : l);
   };
@@ -813,9 +815,11 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const CombineParams
   if (p.sinks.p != nullptr) {
     const float s2 = p.sinks.log2_at(h);
     const float t2 = fmaxf(top, s2);
-    f = top == -INFINITY ? 0.f : exp2f(top - t2);
-    l = l * f + exp2f(s2 - t2);
-    top = t2;
+    if (s2 != -INFINITY) {
+      f = top == -INFINITY ? 0.f : exp2f(top - t2);
+      l = l * f + exp2f(s2 - t2);
+      top = t2;
+    }
   }
   const float inv = l > 0.f ? f / l : (l == l ? 0.f : l);
   if (lane * 4 < p.Dv)

@@ -54,3 +54,40 @@ def test_sinks_of_any_layout_and_type(layout, dtype):
     _done()
     bits = [[[m <= i for m in range(5)] for i in range(5)]] * 2
     W.check(c, W.attention64(q[:, :5].detach(), k.detach(), v.detach(), W.cached_visible([85, 3], 5, 90, bits, None, 0, "cuda"), sinks.detach())["o"], "cached")
+
+
+@pytest.mark.parametrize("s,t", [(1, 60), (1, 1500), (1, 5000), (12, 700), (100, 100), (100, 4000)])     # whole, joined in a cluster, by a second kernel
+def test_rows_without_a_key_whose_sink_is_off(s, t):
+    """A logit of -inf is no key at all: a row that sees nothing yields zeros and adds nothing to any gradient."""
+    from cppmega_mlx_b200 import ops
+    q, k, v, do = _rand(2, s, 4, 64, seed=1), _rand(2, t, 2, 64, seed=2), _rand(2, t, 2, 64, seed=3), _rand(2, s, 4, 64, seed=4)
+    sinks = torch.tensor([float("-inf"), 0.5, float("-inf"), -2.0], device="cuda")
+    n = torch.tensor([0, t], dtype=torch.int32, device="cuda")
+    seen = W.visible(s, t, None, 0, n, "cuda")
+    with torch.no_grad():
+        alone = ops.window_attention(q, k, v, sinks=sinks, key_lengths=n)
+    leaves = [x.requires_grad_() for x in (q, k, v, sinks)]
+    o = ops.window_attention(q, k, v, sinks=sinks, key_lengths=n)
+    grads = torch.autograd.grad(o, leaves, do)
+    _done()
+    assert torch.equal(o, alone) and float(o[0].detach().abs().max()) == 0
+    ref = W.attention64(*(x.detach() for x in leaves[:3]), seen, sinks.detach(), do=do)
+    for got, name in zip((o.detach(), *grads), ("o", "dq", "dk", "dv", "ds")):
+        W.check(got, ref[name], name)
+    assert float(grads[3][0]) == 0 and float(grads[3][2]) == 0
+
+
+@pytest.mark.parametrize("prefix", [20, 900, 6000])
+@pytest.mark.parametrize("h", [2, 8, 40])
+def test_padding_nodes_whose_sink_is_off(prefix, h):
+    from cppmega_mlx_b200 import ops
+    par = [-1, 0, 0, -2, -2]
+    tree = ops.tree_words(par).cuda()
+    q, k, v = _rand(1, 5, h, 64, seed=1), _rand(1, prefix + 5, 2, 64, seed=2), _rand(1, prefix + 5, 2, 64, seed=3)
+    sinks = torch.zeros(h, device="cuda")
+    sinks[::2] = float("-inf")
+    o = ops.cached_attention(q, k, v, None, torch.tensor([prefix], device="cuda"), tree=tree, sinks=sinks)
+    _done()
+    bits = [[[bool(w >> m & 1) for m in range(5)] for w in tree.tolist()]]
+    W.check(o, W.attention64(q, k, v, W.cached_visible([prefix], 5, prefix + 5, bits, None, 0, "cuda"), sinks)["o"], "o")
+    assert float(o[:, 3:].abs().max()) == 0
