@@ -589,6 +589,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = wa_warp_wait(&pv_done[(c - 1) % BUFS], ((c - 1) / BUFS) & 1, abort_flag, status, ST_TIMEOUT_TMEM_FULL);
       tc_fence_after();
     }
+    if (!w.ok) {                             // its scores were never masked: what its query holds (NaN, too) ends here
+      m_ref = -INFINITY;
+      l_sum = 0.f;
+    }
     if constexpr (COPIES == 1) {
       // -------------------------------------------------------------- a thread holds a row; it leaves through the rings, which are
       // free: the last product has completed, and the products read every tile that was fetched
@@ -639,11 +643,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // -------------------------------------------------------------- join the copies, then write
       // The rings are free: the last product has completed, and the products read every tile that was fetched.
       if (c == 0) m_ref = -INFINITY;
-      xml[row] = make_float2(w.ok ? m_ref : -INFINITY, l_sum);
+      xml[row] = make_float2(m_ref, l_sum);
       if (named_bar_and(1, 128, ok)) {
         float top = -INFINITY;
         for (int q = 0; q < COPIES; ++q) top = fmaxf(top, xml[q * Cfg::COPY_ROWS + rr].x);
-        const float wt = w.ok && m_ref > -INFINITY ? exp2f(m_ref - top) : (l_sum == l_sum ? 0.f : l_sum);
+        const float wt = m_ref > -INFINITY ? exp2f(m_ref - top) : (l_sum == l_sum ? 0.f : l_sum);
         float* mine = part + row * Cfg::PART_PITCH;
 #pragma unroll
         for (int cc = 0; cc < DB * 2; ++cc) {

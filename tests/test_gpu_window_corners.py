@@ -91,3 +91,27 @@ def test_padding_nodes_whose_sink_is_off(prefix, h):
     bits = [[[bool(w >> m & 1) for m in range(5)] for w in tree.tolist()]]
     W.check(o, W.attention64(q, k, v, W.cached_visible([prefix], 5, prefix + 5, bits, None, 0, "cuda"), sinks)["o"], "o")
     assert float(o[:, 3:].abs().max()) == 0
+
+
+@pytest.mark.parametrize("batch,prefix", [(2, 20), (2, 700), (2, 6000), (160, 300)])      # one tile, split and joined both ways, whole
+@pytest.mark.parametrize("n,h", [(6, 4), (12, 8), (30, 8), (60, 16)])                     # up to 32 rows, up to 64, more, many
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_padding_nodes_with_anything_in_their_queries(batch, prefix, n, h, bad):
+    """Unused places of a captured step: zeros come out, and the others' results are what they are without them."""
+    from cppmega_mlx_b200 import ops
+    hk = 2
+    par = [(i - 1) // 2 for i in range(n)]
+    hole = [n - 1, n - 2, n // 2 + 1]                      # (leaves: a parent is no padding)
+    for i in hole:
+        par[i] = -2
+    tree = ops.tree_words(par).cuda()
+    q, k, v = _rand(batch, n, h, 64, seed=1), _rand(batch, prefix + n, hk, 64, seed=2), _rand(batch, prefix + n, hk, 64, seed=3)
+    sinks = _rand(h, seed=4)
+    lens = torch.full((batch,), prefix, dtype=torch.int32, device="cuda")
+    for sk in (None, sinks):
+        q[:, hole] = 0
+        want = ops.cached_attention(q, k, v, None, lens, tree=tree, sinks=sk)
+        q[:, hole] = bad
+        got = ops.cached_attention(q, k, v, None, lens, tree=tree, sinks=sk)
+        _done()
+        assert torch.equal(got, want) and float(got[:, hole].abs().max()) == 0
