@@ -44,6 +44,7 @@ class PagedKVBlockManager:
         self._refs = [0] * num_blocks                          # sequences that hold each block
         self.tables: dict[int, list[int]] = {}                 # -1: a block that a window has passed (release_window)
         self.lengths: dict[int, int] = {}
+        self._released: dict[int, tuple[int, int]] = {}        # (window, sink_tokens) of a sequence's latest release_window
 
     # -- accounting ------------------------------------------------------------------------------
     @property
@@ -77,6 +78,7 @@ class PagedKVBlockManager:
         for b in reversed(self.tables.pop(seq_id)):
             self._drop(b)
         self.lengths.pop(seq_id, None)
+        self._released.pop(seq_id, None)
 
     def _take(self) -> int:
         b = self._free.pop()
@@ -96,6 +98,8 @@ class PagedKVBlockManager:
             raise ValueError(f"sequence {new_id} already has blocks")
         self.tables[new_id] = list(self.tables[seq_id][:self.blocks_needed(self.lengths[seq_id])])
         self.lengths[new_id] = self.lengths[seq_id]
+        if seq_id in self._released:
+            self._released[new_id] = self._released[seq_id]
         for b in self.tables[new_id]:
             if b >= 0:
                 self._refs[b] += 1
@@ -122,15 +126,23 @@ class PagedKVBlockManager:
             copy_pages((self.k_pool, self.v_pool), src, [tbl[i] for i in at])
 
     def truncate(self, seq_id: int, num_tokens: int) -> None:
-        """Forget what a sequence holds behind its first ``num_tokens`` tokens; whole blocks behind them are freed."""
+        """Forget what a sequence holds behind its first ``num_tokens`` tokens; whole blocks behind them are freed.  Refused where the next
+        token would see, or be written into, a block that ``release_window`` has given back."""
         if not 0 <= num_tokens <= self.lengths[seq_id]:
             raise ValueError(f"sequence {seq_id} has {self.lengths[seq_id]} tokens, cannot keep {num_tokens}")
         tbl = self.tables[seq_id]
         keep = self.blocks_needed(num_tokens)
+        if num_tokens and seq_id in self._released:
+            window, sink_tokens = self._released[seq_id]
+            near = range(max(0, num_tokens - window + 1) // self.block_size, keep)
+            if any(tbl[i] < 0 for i in (*range(min(keep, self.blocks_needed(sink_tokens))), *near)):
+                raise ValueError(f"sequence {seq_id}: the window of {window} before token {num_tokens} lies in blocks that were released")
         for b in reversed(tbl[keep:]):
             self._drop(b)
         del tbl[keep:]
         self.lengths[seq_id] = num_tokens
+        if not num_tokens:
+            self._released.pop(seq_id, None)
 
     def release_window(self, seq_id: int, window: int, sink_tokens: int = 0) -> int:
         """Free the blocks that no later token sees under a sliding window with visible first tokens; how many."""
@@ -143,6 +155,7 @@ class PagedKVBlockManager:
                 self._drop(tbl[i])
                 tbl[i] = -1
                 n += 1
+        self._released[seq_id] = (window, sink_tokens)
         return n
 
     def accept(self, paths: dict[int, list[int]]) -> None:
