@@ -133,6 +133,16 @@ def check_status(device=None) -> None:
             raise RuntimeError(f"kernel status words non-zero on cuda:{idx}: {vals}")
 
 
+BAD_ARGUMENT = 6        # ST_BAD_ARGUMENT of csrc/sm100.cuh
+
+
+def report(bad: torch.Tensor) -> None:
+    """The plain forms' way to the status words, as a kernel's: where ``bad`` (one truth value on a CUDA device) holds and no earlier
+    error stands there.  Nothing waits for the device."""
+    word = status_buffer(bad.device)[:1]
+    word.masked_fill_(bad.reshape(1) & (word == 0), BAD_ARGUMENT)
+
+
 _launches = 0
 _launches_by_name: dict[str, int] = {}
 

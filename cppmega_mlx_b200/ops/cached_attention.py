@@ -15,7 +15,8 @@ prefix.  ``window`` and ``sink_tokens`` restrict both by position: a key at posi
 or ``j < sink_tokens``.  ``sinks`` [H]: one more key per head with that logit and value 0.
 
 What no token sees — rows past a sequence's end, table entries past them, pages behind the window — may hold anything.  A table
-entry or a length that the pool or the table cannot hold is reported by ``ops.check_status`` (the kernel stays inside the pool).
+entry or a length that the pool or the table cannot hold is reported by ``ops.check_status`` (nothing is read outside the pool); with
+CPU tensors it is a ``ValueError``.
 
 CUDA bf16 tensors run ``csrc/window_attn.cu`` (tcgen05, split over the keys when there are few rows); page sizes that are not a
 multiple of 8, other types and CPU tensors use ``cached_attention_reference``, the test oracle.  No gradients: inputs that require
@@ -74,21 +75,25 @@ def _no_gradient(q, k_rows, v_rows, sinks) -> None:
         raise ValueError("cached_attention has no gradient: call it under torch.no_grad(), or use window_attention")
 
 
+def _refuse(bad: torch.Tensor, what: str) -> None:
+    """As the kernel does: reported by ``ops.check_status``; on the CPU, where reading ``bad`` costs nothing, raised."""
+    if bad.device.type != "cpu":
+        B.report(bad)
+    elif bool(bad):
+        raise ValueError(f"cached_attention: {what}")
+
+
 def cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, *, tree=None, window: int | None = None, sink_tokens: int = 0,
                                sinks=None, scale: float | None = None):
     scale = _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale)
     _no_gradient(q, k_rows, v_rows, sinks)
     b, n = q.shape[:2]
     dev = q.device
-    prefix = prefix_lengths.long()
-    if table is not None:       # entries that no token reaches may be anything
-        ps = k_rows.shape[1]
-        need = torch.arange(table.shape[1], device=dev)[None] * ps < (prefix + n)[:, None]
-        pages = torch.where(need, table.long(), torch.zeros_like(table.long())).clamp_min(0)
-        k, v = k_rows[pages].flatten(1, 2), v_rows[pages].flatten(1, 2)
-    else:
-        k, v = k_rows, v_rows
-    t = k.shape[1]
+    page = k_rows.shape[1]
+    t = page * (1 if table is None else table.shape[1])
+    asked = prefix_lengths.long()
+    prefix = asked.clamp(0, max(0, t - n))
+    _refuse((prefix != asked).any() if t >= n else torch.ones((), dtype=torch.bool, device=dev), f"prefix_lengths and {n} tokens do not fit into {t} rows")
     idx = torch.arange(n, device=dev)
     bits = (idx[None] <= idx[:, None])[None] if tree is None else ((tree.reshape(-1, n, 1) >> idx) & 1).bool()
     bits = bits.expand(b, n, n)
@@ -101,6 +106,13 @@ def cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, *, tree
     held = (j >= prefix[:, None, None]) & (j < prefix[:, None, None] + n)
     mpos = (prefix[:, None] + depth.gather(1, m))[:, None]                # [B, 1, T]
     new = bits.gather(2, m[:, None].expand(b, n, t)) & held & ((pos - mpos < w) | (mpos < sink_tokens))
+    k, v = k_rows, v_rows
+    if table is not None:       # entries that no token reads may be anything
+        pages = table.long()
+        inside = (pages >= 0) & (pages < k_rows.shape[0])
+        _refuse(((old | new).any(1).view(b, table.shape[1], page).any(-1) & ~inside).any(), f"table names a page outside the pool of {k_rows.shape[0]}")
+        pages = torch.where(inside, pages, torch.zeros_like(pages))
+        k, v = (x[pages].flatten(1, 2) if x.shape[0] else x.new_zeros(b, t, *x.shape[2:]) for x in (k_rows, v_rows))
     return masked_softmax_attention(q, k, v, old | new, sinks, scale)
 
 

@@ -79,6 +79,19 @@ def _plan_copy(pools, src, dst):
     return covered, tuple((p.stride(0) * p.element_size(), 0, 0, (p.numel() // p.shape[0]) * p.element_size()) if p.numel() else None for p in pools)
 
 
+def copy_pages_reference(pools, src, dst) -> torch.Tensor:
+    """The plain form.  Pairs that the pool does not hold are left out; returns whether there were any (or pages written twice, or read and
+    written)."""
+    n = pools[0].shape[0]
+    inside = (src >= 0) & (src < n) & (dst >= 0) & (dst < n)
+    bad = (~inside & ((src != -1) | (dst != -1))).any()
+    s, d = src[inside], dst[inside]
+    for p in pools:
+        p[d] = p[s]
+    by_target = d.sort().values
+    return bad | (by_target[1:] == by_target[:-1]).any() | torch.isin(s[s != d], d).any()
+
+
 def copy_pages(pools, src, dst) -> None:
     """See the module docstring."""
     pools = _pools(pools)
@@ -101,12 +114,9 @@ def copy_pages(pools, src, dst) -> None:
     if src.shape[0] == 0 or n == 0:
         return
     if not covered or not B.kernels_enabled():
-        s, d = src.to(dev, torch.int64), dst.to(dev, torch.int64)
-        if src.device.type != "cpu":       # unused places are left out
-            pad = (s == -1) & (d == -1)
-            s, d = (s[~pad], d[~pad]) if bool(pad.any()) else (s, d)
-        for p in pools:
-            p[d] = p[s]
+        bad = copy_pages_reference(pools, src.to(dev, torch.int64), dst.to(dev, torch.int64))
+        if dev.type == "cuda":
+            B.report(bad)
         return
     with on_device(dev):
         if src.dtype != torch.int32 or src.device != dev or not src.is_contiguous():
@@ -122,16 +132,26 @@ def copy_pages(pools, src, dst) -> None:
                        _raw_stream(dev.index)), "copy_pages")
 
 
-def compact_rows_reference(pools, table, start, path, counts) -> None:
-    page = pools[0].shape[2]
-    i = torch.arange(path.shape[1], device=path.device)
+def compact_rows_reference(pools, table, start, path, counts) -> torch.Tensor:
+    """The plain form.  Rows outside the table or the pool are left out; returns whether there were any (or counts outside the path)."""
+    n, page, width, most = pools[0].shape[0], pools[0].shape[2], table.shape[1], path.shape[1]
+    i = torch.arange(most, device=path.device)
+    rows = counts.clamp(0, most)
+    use = (i < rows[:, None]) & (path != i)
+    bad = (rows != counts).any()
+    if width == 0:
+        return bad | use.any()
     to = start.long()[:, None] + i
-    fro = torch.where(i < counts[:, None], start.long()[:, None] + path, to)
-    use = (i < counts[:, None]) & (fro != to)
-    b = torch.arange(table.shape[0], device=path.device)[:, None].expand_as(to)[use]
-    to, fro = to[use], fro[use]
+    fro = start.long()[:, None] + path
+
+    def pool_page(pos):        # and whether the table and the pool hold the position
+        ids = table.long().gather(1, (pos // page).clamp(0, width - 1))
+        return ids, (pos >= 0) & (pos < width * page) & (ids >= 0) & (ids < n)
+    (to_page, to_held), (fro_page, fro_held) = pool_page(to), pool_page(fro)
+    held = use & to_held & fro_held & (path >= 0)
     for p in pools:
-        p[table[b, to // page].long(), :, to % page] = p[table[b, fro // page].long(), :, fro % page]
+        p[to_page[held], :, (to % page)[held]] = p[fro_page[held], :, (fro % page)[held]]
+    return bad | (use & ~held).any()
 
 
 def _plan_compact(pools, table, start, path, counts):
@@ -181,7 +201,9 @@ def compact_rows(pools, table, start, path, counts) -> None:
         if bool(((table < 0) | (table >= n))[need].any()):
             raise ValueError(f"compact_rows: a page outside the pool of {n}")
     if not covered or not B.kernels_enabled():
-        compact_rows_reference(pools, table, start, path, counts)
+        bad = compact_rows_reference(pools, table, start, path, counts)
+        if dev.type == "cuda":
+            B.report(bad)
         return
     with on_device(dev):
         table, start, path, counts = (x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()

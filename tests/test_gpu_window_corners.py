@@ -115,3 +115,35 @@ def test_padding_nodes_with_anything_in_their_queries(batch, prefix, n, h, bad):
         got = ops.cached_attention(q, k, v, None, lens, tree=tree, sinks=sk)
         _done()
         assert torch.equal(got, want) and float(got[:, hole].abs().max()) == 0
+
+
+def test_plain_forms_on_the_gpu_report_what_the_pool_cannot_hold():
+    """Pages that are not dense, page sizes that the kernels do not take and kernels turned off: the same contract, no failed assertion."""
+    from cppmega_mlx_b200 import ops
+    from cppmega_mlx_b200.ops import _backend as B
+    pool = torch.arange(96., device="cuda").view(6, 4, 4)
+    t = lambda *x: torch.tensor(x, device="cuda")  # noqa: E731
+    for thin in (pool[:, :, ::2], pool):
+        keep = pool.clone()
+        with B.use_kernels(thin is not pool):
+            before = B.launch_count("copy_pages")
+            ops.copy_pages(thin, t(1, 9, -3, -1), t(3, 0, 0, -1))
+            assert B.launch_count("copy_pages") == before
+        _reported()
+        assert torch.equal(thin[3], thin[1]) and torch.equal(thin[0], (keep[:, :, ::2] if thin is not pool else keep)[0])
+    pool = torch.randn(5, 2, 4, 3, 2, device="cuda")
+    keep, table = pool.clone(), t([4, 0], [2, 1])
+    for thin in (pool[..., :1], pool):
+        with B.use_kernels(thin is not pool):
+            for start, tbl in ((t(9, 0), table), (t(4, 0), t([4, 7], [2, 1])), (t(4, 0), t([4, -2], [2, 1]))):
+                ops.compact_rows(thin.transpose(-1, -2), tbl, start, t([1], [0]), t(1, 0))
+                _reported()
+                assert torch.equal(pool, keep)
+    q, k = _rand(2, 2, 2, 8), _rand(6, 7, 1, 8)
+    table, n = t([0, 1, 2], [3, 4, 5]), t(9, 3)
+    want = ops.cached_attention(q, k, k, table, n)
+    _done()
+    for tbl, lens in ((t([0, 6, 2], [3, 4, 5]), n), (t([-4, 1, 2], [3, 4, 5]), n), (table, t(10 ** 6, 3)), (table, t(-2, 3))):
+        got = ops.cached_attention(q, k, k, tbl, lens)
+        _reported()
+        assert torch.equal(got[1], want[1])

@@ -66,3 +66,53 @@ def test_truncate_keeps_what_the_released_window_needs():
     m.truncate(1, 31)
     with pytest.raises(ValueError, match="released"):
         m.truncate(1, 30)
+
+
+def test_plain_page_copies_skip_what_the_pool_does_not_hold():
+    """The plain forms serve CUDA tensors too (pages that are not dense, kernels turned off): there an index outside is skipped and
+    reported as the kernels do, and never reaches an indexing operation, which would end the process's context."""
+    from cppmega_mlx_b200.ops.pages import compact_rows_reference, copy_pages_reference
+    pool = torch.arange(24.).view(6, 4)
+    want = pool.clone()
+    want[3] = want[1]
+    t = torch.tensor
+    assert bool(copy_pages_reference((pool,), t([1, 9, -3, 2, -1]), t([3, 0, 0, 6, 2])))
+    assert torch.equal(pool, want)
+    assert not bool(copy_pages_reference((pool,), t([0, -1]), t([5, -1]))) and torch.equal(pool[5], want[0])
+    assert bool(copy_pages_reference((pool,), t([0, 1]), t([2, 2]))) and bool(copy_pages_reference((pool,), t([0, 1]), t([1, 2])))
+    assert not bool(copy_pages_reference((pool,), t([4]), t([4])))
+    pool = torch.randn(5, 2, 4, 3)
+    table = t([[4, 0], [2, 1]])
+    keep = pool.clone()
+    for start, path, counts, tbl in (([9, 0], [[1], [0]], [1, 0], table), ([0, 0], [[-1], [0]], [1, 0], table), ([0, 0], [[0], [0]], [2, 0], table),
+                                     ([-3, 0], [[2], [0]], [1, 0], table), ([4, 0], [[1], [0]], [1, 0], t([[4, 7], [2, 1]])),
+                                     ([4, 0], [[1], [0]], [1, 0], t([[4, -2], [2, 1]])), ([0, 0], [[0], [0]], [-1, 0], table)):
+        assert bool(compact_rows_reference((pool,), tbl, t(start), t(path), t(counts)))
+        assert torch.equal(pool, keep)
+    assert not bool(compact_rows_reference((pool,), table, t([2, 0]), t([[1, 2, 5], [3, 99, -9]]), t([3, 1])))
+    want = keep.clone()             # positions 3, 4 and 7 of the first sequence close up behind its second, 3 of the other moves to its start
+    want[4, :, 2], want[4, :, 3], want[0, :, 0], want[2, :, 0] = keep[4, :, 3], keep[0, :, 0], keep[0, :, 3], keep[2, :, 3]
+    assert torch.equal(pool, want)
+
+
+def test_plain_cached_attention_stays_inside_the_pool():
+    """On the CPU an entry that is read, or a length, that the pool or the table cannot hold is refused; what nobody reads may be anything."""
+    q, k = torch.randn(2, 2, 2, 8), torch.randn(6, 4, 1, 8)
+    table, n = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32), torch.tensor([9, 3])
+    want = ops.cached_attention(q, k, k, table, n)
+    hole = table.clone()
+    hole[1, 2] = 10 ** 6                                        # behind the sequence's end
+    assert torch.equal(ops.cached_attention(q, k, k, hole, n), want)
+    narrow = ops.cached_attention(q, k, k, table, n, window=3)
+    hole[0, :1] = -1                                            # behind the window: the first token at 9 sees 7, 8, 9
+    assert torch.equal(ops.cached_attention(q, k, k, hole, n, window=3), narrow)
+    for bad in (-1, 6, 2 ** 40):
+        tbl = table.long()
+        tbl[0, 1] = bad
+        with pytest.raises(ValueError, match="page"):
+            ops.cached_attention(q, k, k, tbl, n)
+    for lens in ([-1, 3], [11, 3], [9, 2 ** 40]):
+        with pytest.raises(ValueError, match="prefix"):
+            ops.cached_attention(q, k, k, table, torch.tensor(lens))
+    with pytest.raises(ValueError, match="page"):
+        ops.cached_attention(q, k[:0], k[:0], table, n)
