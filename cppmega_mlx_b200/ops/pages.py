@@ -109,8 +109,9 @@ def copy_pages(pools, src, dst) -> None:
             raise ValueError("copy_pages: a page is written twice, or read and written")
         if not used:
             return
-        if len(used) < src.shape[0]:
-            src, dst = torch.tensor([s for s, _ in used]), torch.tensor(to)
+        # the lists that were checked, in memory of their own that is not pinned: it has been read when the upload's call returns, and
+        # what the caller writes into its own then (pinned memory is read when the device comes to it) changes nothing
+        src, dst = torch.tensor([[s for s, _ in used], to], dtype=torch.int32).to(dev, non_blocking=True)
     if src.shape[0] == 0 or n == 0:
         return
     if not covered or not B.kernels_enabled():

@@ -147,3 +147,34 @@ def test_plain_forms_on_the_gpu_report_what_the_pool_cannot_hold():
         got = ops.cached_attention(q, k, k, tbl, lens)
         _reported()
         assert torch.equal(got[1], want[1])
+
+
+def test_host_indexes_are_the_caller_s_again_when_the_call_returns():
+    """Pinned lists that are overwritten behind queued work: the pages copied are those that were checked.  A graph, which would read the
+    lists again at every replay, takes none from the host."""
+    from cppmega_mlx_b200 import ops
+    n = 50000                                          # long enough for a copy that the device makes when it comes to it
+    pool = torch.arange(8 * n, device="cuda").view(2 * n, 4).clone()
+    want = pool.clone()
+    want[n:] = want[:n]
+    src, dst = torch.arange(n, dtype=torch.int32).pin_memory(), torch.arange(n, 2 * n, dtype=torch.int32).pin_memory()
+    other = src.flip(0)
+    ops.copy_pages(pool, [0], [0])                     # (the library is loaded)
+    _done()
+    torch.cuda._sleep(1_000_000_000)                   # half a second: the call returns long before
+    ops.copy_pages(pool, src, dst)
+    src.copy_(other)
+    _done()
+    assert torch.equal(pool, want)
+    a, b = torch.tensor([2], device="cuda"), torch.tensor([9], device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.copy_pages(pool, a, b)
+        for x, y in (([3], [4]), (torch.tensor([3]), torch.tensor([4])), (src[:1], src[1:2])):
+            with pytest.raises(RuntimeError, match="capture"):
+                ops.copy_pages(pool, x, y)
+    a.fill_(5)
+    g.replay()
+    _done()
+    want[9] = want[5]
+    assert torch.equal(pool, want)
