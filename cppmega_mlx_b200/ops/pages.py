@@ -22,7 +22,7 @@ import struct
 import torch
 
 from . import _backend as B
-from .window_attention import Plans, _raw_stream, entry, meta, on_device
+from .window_attention import Plans, _raw_stream, entry, int32, meta, on_device
 
 MAX_POOLS = 32          # of one launch
 MAX_PAIRS = 65535
@@ -120,10 +120,7 @@ def copy_pages(pools, src, dst) -> None:
             B.report(bad)
         return
     with on_device(dev):
-        if src.dtype != torch.int32 or src.device != dev or not src.is_contiguous():
-            src = src.to(dev, torch.int32, non_blocking=True).contiguous()
-        if dst.dtype != torch.int32 or dst.device != dev or not dst.is_contiguous():
-            dst = dst.to(dev, torch.int32, non_blocking=True).contiguous()
+        src, dst = int32(src), int32(dst)
         packed = [_POOL.pack(p.data_ptr(), *x) for p, x in zip(pools, shapes) if x is not None]
         fn = entry("cmb_copy_pages", ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                    ctypes.c_void_p)
@@ -207,8 +204,7 @@ def compact_rows(pools, table, start, path, counts) -> None:
             B.report(bad)
         return
     with on_device(dev):
-        table, start, path, counts = (x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
-                                      for x in (table, start, path, counts))
+        table, start, path, counts = int32(table), int32(start), int32(path), int32(counts)
         packed = [_POOL.pack(p.data_ptr(), *x) for p, x in zip(pools, shapes)]
         fn = entry("cmb_compact_rows", ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                    ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p)

@@ -269,9 +269,18 @@ def launch_forward(plan: ForwardPlan, q, k, v, lengths, tree, table, sinks, want
     return out, lse
 
 
+_INT32 = torch.iinfo(torch.int32)
+
+
+def int32(x: torch.Tensor) -> torch.Tensor:
+    """Indexes as the kernels read them: dense int32.  What does not fit becomes the nearest value that does, which no pool, table or cache
+    holds either: it is reported, and never cut to an index that happens to exist."""
+    return (x if x.dtype == torch.int32 else x.clamp(_INT32.min, _INT32.max).to(torch.int32)).contiguous()
+
+
 def converted(plan: ForwardPlan, lengths, table, sinks):
     a, b, c = plan.convert
-    return (lengths.to(torch.int32).contiguous() if a else lengths, table.to(torch.int32).contiguous() if b else table,
+    return (int32(lengths) if a else lengths, int32(table) if b else table,
             (sinks if sinks.dtype == torch.bfloat16 else sinks.float()).contiguous() if c else sinks)     # bf16 stays: the call says so
 
 

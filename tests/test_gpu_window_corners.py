@@ -178,3 +178,33 @@ def test_host_indexes_are_the_caller_s_again_when_the_call_returns():
     _done()
     want[9] = want[5]
     assert torch.equal(pool, want)
+
+
+@pytest.mark.parametrize("far", [2 ** 32 + 3, -2 ** 32 + 3, 2 ** 31 + 1, 2 ** 40])
+def test_indexes_past_32_bits_are_reported(far):
+    """64-bit indexes are not cut to a page, a length or a row that happens to exist."""
+    from cppmega_mlx_b200 import ops
+    pool = torch.randn(8, 2, 8, 1, 8, device="cuda").to(BF)
+    keep = pool.clone()
+    t = lambda *x: torch.tensor(x, device="cuda")  # noqa: E731
+    for src, dst in ((t(far), t(1)), (t(1), t(far))):
+        ops.copy_pages(pool, src, dst)
+        _reported()
+        assert torch.equal(pool, keep)
+    table = t([0, 1, 2, 3])
+    bad = table.clone()
+    bad[0, 0] = far
+    for args in ((bad, t(1), t([2]), t(1)), (table, t(far), t([2]), t(1)), (table, t(1), t([far]), t(1)), (table, t(1), t([2]), t(far))):
+        ops.compact_rows(pool, *args)
+        _reported()
+        pool.copy_(keep)
+    q = _rand(1, 1, 2, 8)
+    for tbl, n in ((bad, t(5)), (table, t(far))):
+        ops.cached_attention(q, pool[:, 0], pool[:, 1], tbl, n)
+        _reported()
+    k = _rand(1, 20, 2, 8)
+    ops.window_attention(q, k, k, key_lengths=t(far))
+    _reported()
+    ops.copy_pages(pool, t(-1, 3), t(-1, 5))                 # an unused place stays one
+    _done()
+    assert torch.equal(pool[5], keep[3])
