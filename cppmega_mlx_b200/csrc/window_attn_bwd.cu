@@ -420,13 +420,15 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   if (*abort_flag) {
     for (int i = 0; i < 64; ++i) __nanosleep(2000);
   }
-  if (MODE == WB_DQ) asm volatile("griddepcontrol.wait;" ::: "memory");      // done is done for DKV too: what follows reads both
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
+  // Done is done for DKV too: what follows reads both.  This wait comes when the TMEM is back, because a DKV block that shares the SM
+  // may still be waiting for it (every block of this DKV is on an SM by now, so the wait needs nothing that this block holds).
+  if (MODE == WB_DQ) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Row statistics for the kernel above: stats[b, hk, s, hg] = (lse log2 e, do.o).  16 lanes to a row (8 columns each).

@@ -208,3 +208,30 @@ def test_indexes_past_32_bits_are_reported(far):
     ops.copy_pages(pool, t(-1, 3), t(-1, 5))                 # an unused place stays one
     _done()
     assert torch.equal(pool[5], keep[3])
+
+
+@pytest.mark.parametrize("d,logits", [(64, False), (64, True), (32, True), (128, False)])
+def test_backwards_side_by_side(d, logits):
+    """A block that waits for the key gradients' blocks holds no tensor memory that one of them, or of another stream's, may still need."""
+    from cppmega_mlx_b200 import ops
+    sides, work = [torch.cuda.Stream() for _ in range(3)], []
+    for i in range(3):
+        s = 1200 + 333 * i
+        leaves = [_rand(1, s, n, d, seed=10 * i + j).requires_grad_() for j, n in enumerate((8, 4, 4))]
+        if logits:
+            leaves.append(_rand(8, seed=10 * i + 5).requires_grad_())
+        do = _rand(1, s, 8, d, seed=10 * i + 4)
+        o = ops.window_attention(*leaves[:3], window=300, sink_tokens=4, sinks=leaves[3] if logits else None)
+        work.append((o, leaves, do, torch.autograd.grad(o, leaves, do, retain_graph=True)))
+    _done()
+    for side in sides:
+        side.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        got = []
+        for side, (o, leaves, do, _) in zip(sides, work):
+            with torch.cuda.stream(side):
+                got.append([x.clone() for x in torch.autograd.grad(o, leaves, do, retain_graph=True)])
+        for side in sides:
+            side.synchronize()
+        assert all(torch.equal(a, b) for g, (_, _, _, want) in zip(got, work) for a, b in zip(g, want))
+    _done()
