@@ -217,6 +217,13 @@ def dense_attention(q, k, v, mask=None, scale=None, sinks=None, is_causal=False)
     return sdpa_reference(q, k, v, mask, scale, sinks)
 
 
+def flat_sinks(sinks: torch.Tensor | None) -> torch.Tensor | None:
+    """Sink logits as the operators take them, [H] of a floating type, from any shape with one logit per head and any type."""
+    if sinks is None:
+        return None
+    return (sinks if sinks.is_floating_point() else sinks.float()).reshape(-1)
+
+
 class CausalSelfAttention(nn.Module):
     def __init__(self, config: AttentionConfig):
         super().__init__()
@@ -291,6 +298,7 @@ class CausalSelfAttention(nn.Module):
                 layer_idx: int = 0, sinks: torch.Tensor | None = None) -> torch.Tensor:
         c = self.config
         b, s, _ = hidden_states.shape
+        sinks = flat_sinks(sinks)
         if getattr(kv_cache, "static", False):
             if s != 1 or isinstance(mask, torch.Tensor) or (sinks is not None and c.mode == "dsa"):
                 raise ValueError("a static decode cache serves one-token steps without an explicit mask (nor, in mode 'dsa', sinks)")

@@ -235,3 +235,21 @@ def test_backwards_side_by_side(d, logits):
             side.synchronize()
         assert all(torch.equal(a, b) for g, (_, _, _, want) in zip(got, work) for a, b in zip(g, want))
     _done()
+
+
+def test_layer_takes_sinks_of_any_shape_and_type():
+    from cppmega_mlx_b200.nn.attention import AttentionConfig, CausalSelfAttention
+    from cppmega_mlx_b200.ops import _backend as B
+    torch.manual_seed(0)
+    m = CausalSelfAttention(AttentionConfig(128, 4, num_kv_heads=2, mode="gqa")).cuda().to(BF).eval()
+    x, sinks = _rand(2, 70, 128, seed=1), torch.tensor([1, -2, 0, 3], device="cuda")
+    with torch.no_grad():
+        want = m(x, sinks=sinks.float())
+        before = B.launch_count("window_fwd")
+        for other in (sinks, sinks.view(1, 4, 1, 1), sinks.to(BF).view(2, 2)):
+            assert torch.equal(m(x, sinks=other), want)
+        assert B.launch_count("window_fwd") == before + 3
+    leaf = sinks.float().view(1, 4, 1, 1).requires_grad_()
+    m(x, sinks=leaf).float().square().sum().backward()
+    assert leaf.grad.shape == leaf.shape and float(leaf.grad.abs().min()) > 0
+    _done()

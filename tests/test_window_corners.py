@@ -116,3 +116,20 @@ def test_plain_cached_attention_stays_inside_the_pool():
             ops.cached_attention(q, k, k, table, torch.tensor(lens))
     with pytest.raises(ValueError, match="page"):
         ops.cached_attention(q, k[:0], k[:0], table, n)
+
+
+@pytest.mark.parametrize("shape", [(4,), (1, 4, 1, 1), (4, 1), (2, 2)])
+def test_layer_takes_sinks_of_any_shape(shape):
+    from cppmega_mlx_b200.nn.attention import AttentionConfig, CausalSelfAttention, flat_sinks
+    torch.manual_seed(0)
+    m = CausalSelfAttention(AttentionConfig(32, 4, num_kv_heads=2, mode="gqa", sliding_window=5)).eval()
+    x, sinks = torch.randn(2, 9, 32), torch.randn(4)
+    with torch.no_grad():
+        want = m(x, sinks=sinks)
+        assert torch.equal(m(x, sinks=sinks.view(shape)), want)
+        cache = I.StaticDecodeCache(1, 2, 16, "cpu")
+        for i in range(9):
+            y = m(x[:, i:i + 1], kv_cache=cache, sinks=sinks.view(shape))
+            cache.advance()
+            torch.testing.assert_close(y[:, 0], want[:, i], rtol=1e-4, atol=1e-5)
+    assert flat_sinks(None) is None and flat_sinks(torch.ones(2, 2, dtype=torch.int64)).dtype == torch.float32
