@@ -22,7 +22,7 @@ import struct
 import torch
 
 from . import _backend as B
-from .window_attention import Plans, _raw_stream, entry, int32, meta, on_device
+from .window_attention import Plans, _raw_stream, entry, has_tangent, int32, meta, on_device
 
 MAX_POOLS = 32          # of one launch
 MAX_PAIRS = 65535
@@ -46,7 +46,7 @@ def _check_pools(pools, rank: int, what: str) -> None:
 
 
 def _check_grad(pools, what: str) -> None:
-    if torch.is_grad_enabled() and any(p.requires_grad for p in pools):
+    if (torch.is_grad_enabled() and any(p.requires_grad for p in pools)) or has_tangent(*pools):
         raise ValueError(f"{what}: pools are written in place and cannot require a gradient")
 
 

@@ -13,7 +13,8 @@ A key that no query sees may hold anything (NaN included) and gets zero gradient
 
 CUDA bf16 tensors whose head sizes are multiples of 8 up to 128 run ``csrc/window_attn.cu`` and ``csrc/window_attn_bwd.cu``
 (tcgen05; work and memory proportional to the visible pairs, no S x T tensor, no atomics: results do not depend on the order
-in which thread blocks run).  Everything else uses ``window_attention_reference``, which is also the test oracle.  The module
+in which thread blocks run).  Everything else, forward-mode derivatives among it, uses ``window_attention_reference``, which is also the
+test oracle.  The module
 form is ``nn.attention.CausalSelfAttention`` (``sliding_window``, ``sink_tokens``); single tokens and drafted tokens over a cache:
 ``ops.cached_attention``.  Window semantics: ``cppmega_mlx/nn/attention.py:214-248``.
 """
@@ -26,6 +27,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _backend as B
 
@@ -175,6 +177,11 @@ def sink_split(s: int, t: int, window: int, sink_tokens: int, g: int) -> tuple[i
 def meta(t):
     """What a call's preparation depends on of a tensor: nothing of its address or contents."""
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether forward-mode differentiation runs through any of them: the kernels would lose the tangent without a word."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class Plans:
@@ -364,7 +371,7 @@ def window_attention(q, k, v, *, window: int | None = None, sink_tokens: int = 0
     plan = _plans.get((meta(q), meta(k), meta(v), meta(sinks), meta(key_lengths), window, sink_tokens, scale),
                       _plan, q, k, v, window, sink_tokens, sinks, key_lengths, scale)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (sinks is not None and sinks.requires_grad))
-    if not plan.covered or not B.kernels_enabled() or (grad and q.shape[2] // k.shape[2] > MAX_GROUP_GRAD):
+    if not plan.covered or not B.kernels_enabled() or (grad and q.shape[2] // k.shape[2] > MAX_GROUP_GRAD) or has_tangent(q, k, v, sinks):
         return window_attention_reference(q, k, v, window=window, sink_tokens=sink_tokens, sinks=sinks, key_lengths=key_lengths, scale=scale)
     if not plan.ready or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
         return window_attention(in_place(q), in_place(k), in_place(v), window=window, sink_tokens=sink_tokens, sinks=sinks,

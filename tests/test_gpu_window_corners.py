@@ -253,3 +253,23 @@ def test_layer_takes_sinks_of_any_shape_and_type():
     m(x, sinks=leaf).float().square().sum().backward()
     assert leaf.grad.shape == leaf.shape and float(leaf.grad.abs().min()) > 0
     _done()
+
+
+def test_forward_mode_derivatives():
+    """Tangents pass through the plain form, with or without gradients wanted beside them; a cache has none and says so."""
+    from torch.autograd import forward_ad as F
+
+    from cppmega_mlx_b200 import ops
+    q, k, v, dk = _rand(1, 20, 4, 64, seed=1), _rand(1, 20, 2, 64, seed=2), _rand(1, 20, 2, 64, seed=3), _rand(1, 20, 2, 64, seed=4)
+    f = lambda x: ops.window_attention_reference(q, x, v, window=7, sink_tokens=1)  # noqa: E731
+    want = torch.func.jvp(f, (k,), (dk,))[1]
+    assert float(want.abs().max()) > 0.01
+    for grad in (False, True):
+        with F.dual_level():
+            o = ops.window_attention(q.detach().requires_grad_(grad), F.make_dual(k, dk), v, window=7, sink_tokens=1)
+            assert torch.equal(F.unpack_dual(o).tangent.detach(), want)
+            with torch.no_grad(), pytest.raises(ValueError, match="no gradient"):
+                ops.cached_attention(q, F.make_dual(k, dk), v, None, torch.zeros(1, dtype=torch.int32, device="cuda"))
+            with pytest.raises(ValueError, match="gradient"):
+                ops.copy_pages(F.make_dual(k[0], dk[0]), [0], [1])
+    _done()
