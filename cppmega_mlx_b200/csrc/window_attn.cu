@@ -112,18 +112,19 @@ __device__ __forceinline__ WindowRow window_row(const WindowParams& p, int r, in
   w.plim = min(w.p, klim - 1);
   if (w.ok && p.tree != nullptr) {
     const unsigned long long* tree = p.tree + static_cast<long long>(b) * p.tree_sb;
-    const unsigned long long word = tree[w.s];
+    const unsigned long long places = p.S < 64 ? (1ull << p.S) - 1ull : ~0ull;      // bits past the last node say nothing
+    const unsigned long long word = tree[w.s] & places;
     const int depth = __popcll(word) - 1;
     w.ok = word != 0ull;
     w.p = prefix + depth;
     w.plim = prefix - 1;
-    w.nodes = p.S < 64 ? word & ((1ull << p.S) - 1ull) : word;
+    w.nodes = word;
     if (p.window <= depth) {                 // the window ends inside the drafted nodes
       unsigned long long left = w.nodes;
       while (left) {
         const int m = __ffsll(static_cast<long long>(left)) - 1;
         left &= left - 1ull;
-        const int dm = __popcll(tree[m]) - 1;
+        const int dm = __popcll(tree[m] & places) - 1;
         if (!(depth - dm < p.window || prefix + dm < p.ns)) w.nodes &= ~(1ull << m);
       }
     }

@@ -9,7 +9,7 @@ or a single next token; with an optional sliding window and first tokens that st
 * contiguous: ``table is None`` and the views are ``[B, T, kv_heads, D]``.
 
 ``tree`` [N] (one for the batch) or [B, N] int64, N <= 64: bit m of word n is set where token n sees token m — itself and its
-ancestors (``tree_words``).  Token n then stands at position ``prefix + (bits of word n) - 1``, a token whose word is 0 is padding
+ancestors (``tree_words``); bits from N on say nothing.  Token n then stands at position ``prefix + (bits of word n) - 1``, a token whose word is 0 is padding
 and yields zeros.  ``tree is None``: a chain, token n sees all tokens up to itself (any N).  Every token sees the sequence's
 prefix.  ``window`` and ``sink_tokens`` restrict both by position: a key at position j is seen from position P when ``P - j < window``
 or ``j < sink_tokens``.  ``sinks`` [H]: one more key per head with that logit and value 0.

@@ -273,3 +273,21 @@ def test_forward_mode_derivatives():
             with pytest.raises(ValueError, match="gradient"):
                 ops.copy_pages(F.make_dual(k[0], dk[0]), [0], [1])
     _done()
+
+
+@pytest.mark.parametrize("n", [1, 5, 31, 63])
+@pytest.mark.parametrize("window", [None, 2])
+def test_bits_past_the_last_token_say_nothing(n, window):
+    from cppmega_mlx_b200 import ops
+    par = [(i - 1) // 2 for i in range(n)]
+    par[-1] = -2 if n > 1 else -1
+    tree = ops.tree_words(par).cuda()
+    q, k, v = _rand(2, n, 4, 64, seed=1), _rand(2, 200, 2, 64, seed=2), _rand(2, 200, 2, 64, seed=3)
+    lens = torch.tensor([100, 0], dtype=torch.int32, device="cuda")
+    want = ops.cached_attention(q, k, v, None, lens, tree=tree, window=window)
+    stray = tree | (-1 << n)                                     # every bit from n on
+    got = ops.cached_attention(q, k, v, None, lens, tree=stray, window=window)
+    _done()
+    assert torch.equal(got, want)
+    plain = ops.cached_attention_reference(q, k, v, None, lens, tree=stray, window=window)
+    assert torch.equal(plain, ops.cached_attention_reference(q, k, v, None, lens, tree=tree, window=window))
