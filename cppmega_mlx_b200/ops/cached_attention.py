@@ -18,9 +18,10 @@ What no token sees — rows past a sequence's end, table entries past them, page
 entry or a length that the pool or the table cannot hold is reported by ``ops.check_status`` (nothing is read outside the pool); with
 CPU tensors it is a ``ValueError``.
 
-CUDA bf16 tensors run ``csrc/window_attn.cu`` (tcgen05, split over the keys when there are few rows); page sizes that are not a
-multiple of 8, other types and CPU tensors use ``cached_attention_reference``, the test oracle.  No gradients: inputs that require
-one are refused.  The reference verifies drafts as a plain chain (``cppmega_mlx/inference/speculative_decode.py:92``) and never attends
+CUDA bf16 tensors run ``csrc/window_attn.cu`` (tcgen05, split over the keys when there are few rows).  CPU tensors, other types, heads that
+are not a multiple of 8 or larger than 128, page sizes that are not a multiple of 8, and cache rows whose address or strides are not
+multiples of 16 bytes use ``cached_attention_reference``, the test oracle, which gathers every sequence's whole capacity in fp32.  No gradients,
+neither mode: inputs that require one are refused.  The reference verifies drafts as a plain chain (``cppmega_mlx/inference/speculative_decode.py:92``) and never attends
 over its pages (``cppmega_mlx/inference/serving.py:522``).
 """
 from __future__ import annotations
@@ -125,7 +126,7 @@ def _plan(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, s
     rows = k_rows.shape[1]
     t = rows * (1 if table is None else table.shape[1])
     if (not _sizes_covered(q, k_rows, v_rows) or not (usable(k_rows) and usable(v_rows)) or 0 in q.shape[:2] or not q.shape[1] <= t <= NO_WINDOW // 2
-            or (table is not None and (rows % 8 or not k_rows.shape[0])) or (tree is not None and not tree.is_contiguous())):
+            or (table is not None and (rows % 8 or not k_rows.shape[0]))):
         return ForwardPlan(False, False, scale)
     if not usable(q):
         return ForwardPlan(True, False, scale)
@@ -138,13 +139,15 @@ def cached_attention(q, k_rows, v_rows, table, prefix_lengths, *, tree: torch.Te
                      max_keys: int | None = None) -> torch.Tensor:
     """See the module docstring; returns [B, N, H, Dv] in ``q.dtype``.  ``max_keys`` (a bound on ``prefix_lengths + N``) only tunes how
     the work is split and never costs correctness."""
+    if tree is not None:
+        tree = tree.contiguous()
     plan = _plans.get((meta(q), meta(k_rows), meta(v_rows), meta(table), meta(prefix_lengths), meta(tree), meta(sinks), window, sink_tokens, scale,
                        max_keys), _plan, q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens, sinks, scale, max_keys)
     _no_gradient(q, k_rows, v_rows, sinks)
     if q.shape[0] == 0 or q.shape[1] == 0:
         return q.new_zeros(*q.shape[:3], v_rows.shape[3])
     if not plan.covered or not B.kernels_enabled() or (k_rows.data_ptr() | v_rows.data_ptr()) % 16:
-        return cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, tree=None if tree is None else tree.contiguous(),
+        return cached_attention_reference(q, k_rows, v_rows, table, prefix_lengths, tree=tree,
                                           window=window, sink_tokens=sink_tokens, sinks=sinks, scale=scale)
     if not plan.ready or q.data_ptr() % 16:
         return cached_attention(in_place(q), k_rows, v_rows, table, prefix_lengths, tree=tree, window=window, sink_tokens=sink_tokens,

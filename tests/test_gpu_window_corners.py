@@ -291,3 +291,19 @@ def test_bits_past_the_last_token_say_nothing(n, window):
     assert torch.equal(got, want)
     plain = ops.cached_attention_reference(q, k, v, None, lens, tree=stray, window=window)
     assert torch.equal(plain, ops.cached_attention_reference(q, k, v, None, lens, tree=tree, window=window))
+
+
+def test_trees_of_any_layout_run_the_kernel():
+    from cppmega_mlx_b200 import ops
+    from cppmega_mlx_b200.ops import _backend as B
+    tree = ops.tree_words([[-1, 0, 0, 2, 2], [-1, -1, 1, 1, 0]]).cuda()
+    q, k, v = _rand(2, 5, 4, 64, seed=1), _rand(2, 200, 2, 64, seed=2), _rand(2, 200, 2, 64, seed=3)
+    lens = torch.tensor([100, 9], dtype=torch.int32, device="cuda")
+    wide = torch.zeros(2, 9, dtype=torch.int64, device="cuda")
+    wide[:, 2:7] = tree
+    for same, other in ((tree, wide[:, 2:7]), (tree, tree.t().contiguous().t()), (tree[:1].repeat(2, 1), tree[:1].expand(2, 5)), (tree[1], wide[1, 2:7])):
+        want = ops.cached_attention(q, k, v, None, lens, tree=same)
+        before = B.launch_count("window_fwd")
+        assert torch.equal(ops.cached_attention(q, k, v, None, lens, tree=other), want)
+        assert B.launch_count("window_fwd") == before + 1
+    _done()
