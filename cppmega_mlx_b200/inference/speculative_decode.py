@@ -71,13 +71,18 @@ def greedy_tree_accept(parents, draft_tokens, target_tokens) -> tuple[list[int],
     par, tok, want = (torch.as_tensor(x).tolist() for x in (parents, draft_tokens, target_tokens))
     if len(tok) != len(par) or len(want) != len(par) + 1:
         raise ValueError("parents and draft_tokens must have N entries and target_tokens N + 1")
-    path, at = [], -1
-    while True:
-        nxt = next((n for n, m in enumerate(par) if m == at and n > at and tok[n] == want[at + 1]), None)
-        if nxt is None:
-            return path, want[at + 1]
-        path.append(nxt)
-        at = nxt
+    depth = [0] * len(par)          # tokens of the path that ends here, 0 where the target does not follow it
+    for n, m in enumerate(par):     # (parents stand before their children; siblings may draft the same token)
+        if -1 <= m < n and tok[n] == want[m + 1] and (m < 0 or depth[m]):
+            depth[n] = 1 + (depth[m] if m >= 0 else 0)
+    at = max(range(len(par)), key=depth.__getitem__, default=-1)
+    if at < 0 or not depth[at]:
+        return [], want[0]
+    path, last = [], at
+    while at >= 0:
+        path.append(at)
+        at = par[at]
+    return path[::-1], want[last + 1]
 
 
 def batched_leviathan_accept(draft_tokens, draft_probs, target_probs, *, generator=None, pad: int = -1):

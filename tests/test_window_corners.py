@@ -133,3 +133,13 @@ def test_layer_takes_sinks_of_any_shape(shape):
             cache.advance()
             torch.testing.assert_close(y[:, 0], want[:, i], rtol=1e-4, atol=1e-5)
     assert flat_sinks(None) is None and flat_sinks(torch.ones(2, 2, dtype=torch.int64)).dtype == torch.float32
+
+
+def test_greedy_tree_accept_among_equal_siblings():
+    """Two drafts of one token: the path goes on where it is longest."""
+    par, tok = [-1, -1, 1, 0, 2], [5, 5, 7, 8, 9]
+    assert I.greedy_tree_accept(par, tok, [5, 7, 7, 9, 0, 4]) == ([1, 2, 4], 4)
+    assert I.greedy_tree_accept(par, tok, [5, 8, 8, 9, 1, 4]) == ([0, 3], 1)
+    assert I.greedy_tree_accept([-1, -1], [5, 5], [5, 6, 6]) == ([0], 6)            # the first of equally long ones
+    assert I.greedy_tree_accept([-1, -2, 0], [5, 5, 6], [5, 6, 0, 3]) == ([0, 2], 3)
+    assert I.greedy_tree_accept([], [], [8]) == ([], 8)
