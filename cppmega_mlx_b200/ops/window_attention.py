@@ -13,8 +13,8 @@ A key that no query sees may hold anything (NaN included) and gets zero gradient
 
 CUDA bf16 tensors whose head sizes are multiples of 8 up to 128 run ``csrc/window_attn.cu`` and ``csrc/window_attn_bwd.cu``
 (tcgen05; work and memory proportional to the visible pairs, no S x T tensor, no atomics: results do not depend on the order
-in which thread blocks run).  Everything else, forward-mode derivatives among it, uses ``window_attention_reference``, which is also the
-test oracle.  The module
+in which thread blocks run).  Everything else, forward-mode derivatives and gradients with ``create_graph`` among it, uses
+``window_attention_reference``, which is also the test oracle.  The module
 form is ``nn.attention.CausalSelfAttention`` (``sliding_window``, ``sink_tokens``); single tokens and drafted tokens over a cache:
 ``ops.cached_attention``.  Window semantics: ``cppmega_mlx/nn/attention.py:214-248``.
 """
@@ -318,11 +318,17 @@ class _WindowAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, sinks, lengths, out, lse = ctx.saved_tensors
         plan = ctx.plan
         need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
+        if torch.is_grad_enabled():        # gradients that are differentiated again (create_graph): the plain form's
+            need = (need_q, need_k, need_v, need_s)
+            # (each input as a tensor of its own: one that is used twice gets each use's part)
+            own = [None if t is None else t.view_as(t) for t in (q, k, v, sinks)]
+            o = window_attention_reference(*own[:3], window=plan.window, sink_tokens=plan.sink_tokens, sinks=own[3], key_lengths=lengths, scale=plan.scale)
+            grads = iter(torch.autograd.grad(o, [t for t, n in zip(own, need) if n], do, create_graph=True))
+            return *(next(grads) if n else None for n in need), None, None
         need_kv = need_k or need_v
         do = in_place(do)
         dev = q.device

@@ -307,3 +307,20 @@ def test_trees_of_any_layout_run_the_kernel():
         assert torch.equal(ops.cached_attention(q, k, v, None, lens, tree=other), want)
         assert B.launch_count("window_fwd") == before + 1
     _done()
+
+
+def test_second_derivatives():
+    """A layer's sink logits had them before there was a kernel: they come from the plain form, the first ones that carry a graph too."""
+    from cppmega_mlx_b200 import ops
+    leaves = [_rand(1, 20, n, 64, seed=n).requires_grad_() for n in (4, 2)] + [_rand(1, 20, 2, 64, seed=9).requires_grad_(), _rand(4, seed=7).requires_grad_()]
+    do, dd = _rand(1, 20, 4, 64, seed=8).requires_grad_(), _rand(1, 20, 2, 64, seed=6)
+    res = []
+    for f in (ops.window_attention, ops.window_attention_reference):
+        o = f(*leaves[:3], window=7, sink_tokens=1, sinks=leaves[3])
+        first = torch.autograd.grad(o, leaves, do, create_graph=True)
+        res.append([*first, *torch.autograd.grad((first[1] * dd).float().sum() + first[3].float().sum(), [*leaves, do])])
+    _done()
+    assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(*res))
+    x = leaves[1]                                                 # one tensor as keys and as values: each use counts once
+    got, want = (torch.autograd.grad(f(leaves[0], x, x, window=7), x, do.detach(), create_graph=True)[0] for f in (ops.window_attention, ops.window_attention_reference))
+    assert torch.equal(got, want)
