@@ -336,7 +336,7 @@ class CausalSelfAttention(nn.Module):
                 lengths = torch.full((b,), klen, dtype=torch.int32, device=q.device)
                 out = DA.decode_attention(q[:, 0], k, v, None, lengths, scale=c.q_head_dim ** -0.5, max_keys=klen)
                 return self._out(out.reshape(b, s, c.q_proj_dim))
-        if plain_causal and (c.sliding_window is not None or sinks is not None) and kernel_covers(q, k, v):
+        if plain_causal and (c.sliding_window is not None or sinks is not None) and kernel_covers(q, k, v, sinks):
             # the window's kernel (training, prompts and single tokens alike): work and memory go by the visible pairs
             out = ops.window_attention(q, k, v, window=c.sliding_window, sink_tokens=c.sink_tokens, sinks=sinks)
             return self._out(out.reshape(b, s, c.q_proj_dim))

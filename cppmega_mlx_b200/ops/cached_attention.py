@@ -29,8 +29,8 @@ from __future__ import annotations
 import torch
 
 from . import _backend as B
-from .window_attention import (NO_WINDOW, ForwardPlan, Plans, _check, _check_lengths, _sizes_covered, converted, has_tangent, in_place,
-                               launch_forward, masked_softmax_attention, meta, on_device, plan_forward, usable)
+from .window_attention import (NO_WINDOW, ForwardPlan, Plans, _check, _check_lengths, _sizes_covered, _wants_grad, converted,
+                               has_tangent, in_place, launch_forward, masked_softmax_attention, meta, on_device, plan_forward, usable)
 
 MAX_TREE = 64
 
@@ -72,8 +72,7 @@ def _checked(q, k_rows, v_rows, table, prefix_lengths, tree, window, sink_tokens
 
 
 def _no_gradient(q, k_rows, v_rows, sinks) -> None:
-    grad = torch.is_grad_enabled() and (q.requires_grad or k_rows.requires_grad or v_rows.requires_grad or (sinks is not None and sinks.requires_grad))
-    if grad or has_tangent(q, k_rows, v_rows, sinks):
+    if _wants_grad(q, k_rows, v_rows, sinks) or has_tangent(q, k_rows, v_rows, sinks):
         raise ValueError("cached_attention has no gradient: call it under torch.no_grad(), or use window_attention")
 
 

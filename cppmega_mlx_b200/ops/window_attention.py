@@ -142,9 +142,13 @@ def strides3(t: torch.Tensor) -> tuple[int, int, int]:
     return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3]))
 
 
-def kernel_covers(q, k, v) -> bool:
-    """Types, head sizes and devices of the kernels (layouts apart)."""
-    return B.on_gpu(q, k, v) and _sizes_covered(q, k, v)
+def kernel_covers(q, k, v, sinks=None) -> bool:
+    """Types, head sizes, groups and devices of the kernels (layouts apart), with the backward where gradients are wanted."""
+    return B.on_gpu(q, k, v) and _sizes_covered(q, k, v) and (q.shape[2] // k.shape[2] <= MAX_GROUP_GRAD or not _wants_grad(q, k, v, sinks))
+
+
+def _wants_grad(q, k, v, sinks) -> bool:
+    return torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (sinks is not None and sinks.requires_grad))
 
 
 def _sizes_covered(q, k, v) -> bool:
@@ -376,7 +380,7 @@ def window_attention(q, k, v, *, window: int | None = None, sink_tokens: int = 0
     """See the module docstring; returns [B, S, H, Dv] in ``q.dtype``."""
     plan = _plans.get((meta(q), meta(k), meta(v), meta(sinks), meta(key_lengths), window, sink_tokens, scale),
                       _plan, q, k, v, window, sink_tokens, sinks, key_lengths, scale)
-    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (sinks is not None and sinks.requires_grad))
+    grad = _wants_grad(q, k, v, sinks)
     if not plan.covered or not B.kernels_enabled() or (grad and q.shape[2] // k.shape[2] > MAX_GROUP_GRAD) or has_tangent(q, k, v, sinks):
         return window_attention_reference(q, k, v, window=window, sink_tokens=sink_tokens, sinks=sinks, key_lengths=key_lengths, scale=scale)
     if not plan.ready or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:

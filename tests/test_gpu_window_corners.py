@@ -324,3 +324,21 @@ def test_second_derivatives():
     x = leaves[1]                                                 # one tensor as keys and as values: each use counts once
     got, want = (torch.autograd.grad(f(leaves[0], x, x, window=7), x, do.detach(), create_graph=True)[0] for f in (ops.window_attention, ops.window_attention_reference))
     assert torch.equal(got, want)
+
+
+def test_layers_whose_groups_the_backward_does_not_take_train_as_before(monkeypatch):
+    """Groups of more than 64 heads: the library's attention under a window, not the fp32 form of every pair."""
+    from cppmega_mlx_b200 import ops
+    from cppmega_mlx_b200.nn import attention as A
+    torch.manual_seed(0)
+    m = A.CausalSelfAttention(A.AttentionConfig(65 * 16, 65, num_kv_heads=1, mode="gqa", sliding_window=20)).cuda().to(BF)
+    x = _rand(1, 50, 65 * 16, seed=1)
+    asked = []
+    real = ops.window_attention
+    monkeypatch.setattr(ops, "window_attention", lambda *a, **kw: asked.append(1) or real(*a, **kw))
+    m(x).float().sum().backward()
+    assert not asked and all(p.grad is not None for p in m.parameters())
+    with torch.no_grad():
+        m(x)
+    assert len(asked) == 1
+    _done()
