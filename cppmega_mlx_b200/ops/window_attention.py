@@ -23,6 +23,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import numbers
 import struct
 from typing import NamedTuple
 
@@ -55,16 +56,17 @@ def _check(q, k, v, window, sink_tokens, sinks, scale, what: str) -> float:
         raise ValueError(f"{what}: {q.shape[2]} query heads are not a multiple of {k.shape[2]} key heads")
     if q.shape[3] == 0 or v.shape[3] == 0:
         raise ValueError(f"{what}: head sizes must be positive")
-    if window is not None and window < 1:
-        raise ValueError(f"{what}: window must be positive, got {window}")
-    if sink_tokens < 0:
-        raise ValueError(f"{what}: sink_tokens must not be negative, got {sink_tokens}")
+    # plain numbers only: prepared calls are found by their options' values, and a tensor's may change
+    if window is not None and (not isinstance(window, numbers.Integral) or window < 1):
+        raise ValueError(f"{what}: window must be positive and whole, got {window}")
+    if not isinstance(sink_tokens, numbers.Integral) or sink_tokens < 0:
+        raise ValueError(f"{what}: sink_tokens must be whole and not negative, got {sink_tokens}")
     if sinks is not None and (sinks.shape != (q.shape[2],) or sinks.device != q.device or not sinks.is_floating_point()):
         raise ValueError(f"{what}: sinks must be {q.shape[2]} logits on {q.device}, got {tuple(sinks.shape)} on {sinks.device}")
-    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
-    return scale
+    scale = q.shape[3] ** -0.5 if scale is None else scale
+    if not (isinstance(scale, numbers.Real) and scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"{what}: scale must be a positive and finite number, got {scale}")
+    return float(scale)
 
 
 def _check_lengths(n, batch: int, device, what: str) -> None:

@@ -143,3 +143,21 @@ def test_greedy_tree_accept_among_equal_siblings():
     assert I.greedy_tree_accept([-1, -1], [5, 5], [5, 6, 6]) == ([0], 6)            # the first of equally long ones
     assert I.greedy_tree_accept([-1, -2, 0], [5, 5, 6], [5, 6, 0, 3]) == ([0, 2], 3)
     assert I.greedy_tree_accept([], [], [8]) == ([], 8)
+
+
+@pytest.mark.parametrize("change,match", [(dict(window=torch.tensor(3)), "window"), (dict(window=2.5), "window"), (dict(sink_tokens=1.5), "sink_tokens"),
+                                          (dict(sink_tokens=torch.tensor(1)), "sink_tokens"), (dict(scale=torch.tensor(0.5)), "scale")])
+def test_options_are_plain_numbers(change, match):
+    """Prepared calls are found by their options' values: a tensor, which is found by its identity and may change, is refused."""
+    q = torch.randn(1, 6, 2, 8)
+    with pytest.raises(ValueError, match=match):
+        ops.window_attention(q, q, q, **{"window": 3, **change})
+    with pytest.raises(ValueError, match=match):
+        ops.cached_attention(q, q, q, None, torch.zeros(1, dtype=torch.int32), **{"window": 3, **change})
+
+
+def test_numpy_numbers_are_numbers():
+    import numpy as np
+    q = torch.randn(1, 6, 2, 8)
+    assert torch.equal(ops.window_attention(q, q, q, window=np.int64(3), sink_tokens=np.int32(1), scale=np.float32(0.5)),
+                       ops.window_attention(q, q, q, window=3, sink_tokens=1, scale=0.5))
