@@ -146,7 +146,11 @@ def strides3(t: torch.Tensor) -> tuple[int, int, int]:
 
 def kernel_covers(q, k, v, sinks=None) -> bool:
     """Types, head sizes, groups and devices of the kernels (layouts apart), with the backward where gradients are wanted."""
-    return B.on_gpu(q, k, v) and _sizes_covered(q, k, v) and (q.shape[2] // k.shape[2] <= MAX_GROUP_GRAD or not _wants_grad(q, k, v, sinks))
+    return B.on_gpu(q, k, v) and _sizes_covered(q, k, v) and (_heads_covered_grad(q, k) or not _wants_grad(q, k, v, sinks))
+
+
+def _heads_covered_grad(q, k) -> bool:
+    return q.shape[2] // k.shape[2] <= MAX_GROUP_GRAD and q.shape[2] <= 65535
 
 
 def _wants_grad(q, k, v, sinks) -> bool:
@@ -383,7 +387,7 @@ def window_attention(q, k, v, *, window: int | None = None, sink_tokens: int = 0
     plan = _plans.get((meta(q), meta(k), meta(v), meta(sinks), meta(key_lengths), window, sink_tokens, scale),
                       _plan, q, k, v, window, sink_tokens, sinks, key_lengths, scale)
     grad = _wants_grad(q, k, v, sinks)
-    if not plan.covered or not B.kernels_enabled() or (grad and q.shape[2] // k.shape[2] > MAX_GROUP_GRAD) or has_tangent(q, k, v, sinks):
+    if not plan.covered or not B.kernels_enabled() or (grad and not _heads_covered_grad(q, k)) or has_tangent(q, k, v, sinks):
         return window_attention_reference(q, k, v, window=window, sink_tokens=sink_tokens, sinks=sinks, key_lengths=key_lengths, scale=scale)
     if not plan.ready or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
         return window_attention(in_place(q), in_place(k), in_place(v), window=window, sink_tokens=sink_tokens, sinks=sinks,

@@ -342,3 +342,16 @@ def test_layers_whose_groups_the_backward_does_not_take_train_as_before(monkeypa
         m(x)
     assert len(asked) == 1
     _done()
+
+
+def test_more_heads_than_a_grid_has_rows():
+    from cppmega_mlx_b200 import ops
+    h, g = 2 * 33000, 2
+    leaves = [_rand(1, 2, n, 8, seed=1 + i).requires_grad_() for i, n in enumerate((h, h // g, h // g))]
+    do = _rand(1, 2, h, 8, seed=5)
+    o = ops.window_attention(*leaves, window=2)
+    grads = torch.autograd.grad(o, leaves, do)
+    _done()
+    ref = W.attention64(*(x.detach() for x in leaves), W.visible(2, 2, 2, 0, device="cuda"), do=do)
+    for got, name in zip((o.detach(), *grads), ("o", "dq", "dk", "dv")):
+        W.check(got, ref[name], name)
