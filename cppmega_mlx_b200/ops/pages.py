@@ -189,13 +189,14 @@ def compact_rows(pools, table, start, path, counts) -> None:
     if dev.type == "cpu":
         i = torch.arange(path.shape[1])
         use = i < counts[:, None]
+        moves = use.any(1)                  # (a sequence that moves nothing may stand anywhere)
         far = torch.where(use, torch.maximum(path, i.to(path.dtype)), torch.full_like(path, -1)).amax(1) + start
-        if bool((counts < 0).any()) or bool((counts > path.shape[1]).any()) or bool((path[use] < 0).any()) or bool((start < 0).any()) or \
-                bool((far >= table.shape[1] * page).any()):
+        if bool((counts < 0).any()) or bool((counts > path.shape[1]).any()) or bool((path[use] < 0).any()) or \
+                bool((moves & ((start < 0) | (far >= table.shape[1] * page))).any()):
             raise ValueError("compact_rows: a row outside the table")
         need = torch.arange(table.shape[1]) * page <= far[:, None]
         need &= (torch.arange(table.shape[1]) + 1) * page > start[:, None]
-        need &= (counts > 0)[:, None]
+        need &= moves[:, None]
         if bool(((table < 0) | (table >= n))[need].any()):
             raise ValueError(f"compact_rows: a page outside the pool of {n}")
     if not covered or not B.kernels_enabled():

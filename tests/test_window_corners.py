@@ -161,3 +161,14 @@ def test_numpy_numbers_are_numbers():
     q = torch.randn(1, 6, 2, 8)
     assert torch.equal(ops.window_attention(q, q, q, window=np.int64(3), sink_tokens=np.int32(1), scale=np.float32(0.5)),
                        ops.window_attention(q, q, q, window=3, sink_tokens=1, scale=0.5))
+
+
+def test_sequences_that_move_nothing_may_stand_anywhere():
+    pool = torch.randn(5, 2, 4, 3)
+    keep, t = pool.clone(), torch.tensor
+    ops.compact_rows(pool, t([[-1, 99], [2, 1]]), t([-1, 0]), t([[7], [0]]), t([0, 1]))
+    ops.compact_rows(pool, t([[-1, 99], [2, 1]]), t([400, 0]), t([[7], [0]]), t([0, 1]))
+    assert torch.equal(pool, keep)
+    for start in (-1, 400):
+        with pytest.raises(ValueError):
+            ops.compact_rows(pool, t([[4, 0], [2, 1]]), t([start, 0]), t([[7], [0]]), t([1, 1]))
