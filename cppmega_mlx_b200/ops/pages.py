@@ -190,7 +190,7 @@ def compact_rows(pools, table, start, path, counts) -> None:
         i = torch.arange(path.shape[1])
         use = i < counts[:, None]
         moves = use.any(1)                  # (a sequence that moves nothing may stand anywhere)
-        far = torch.where(use, torch.maximum(path, i.to(path.dtype)), torch.full_like(path, -1)).amax(1) + start
+        far = torch.where(use, torch.maximum(path.long(), i), -1).amax(1) + start.long()
         if bool((counts < 0).any()) or bool((counts > path.shape[1]).any()) or bool((path[use] < 0).any()) or \
                 bool((moves & ((start < 0) | (far >= table.shape[1] * page))).any()):
             raise ValueError("compact_rows: a row outside the table")

@@ -172,3 +172,13 @@ def test_sequences_that_move_nothing_may_stand_anywhere():
     for start in (-1, 400):
         with pytest.raises(ValueError):
             ops.compact_rows(pool, t([[4, 0], [2, 1]]), t([start, 0]), t([[7], [0]]), t([1, 1]))
+
+
+def test_positions_past_32_bits_are_refused():
+    """int32 starts and paths whose sum does not fit: not wrapped to a position in front of the table."""
+    pool = torch.randn(5, 2, 4, 3)
+    keep = pool.clone()
+    t = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError, match="outside"):
+        ops.compact_rows(pool, t([4, 0]), t(5), t([2 ** 31 - 3]), t(1))
+    assert torch.equal(pool, keep)
