@@ -355,3 +355,32 @@ def test_more_heads_than_a_grid_has_rows():
     ref = W.attention64(*(x.detach() for x in leaves), W.visible(2, 2, 2, 0, device="cuda"), do=do)
     for got, name in zip((o.detach(), *grads), ("o", "dq", "dk", "dv")):
         W.check(got, ref[name], name)
+
+
+@pytest.mark.parametrize("s,t,g,d,window,ns,lengths", [(16, 16, 2, 64, None, 0, None), (40, 300, 3, 128, 9, 3, None), (70, 70, 1, 40, 12, 4, None),
+                                                       (33, 700, 4, 96, 13, 0, None), (20, 200, 2, 64, None, 0, [11, 16])])
+def test_rows_that_see_nine_to_sixteen_keys(s, t, g, d, window, ns, lengths):
+    """As for a handful of keys: delta comes from p and dP there, three and four rounds of four keys."""
+    from cppmega_mlx_b200 import ops
+    b = 2
+    q, k, v, do = _rand(b, s, 2 * g, d, seed=1), _rand(b, t, 2, d, seed=2), _rand(b, t, 2, d, seed=3), _rand(b, s, 2 * g, d, seed=4)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    dq, dk, _ = torch.autograd.grad(ops.window_attention(q, k, v, window=window, sink_tokens=ns, key_lengths=n), leaves, do)
+    _done()
+    q, k, v, do = (x.detach().double() for x in (q, k, v, do))
+    seen = W.visible(s, t, window, ns, n, "cuda").expand(b, s, t)
+    most = seen.sum(-1).max()
+    assert 9 <= int(most) <= 16
+    kk, vv = k.repeat_interleave(g, 2), v.repeat_interleave(g, 2)
+    p = torch.softmax((torch.einsum("bshd,bthd->bhst", q, kk) * d ** -0.5).masked_fill(~seen[:, None], float("-inf")), -1)
+    dp, dpa = torch.einsum("bshd,bthd->bhst", do, vv), torch.einsum("bshd,bthd->bhst", do.abs(), vv.abs())
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    # dS's rounding and fp32 in p, dP and delta
+    eds = (W.H + W.F32) * ds.abs() + 2 * W.F32 * p * (dpa + (p * dpa).sum(-1, keepdim=True))
+    for got, a, name in ((dq, kk, "dq"), (dk, q, "dk")):
+        eq = "bhst,bthd->bshd" if name == "dq" else "bhst,bshd->bthd"
+        value, bound = d ** -0.5 * torch.einsum(eq, ds, a), d ** -0.5 * torch.einsum(eq, eds, a.abs())
+        if name == "dk":
+            value, bound = (x.view(b, t, 2, g, d).sum(3) for x in (value, bound))
+        W.check(got, (value, (bound + W.H * (value.abs() + bound)) * 1.01 + 1e-30), name)
