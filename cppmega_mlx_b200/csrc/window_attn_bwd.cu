@@ -23,8 +23,9 @@
 // long blocks, 256 where 2 x 4096 queries meet 4 key heads, which keep 148 SMs busy for 86% of two waves.  Forward and backward of
 // that call, 16 heads of 128, a window of 1024: 414 -> 388 us; 16384 queries, a window of 2048: 1414 -> 1255 us.
 //
-// What bounds it: the tensor pipe.  A 64-wide sub-tile of DKV takes 1304 clocks of products (DQ 1044) and 1640 (1430) in all; products
-// of N = 64 with both operands in shared memory run at 70% of the full rate.
+// What bounds it: inside a sub-tile the products, 1304 of its 1640 clocks in DKV and 1044 of 1430 in DQ, because those of N = 64 with
+// both operands in shared memory run at 70% of the full rate.  Over the whole kernels the pipe multiplies 43% (37%) of the time: the rest is
+// that rate, the hand-overs, the blocks' starts and ends, and SMs on which a DQ block that is done waits for the last DKV block.
 //
 // A key that no row sees may hold anything: K rows of no row of the tile are zeroed in shared memory before dQ's product.
 #include "window_attn.h"

@@ -4,7 +4,8 @@ Modes: ``mla`` / ``full`` (dense causal SDPA), ``gqa`` (grouped KV heads), ``dsa
 through :func:`ops.sparse_mla_attention` over a shared ``sparse_kv`` projection).  Supports split-half
 RoPE (standard / llama3 / YaRN), sliding windows with visible first tokens, document masks, attention sinks and a contiguous or
 static KV cache for decode.  A window or sink logits without a mask tensor run ``ops.window_attention`` / ``ops.cached_attention`` on
-CUDA bf16.  Behavioural parity: ``cppmega_mlx/nn/attention.py:47-188`` (config),
+CUDA bf16, whose probabilities are rounded to bf16 before their product with the values, as in every tensor-core attention (the forms with
+a mask tensor keep those under sink logits in fp32).  Behavioural parity: ``cppmega_mlx/nn/attention.py:47-188`` (config),
 ``:214-248`` (mask), ``:251-284`` (recency-window indices), ``:287-360`` (mask → indices),
 ``:541-986`` (module).  The low-rank MLA + learned-indexer attention lives in ``nn/mla.py``.
 """

@@ -6,11 +6,13 @@ call and not read in the same call; a pair (-1, -1) is an unused place of the li
 
 ``compact_rows(pools, table, start, path, counts)`` moves, in every sequence b, the cached rows of tokens ``start[b] + path[b, i]`` to
 ``start[b] + i`` for ``i < counts[b]``, as if all were read before any is written: the accepted path of a drafted tree closes up
-behind the prefix.  Pools are ``[num_pages, layers, page_size, ...]`` with dense rows.
+behind the prefix.  Pools are ``[num_pages, layers, page_size, ...]`` with dense rows.  The pages that a sequence's rows move to are its own:
+no other sequence of the call reads or writes them.
 
-Both work in place on CPU and CUDA tensors of any type, one launch for all pools of a cache (``csrc/pages.cu``).  Indexes given as
-Python lists or CPU tensors are checked before anything moves; in CUDA tensors, which are never read back, what lies outside the
-pool or the table is skipped and reported by ``ops.check_status``.  ``inference.PagedKVBlockManager`` builds fork, copy on write,
+Both work in place on CPU and CUDA tensors of any type, one launch for all pools of a cache (``csrc/pages.cu``; pages or rows that are
+not dense take the plain forms).  Indexes given as Python lists or CPU tensors are checked before anything moves, and cannot be captured
+into a graph with CUDA pools; in CUDA tensors, which the kernels never read back, what lies outside the pool or the table is skipped and
+reported by ``ops.check_status``.  ``inference.PagedKVBlockManager`` builds fork, copy on write,
 acceptance and compaction of the pool on them.  The reference's manager only hands blocks out and takes them back
 (``cppmega_mlx/inference/serving.py:47-215``).
 """
