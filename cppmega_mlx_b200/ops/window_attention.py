@@ -4,8 +4,8 @@
 the last S positions of the T that the keys hold (``T == S`` in training; a prompt over a filled cache has more keys).  The query
 at position P sees key j when
 
-* ``j <= P``, and ``j < key_lengths[b]`` where lengths are given (padding at the end of a row of the batch; lengths outside 0 .. T are
-  reported by ``ops.check_status`` on CUDA and count as the nearest inside), and
+* ``j <= P``, and ``j < key_lengths[b]`` where lengths are given (padding at the end of a row of the batch; lengths outside 0 .. T
+  count as the nearest inside, and the kernel reports them through ``ops.check_status``), and
 * ``P - j < window`` (the window counts the query's own position) or ``j < sink_tokens``.
 
 ``sinks`` [H] adds, per head, one key of that logit whose value is 0 (learned sink logits).  Softmax statistics are fp32; a query
